@@ -244,7 +244,8 @@ def _plain_rope(st):
 
 def _plain_append_one(new, cache, scale, st):
     """new [B, S, Hkv, D] behind each sequence's cached tokens.  A page's scale is a power of two that holds its largest
-    value; when it grows, the codes already there are rounded again; a page whose first slot is written starts anew."""
+    value; when it grows, the codes before the new ones are rounded again; a page whose first slot is written starts anew.
+    Slots behind the new tokens stay as they were."""
     B, S, H, D = new.shape
     page = st["page"]
     first = st["lens"].long() // page                                            # first page touched
@@ -267,7 +268,8 @@ def _plain_append_one(new, cache, scale, st):
     was = cache[ids].float()
     again = (was * (torch.where(kept, old, s) / s)[..., None, None]).to(torch.float8_e4m3fn).float()
     put = (x / s[..., None, None]).clamp(-448.0, 448.0)
-    cache[ids] = torch.where(fr, put, torch.where(kept[..., None, None], again, was)).to(torch.float8_e4m3fn)
+    before = (src < 0)[:, None, :, None]
+    cache[ids] = torch.where(fr, put, torch.where(before, again, was)).to(torch.float8_e4m3fn)
     scale[ids] = s
 
 
@@ -418,7 +420,6 @@ def _exact_append(case, st):
                     s = torch.maximum(s, scale[i])
                     m = a - j * page
                     codes[i, :, :m] = _e4m3(codes[i, :, :m] * (scale[i] / s)[:, None, None])
-                    codes[i, :, z - j * page:] = _e4m3(codes[i, :, z - j * page:] * (scale[i] / s)[:, None, None])
                 codes[i, :, a - j * page:z - j * page] = _e4m3(x / s[:, None, None])
                 scale[i] = s
         out[name + "_cache"], out[name + "_scale"] = codes, scale
