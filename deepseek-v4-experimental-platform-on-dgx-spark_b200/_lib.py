@@ -17,6 +17,7 @@ LIB_PATH = os.path.join(HERE, "libbsgemm.so")
 DT_F32, DT_BF16, DT_F16, DT_E4M3, DT_E8M0, DT_E2M1X2 = 0, 1, 2, 3, 4, 5
 # status codes
 BS_OK, BS_ERR_INVALID_ARG, BS_ERR_UNSUPPORTED, BS_ERR_CUDA, BS_ERR_DEVICE_TIMEOUT = 0, 1, 2, 3, 4
+BS_ERR_BAD_INDEX = 6
 
 _c_void_p, _i64, _i32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int
 
@@ -71,12 +72,24 @@ SIGNATURES = {
                        _c_void_p, _c_void_p, _c_void_p, _c_void_p],
     "bs_moe_experts": [_i32, _i64, _i32, _i32, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
                        _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p],
+    "bs_rms_norm": [_c_void_p, _c_void_p, _c_void_p, _i32, _i64, _i64, ctypes.c_float, _c_void_p, _c_void_p, _c_void_p],
+    "bs_rms_norm_quant": [_c_void_p, _c_void_p, _c_void_p, _i32, _i64, _i64, ctypes.c_float, _i32, _c_void_p, _c_void_p,
+                          _c_void_p, _i32, _c_void_p],
+    "bs_rope": [_c_void_p, _i32, _i64, _i32, _i32, _i64, _i64, _c_void_p, _i32, _c_void_p, _i32, _i32, _i32, _i32,
+                ctypes.c_float, _c_void_p, _i64, _i64, _c_void_p],
+    "bs_cache_append": [_c_void_p, _c_void_p, _i32, _i64, _i64, _i32, _i32, ctypes.POINTER(_i64), ctypes.POINTER(_i64),
+                        _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i32, _c_void_p, _i64, _c_void_p, _c_void_p,
+                        _c_void_p],
+    "bs_cache_attn_workspace_size": [_i64, _i64, _i32, _i32, _i32, _i32],
+    "bs_cache_attn": [_c_void_p, _i32, _i64, _i64, _i32, _i32, _i32, ctypes.POINTER(_i64), _c_void_p, _c_void_p,
+                      _c_void_p, _c_void_p, _i64, _i32, _c_void_p, _i64, _c_void_p, _c_void_p, _c_void_p,
+                      ctypes.c_float, _c_void_p, _c_void_p, ctypes.c_size_t, _c_void_p],
     "bs_moe_combine": [_c_void_p, _c_void_p, _c_void_p, _i64, _i32, _i32, _c_void_p, _c_void_p],
 }
 RESTYPES = {"bs_last_error": ctypes.c_char_p, "bs_moe_workspace_size": ctypes.c_size_t,
             "bs_moe_staged_workspace_size": ctypes.c_size_t, "bs_moe_chunk_capacity": ctypes.c_int64,
             "bs_moe_time_layer": None, "bs_sparse_attn_workspace_size": ctypes.c_size_t,
-            "bs_indexer_topk_workspace_size": ctypes.c_size_t}
+            "bs_indexer_topk_workspace_size": ctypes.c_size_t, "bs_cache_attn_workspace_size": ctypes.c_size_t}
 
 
 class BsError(RuntimeError):

@@ -93,6 +93,8 @@ int bs_device_error_check(void) {
   if (e != cudaSuccess) return cuda_status(e, "read device error word");
   if (v != 0) {
     cudaMemcpyToSymbol(bs_device_error, &zero, sizeof(int));
+    if (v == BS_ERR_BAD_INDEX)
+      return fail(v, "device-side error %d (a page index or a length in device memory is out of range)", v);
     return fail(v, "device-side error %d (a bounded wait in a kernel ran out)", v);
   }
   return BS_OK;
@@ -718,6 +720,168 @@ int bs_moe_combine(const void* y, const int* pos_of, const float* w, int64_t T, 
   return cuda_status(bs_launch_moe_combine((const __nv_bfloat16*)y, pos_of, w, (int)T, topk, H, (__nv_bfloat16*)out,
                                            (cudaStream_t)stream),
                      "moe_combine");
+}
+
+// ---- serving operators: norm, rope, cache append, cache attention
+
+static int norm_common(const void* x, const void* residual, const void* weight, int dtype, int64_t rows, int64_t H,
+                       float eps, void* h, void* y, void* s, int s_dtype, int pow2, bool codes, void* stream,
+                       const char* name) {
+  if (dtype != BS_DT_BF16 && dtype != BS_DT_F16 && dtype != BS_DT_F32)
+    return fail(BS_ERR_INVALID_ARG, "%s: dtype tag %d: expected bf16, f16 or f32", name, dtype);
+  if (rows < 0 || H <= 0) return fail(BS_ERR_INVALID_ARG, "%s: bad shape rows=%lld H=%lld", name, (long long)rows, (long long)H);
+  const int unit = codes ? 128 : 8;
+  if (H % unit != 0 || H > rmsn::kMaxH)
+    return fail(BS_ERR_UNSUPPORTED, "%s: H=%lld: expected a multiple of %d up to %d", name, (long long)H, unit, rmsn::kMaxH);
+  if (rows > 0x7fffffff) return fail(BS_ERR_UNSUPPORTED, "%s: %lld rows", name, (long long)rows);
+  if (codes && s_dtype != BS_DT_F32 && s_dtype != BS_DT_E8M0)
+    return fail(BS_ERR_UNSUPPORTED, "%s: scale dtype tag %d: expected f32 or e8m0", name, s_dtype);
+  if (!(eps >= 0.0f)) return fail(BS_ERR_INVALID_ARG, "%s: eps %g", name, (double)eps);
+  if (rows == 0) return BS_OK;
+  if (!x || !weight || !y || (codes && !s) || (residual && !h)) return fail(BS_ERR_INVALID_ARG, "%s: null pointer", name);
+  if (!aligned(x, 16) || !aligned(weight, 16) || !aligned(residual, 16) || !aligned(h, 16) || !aligned(y, 16) ||
+      !aligned(s, s_dtype == BS_DT_F32 ? 4 : 1))
+    return fail(BS_ERR_INVALID_ARG, "%s: pointers must be 16-byte aligned", name);
+  rmsn::Args a = {};
+  a.x = x; a.res = residual; a.w = weight; a.h = h; a.y = y; a.s = s;
+  a.rows = rows; a.H = (int)H; a.eps = eps; a.s_e8m0 = s_dtype == BS_DT_E8M0; a.pow2 = pow2;
+  return cuda_status(bs_launch_rms_norm(a, dtype, codes, (cudaStream_t)stream), name);
+}
+
+int bs_rms_norm(const void* x, const void* residual, const void* weight, int dtype, int64_t rows, int64_t H, float eps,
+                void* h, void* y, void* stream) {
+  return norm_common(x, residual, weight, dtype, rows, H, eps, h, y, nullptr, BS_DT_F32, 0, false, stream, "rms_norm");
+}
+
+int bs_rms_norm_quant(const void* x, const void* residual, const void* weight, int dtype, int64_t rows, int64_t H,
+                      float eps, int pow2, void* h, void* y, void* s, int s_dtype, void* stream) {
+  return norm_common(x, residual, weight, dtype, rows, H, eps, h, y, s, s_dtype, pow2, true, stream, "rms_norm_quant");
+}
+
+int bs_rope(const void* x, int dtype, int64_t tokens, int H, int D, int64_t x_tok_stride, int64_t x_head_stride,
+            const void* positions, int pos_int64, const double* freqs, int rope_dim, int offset, int half, int inverse,
+            float scale, void* out, int64_t out_tok_stride, int64_t out_head_stride, void* stream) {
+  if (dtype != BS_DT_BF16 && dtype != BS_DT_F16 && dtype != BS_DT_F32)
+    return fail(BS_ERR_INVALID_ARG, "rope: dtype tag %d: expected bf16, f16 or f32", dtype);
+  if (tokens < 0 || H <= 0 || D <= 0 || rope_dim <= 0 || offset < 0 || (int64_t)offset + rope_dim > D)
+    return fail(BS_ERR_INVALID_ARG, "rope: tokens=%lld H=%d D=%d rope_dim=%d offset=%d", (long long)tokens, H, D, rope_dim, offset);
+  if (rope_dim % 16 != 0 || rope_dim > 2 * rope::kMaxPairs || offset % 8 != 0 || D % 8 != 0)
+    return fail(BS_ERR_UNSUPPORTED, "rope: rope_dim=%d (a multiple of 16 up to %d), offset=%d and D=%d (multiples of 8)",
+                rope_dim, 2 * rope::kMaxPairs, offset, D);
+  if (tokens > 0x7fffffff || H > 65535) return fail(BS_ERR_UNSUPPORTED, "rope: %lld tokens of %d heads", (long long)tokens, H);
+  if (tokens == 0) return BS_OK;
+  if (!x || !positions || !freqs || !out) return fail(BS_ERR_INVALID_ARG, "rope: null pointer");
+  const int e = 16 / elem_bytes(dtype);
+  if (!aligned(x, 16) || !aligned(out, 16) || !aligned(positions, pos_int64 ? 8 : 4) || !aligned(freqs, 8) ||
+      x_tok_stride % e || x_head_stride % e || out_tok_stride % e || out_head_stride % e)
+    return fail(BS_ERR_INVALID_ARG, "rope: pointers and strides must keep 16-byte vectors aligned");
+  rope::Args a = {};
+  a.x = x; a.out = out; a.x_tok = x_tok_stride; a.x_head = x_head_stride; a.o_tok = out_tok_stride; a.o_head = out_head_stride;
+  if (pos_int64) a.pos64 = (const int64_t*)positions;
+  else a.pos32 = (const int*)positions;
+  a.freq = freqs; a.tokens = tokens; a.H = H; a.D = D; a.n = rope_dim; a.offset = offset; a.scale = scale;
+  a.inverse = inverse; a.copy = x != out;
+  return cuda_status(bs_launch_rope(a, dtype, half, (cudaStream_t)stream), "rope");
+}
+
+// What append and attention ask of a cache; 0 or a status.
+static int cache_check(const char* name, int64_t B, int64_t S, int Hkv, int D, int64_t page, int64_t n_pages,
+                       int64_t max_pages) {
+  if (B < 0 || S <= 0 || Hkv <= 0 || D <= 0 || n_pages <= 0 || max_pages <= 0)
+    return fail(BS_ERR_INVALID_ARG, "%s: B=%lld S=%lld Hkv=%d D=%d n_pages=%lld max_pages=%lld", name, (long long)B,
+                (long long)S, Hkv, D, (long long)n_pages, (long long)max_pages);
+  if (!(page == 16 || page == 32 || page == 64 || page == 128))
+    return fail(BS_ERR_UNSUPPORTED, "%s: pages of %lld tokens (16, 32, 64 or 128)", name, (long long)page);
+  if (D % 16 != 0 || D > 512) return fail(BS_ERR_UNSUPPORTED, "%s: head dim %d (a multiple of 16 up to 512)", name, D);
+  if (n_pages * Hkv > 0x7ffffffe || max_pages * page > 0x7fffffff || n_pages > 0x7fffffff)
+    return fail(BS_ERR_UNSUPPORTED, "%s: %lld pages of %d heads, %lld pages per sequence", name, (long long)n_pages, Hkv,
+                (long long)max_pages);
+  return BS_OK;
+}
+
+int bs_cache_append(const void* k, const void* v, int dtype, int64_t B, int64_t S, int Hkv, int D,
+                    const int64_t* k_strides, const int64_t* v_strides, void* k_cache, void* v_cache, float* k_scale,
+                    float* v_scale, int64_t n_pages, int page, const int* block_table, int64_t max_pages,
+                    const int* start, const int* new_lens, void* stream) {
+  if (dtype != BS_DT_BF16 && dtype != BS_DT_F16 && dtype != BS_DT_F32)
+    return fail(BS_ERR_INVALID_ARG, "cache_append: dtype tag %d: expected bf16, f16 or f32", dtype);
+  int st = cache_check("cache_append", B, S, Hkv, D, page, n_pages, max_pages);
+  if (st) return st;
+  const int64_t span = (S + page - 2) / page + 1;
+  if (S > 0x7fffffff || B > 0x7fffffff || B * span > 0x7fffffff / Hkv)
+    return fail(BS_ERR_UNSUPPORTED, "cache_append: B=%lld S=%lld", (long long)B, (long long)S);
+  if (B == 0) return BS_OK;
+  const bool both = v != nullptr;
+  if (!k || !k_cache || !k_scale || !k_strides || !block_table || !start || (both && (!v_cache || !v_scale || !v_strides)))
+    return fail(BS_ERR_INVALID_ARG, "cache_append: null pointer");
+  const int e = 16 / elem_bytes(dtype);
+  for (int i = 0; i < 3; ++i)
+    if (k_strides[i] % e || (both && v_strides[i] % e))
+      return fail(BS_ERR_INVALID_ARG, "cache_append: strides must keep 16-byte vectors aligned");
+  if (!aligned(k, 16) || !aligned(v, 16) || !aligned(k_cache, 16) || !aligned(v_cache, 16) || !aligned(k_scale, 4) ||
+      !aligned(v_scale, 4) || !aligned(block_table, 4) || !aligned(start, 4) || !aligned(new_lens, 4))
+    return fail(BS_ERR_INVALID_ARG, "cache_append: misaligned pointer");
+  kvc::Args a = {};
+  a.src[0] = k; a.src[1] = v;
+  a.sb[0] = k_strides[0]; a.ss[0] = k_strides[1]; a.sh[0] = k_strides[2];
+  if (both) { a.sb[1] = v_strides[0]; a.ss[1] = v_strides[1]; a.sh[1] = v_strides[2]; }
+  a.cache[0] = (uint8_t*)k_cache; a.cache[1] = (uint8_t*)v_cache; a.scale[0] = k_scale; a.scale[1] = v_scale;
+  a.table = block_table; a.start = start; a.new_lens = new_lens;
+  a.B = (int)B; a.S = (int)S; a.Hkv = Hkv; a.D = D; a.max_pages = (int)max_pages; a.n_pages = (int)n_pages;
+  a.page_log2 = page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : 7;
+  a.span = (int)span;
+  return cuda_status(bs_launch_cache_append(a, dtype, both, (cudaStream_t)stream), "cache_append");
+}
+
+static int cattn_sizes(int64_t B, int64_t S, int H, int Hkv, int D, int dtype) {
+  if (B < 0 || S <= 0 || H <= 0 || Hkv <= 0 || D <= 0 || H % Hkv != 0)
+    return fail(BS_ERR_INVALID_ARG, "cache_attn: B=%lld S=%lld H=%d Hkv=%d D=%d", (long long)B, (long long)S, H, Hkv, D);
+  if (dtype != BS_DT_BF16 && dtype != BS_DT_F16)
+    return fail(BS_ERR_UNSUPPORTED, "cache_attn: q dtype tag %d (bf16 or f16)", dtype);
+  if (D % 16 != 0 || D > 512) return fail(BS_ERR_UNSUPPORTED, "cache_attn: head dim %d (a multiple of 16 up to 512)", D);
+  if (B > 0x7fffffff || S > 0x7fffffff || S * (H / Hkv) > 0x7fffffff - 64 || B * ((S * (H / Hkv) + 7) / 8) > 0x7fffffff)
+    return fail(BS_ERR_UNSUPPORTED, "cache_attn: B=%lld S=%lld H=%d", (long long)B, (long long)S, H);
+  return BS_OK;
+}
+
+size_t bs_cache_attn_workspace_size(int64_t B, int64_t S, int H, int Hkv, int D, int dtype) {
+  if (cattn_sizes(B, S, H, Hkv, D, dtype)) return 0;
+  return bs_cache_attn_ws(B, S, H, Hkv, D, dtype == BS_DT_F16);
+}
+
+int bs_cache_attn(const void* q, int dtype, int64_t B, int64_t S, int H, int Hkv, int D, const int64_t* q_strides,
+                  const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale, int64_t n_pages,
+                  int page, const int* block_table, int64_t max_pages, const int* seq_lens, const int* new_lens,
+                  const float* attn_sink, float softmax_scale, void* out, void* workspace, size_t workspace_bytes,
+                  void* stream) {
+  int st = cattn_sizes(B, S, H, Hkv, D, dtype);
+  if (st) return st;
+  st = cache_check("cache_attn", B, S, Hkv, D, page, n_pages, max_pages);
+  if (st) return st;
+  if (B == 0) return BS_OK;
+  if (!q || !q_strides || !k_cache || !k_scale || !block_table || !seq_lens || !out || (!v_cache != !v_scale))
+    return fail(BS_ERR_INVALID_ARG, "cache_attn: null pointer");
+  if (q_strides[0] % 4 || q_strides[1] % 4 || q_strides[2] % 4 || !aligned(q, 8) || !aligned(k_cache, 16) ||
+      !aligned(v_cache, 16) || !aligned(k_scale, 4) || !aligned(v_scale, 4) || !aligned(block_table, 4) ||
+      !aligned(seq_lens, 4) || !aligned(new_lens, 4) || !aligned(attn_sink, 4) || !aligned(out, 16))
+    return fail(BS_ERR_INVALID_ARG, "cache_attn: misaligned pointer, or q strides that are not multiples of 4");
+  const size_t need = bs_cache_attn_ws(B, S, H, Hkv, D, dtype == BS_DT_F16);
+  if (!workspace || workspace_bytes < need || !aligned(workspace, 256))
+    return fail(BS_ERR_INVALID_ARG, "cache_attn: workspace of %zu bytes, %zu needed (256-byte aligned)", workspace_bytes, need);
+  cattn::Args a = {};
+  a.q = q; a.q_sb = q_strides[0]; a.q_ss = q_strides[1]; a.q_sh = q_strides[2];
+  a.k_scale = k_scale; a.v_scale = v_scale; a.table = block_table; a.seq_lens = seq_lens; a.new_lens = new_lens;
+  a.sink = attn_sink; a.out = out;
+  a.B = (int)B; a.S = (int)S; a.H = H; a.Hkv = Hkv; a.G = H / Hkv; a.D = D;
+  a.page_log2 = page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : 7;
+  a.max_pages = (int)max_pages; a.n_pages = (int)n_pages;
+  a.scale_log2 = softmax_scale * 1.4426950408889634f;
+  a.shared = v_cache == nullptr;
+  cudaError_t cerr;
+  st = bs_launch_cache_attn(a, k_cache, v_cache, dtype == BS_DT_F16, workspace, (cudaStream_t)stream, &cerr);
+  if (st == BS_ERR_CUDA) return cuda_status(cerr, "cache_attn");
+  if (st) return fail(st, "cache_attn: no TMA descriptor for this cache");
+  return BS_OK;
 }
 
 }  // extern "C"

@@ -1,0 +1,1034 @@
+// Attention of each sequence's newest tokens over a paged e4m3 cache with one
+// scale per page and head (grouped-query heads; or one latent that is key and
+// value at once), with an optional sink logit per head.
+//
+//   o[b, s, h] = sum_t w_t v_t / (sum_t w_t + e^{sink_h}),   w_t = exp(scale q.k_t)
+//   over the cached tokens t < seq_len[b] - new[b] + s + 1
+//
+// The cached codes go from HBM to the tensor cores without being touched by a
+// thread: TMA brings 128 tokens x 128 bytes into 128B-swizzled shared memory,
+// and that one tile is the K-major A operand of S^T = K Q^T and, for values,
+// the MN-major A operand of O^T = V^T P^T.  A tcgen05.mma with M = 128 costs
+// the same for any N up to 128, so the few query rows of a decode step sit in
+// N, and what e4m3 would lose of Q and P is bought back with more columns:
+//
+//   x = c1 + c2/16 + c3/256,  c1 = e4m3(x), c2 = e4m3(16 (x - c1)), ...
+//
+// Each e4m3 term takes 4 significant bits.  Two terms hold a bf16 value
+// exactly (8 bits); three hold an f16 value (11 bits).  Rows of Q are first
+// scaled by a power of two so that their amax lies in [128, 256): what the
+// terms cannot hold is below 2^-22 of the row's amax for two terms and 2^-26
+// for three.  P = exp2(s - max) * (page's value scale / largest of the tile) *
+// 256 is rounded to the same number of terms: 2^-8 of the value at most with
+// bf16 outputs (half a step of bf16 itself is 2^-8), 2^-12 with f16.
+// Accumulation is fp32 in TMEM; O is taken out after every tile and added, in
+// fp32, to accumulators in registers, where the running maximum's factor and
+// the tile's value scale are applied.
+//
+// One work unit is a tile: 128 tokens of one (sequence, row tile, kv head);
+// a row tile is R of the S * (H / Hkv) query rows of a kv head.  All tiles of
+// the call lie in one sequence, and each CTA (one per SM) takes an equal
+// contiguous share of it, whatever the lengths; where a share ends inside a
+// head's tokens, both sides leave partial results (unnormalised O, max, sum)
+// and a second kernel joins them.  Lengths are read on the device only.
+//
+// Roles (10 warps): TMA producer; MMA issuer; four softmax warps, one token
+// per thread; four warps that stage Q and accumulate O, one head dim per
+// thread and 128-dim chunk.  Shared memory: a ring of 16 KB chunks, two Q
+// buffers (this segment's and the next one's), two P buffers.
+#include "common.cuh"
+
+namespace cattn {
+
+constexpr int kTok = 128;
+constexpr int kChunk = kTok * 128;
+constexpr int kThreads = 320;
+constexpr int kInfo = 16;          // tile info ring: above the tiles between the producer and the accumulators
+constexpr int kSegRing = 5;        // row sums of finished segments: the softmax warps run at most four segments ahead
+constexpr int kMaxSlots = 12;
+
+struct Args {
+  const void* q;
+  int64_t q_sb, q_ss, q_sh;        // strides in elements
+  const float* k_scale;
+  const float* v_scale;            // [n_pages, Hkv]
+  const int* table;                // [B, max_pages]
+  const int* seq_lens;
+  const int* new_lens;             // or null: S for every sequence
+  const float* sink;               // [H] or null
+  void* out;                       // [B, S, H, D]
+  int64_t* plan;                   // [1 + B * RT]: tiles per CTA, first tile of each (sequence, row tile)
+  float* part_ml;                  // [2 * grid][R][2]
+  float* part_o;                   // [2 * grid][R][NC * 128]
+  int B, S, H, Hkv, G, D, RT, page_log2, max_pages, n_pages;
+  float scale_log2;                // softmax scale x log2(e)
+  int shared;                      // values are the keys' codes
+  int slots;                       // chunks in the ring
+};
+
+// Lengths of one sequence as the kernels use them; what is out of range reads as nothing and is recorded.
+struct Seq {
+  int len, nl;
+};
+BS_DEVINL Seq load_seq(const Args& a, int b, bool report) {
+  Seq s;
+  s.len = a.seq_lens[b];
+  s.nl = a.new_lens ? a.new_lens[b] : a.S;
+  const int64_t most = (int64_t)a.max_pages << a.page_log2;
+  if (s.len < 0 || s.len > most || s.nl < 0 || s.nl > a.S) {
+    if (report) bs_set_error(BS_ERR_BAD_INDEX);
+    s.len = 0;
+    s.nl = 0;
+  }
+  return s;
+}
+// Tokens that query token i sees (0 for a padded one).
+BS_DEVINL int row_limit(const Seq& s, int i) { return i < s.nl ? max(0, s.len - s.nl + i + 1) : 0; }
+// Tokens that any row of row tile rt sees: those of its last row.
+BS_DEVINL int tile_limit(const Args& a, const Seq& s, int rt, int R) {
+  const int last = min((rt + 1) * R, a.S * a.G) - 1;
+  const int i = min(last / a.G, s.nl - 1);
+  return i < rt * R / a.G ? 0 : row_limit(s, i);
+}
+BS_DEVINL int tiles_of(int limit) { return (limit + kTok - 1) / kTok; }
+
+// A CTA's walk over its share: units (b, rt) in order, within a unit all kv heads, within a head its tiles.
+struct Walk {
+  int unit, h, t, nt;
+  int64_t left;
+  int b, rt, limit;
+  Seq s;
+  BS_DEVINL void enter(const Args& a, int R) {
+    b = unit / a.RT;
+    rt = unit - b * a.RT;
+    s = load_seq(a, b, false);
+    limit = tile_limit(a, s, rt, R);
+    nt = tiles_of(limit);
+  }
+  BS_DEVINL void start(const Args& a, int R, int unit0, int64_t off, int64_t n) {
+    unit = unit0;
+    left = n;
+    h = t = nt = 0;
+    if (left > 0) {
+      enter(a, R);
+      h = (int)(off / nt);
+      t = (int)(off - (int64_t)h * nt);
+    }
+  }
+  BS_DEVINL int seg_end() const { return (int)min((int64_t)nt, (int64_t)t + left); }
+  BS_DEVINL void next(const Args& a, int R) {
+    left -= seg_end() - t;
+    t = 0;
+    if (left <= 0) return;
+    if (++h == a.Hkv) {
+      h = 0;
+      do {
+        ++unit;
+        enter(a, R);
+      } while (nt == 0);            // left > 0: a later unit has tiles
+    }
+  }
+};
+
+struct Info {                       // one tile, from the producer
+  float ks[8], vs[8];               // per page of the tile; a page that is not there has valid bit 0
+  float unit;                       // largest |vs|
+  int valid;                        // bits of the pages that are there
+  int t0;                           // first token
+  int limit;                        // tokens that any row sees
+  int first, last;                  // of its segment
+  int vslot;                        // running index of its first value chunk
+  int mask;                         // some row does not see all of the tile
+};
+
+template <int R, int PP, int NC>
+struct Cfg {
+  static constexpr int N = R * PP % 16 ? R * PP + 8 : R * PP;      // columns of one MMA
+  static constexpr int kQBytes = NC * N * 128;
+  static constexpr int kPBytes = N * kTok;
+  static constexpr int OB = 2 * N + 2 * NC * N <= 512 ? 2 : 1;     // O buffers
+  static constexpr int SB = 2 * N + OB * NC * N <= 512 ? 2 : 1;    // S buffers
+  static constexpr int kCols = SB * N + OB * NC * N;
+  static constexpr int kTmem = kCols <= 32 ? 32 : kCols <= 64 ? 64 : kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
+  static_assert(kCols <= 512 && N % 16 == 0 && N <= 256, "TMEM");
+  struct Tail {                     // behind the ring, Q and P
+    Info info[kInfo];
+    float qf[2][R];                 // 2^-k x scale x log2(e) of each row
+    int lim[2][R];                  // tokens each row sees
+    int64_t off[2][R];              // element offset of the row's output, -1: no row
+    float wmax[4][R], muse[R], alpha[4][R];
+    float lsum[kSegRing][4][R], mfin[kSegRing][R];
+    int nanmin[kSegRing][NC * 128]; // first token with a NaN value in partly hidden tiles
+    int nanseen[kSegRing];
+    uint64_t full[kMaxSlots], empty[kMaxSlots];
+    uint64_t s_full[2], s_empty[2], p_full[2], o_full[2], o_empty[2], q_full[2], l_full[kSegRing];
+    uint32_t tmem;
+    int abort;
+    int64_t scan[12];
+    int64_t start_off, total;
+    int start_unit;
+  };
+  static constexpr int smem(int slots) { return 1024 + slots * kChunk + 2 * kQBytes + 2 * kPBytes + (int)sizeof(Tail); }
+};
+
+// Descriptor of a 128-token x 128-byte tile (128B swizzle) read along tokens: M is the byte within a row, K the row.
+// 8 rows (1024 bytes) to the next group along K; M = 128 is one swizzle atom wide.
+BS_DEVINL uint64_t sdesc_mn_sw128(uint32_t addr) {
+  uint64_t d = 0;
+  d |= (uint64_t)((addr >> 4) & 0x3FFF);
+  d |= (uint64_t)(1024 >> 4) << 16;
+  d |= (uint64_t)(1024 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+// Descriptor of P: [N / 16][128 tokens][16 bytes], no swizzle; 128 bytes to the next 8 tokens, 2048 to the next 16 columns.
+BS_DEVINL uint64_t sdesc_mn_plain(uint32_t addr) {
+  uint64_t d = 0;
+  d |= (uint64_t)((addr >> 4) & 0x3FFF);
+  d |= (uint64_t)(128 >> 4) << 16;
+  d |= (uint64_t)(2048 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  return d;
+}
+
+BS_DEVINL float redux_max(float v) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+// Barrier of the four softmax warps that also says whether all of them are still alive.
+BS_DEVINL bool group_all(bool ok) {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.and.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+               : "=r"(r)
+               : "r"((uint32_t)ok)
+               : "memory");
+  return r != 0;
+}
+BS_DEVINL void group_sync() { asm volatile("barrier.cta.sync 1, 128;" ::: "memory"); }
+
+// Two e4m3 codes -> two floats.
+BS_DEVINL float2 e4m3x2_to_f32(uint16_t c) {
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(c));
+  return __half22float2(*reinterpret_cast<__half2*>(&h));
+}
+// The PP terms of two values.
+template <int PP>
+BS_DEVINL void split2(float x, float y, uint16_t* c) {
+#pragma unroll
+  for (int p = 0; p < PP; ++p) {
+    c[p] = bs_cvt_e4m3x2(x, y);
+    if (p + 1 < PP) {
+      const float2 b = e4m3x2_to_f32(c[p]);
+      x = (x - b.x) * 16.0f;
+      y = (y - b.y) * 16.0f;
+    }
+  }
+}
+
+// R values of one TMEM lane out of their PP terms: columns term * R + row.
+template <int R, int PP>
+BS_DEVINL void load_rows(uint32_t taddr, float* s) {
+  if constexpr (R == 8 && PP == 2) {
+    uint32_t v[16];
+    BS_TMEM_LD16(taddr, v);
+    tmem_ld_wait();
+#pragma unroll
+    for (int r = 0; r < 8; ++r) s[r] = fmaf(__uint_as_float(v[8 + r]), 0.0625f, __uint_as_float(v[r]));
+  } else if constexpr (R == 8) {
+    uint32_t v[32];
+    BS_TMEM_LD32(taddr, v);
+    tmem_ld_wait();
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+      s[r] = fmaf(fmaf(__uint_as_float(v[16 + r]), 0.0625f, __uint_as_float(v[8 + r])), 0.0625f, __uint_as_float(v[r]));
+  } else if constexpr (R == 16) {
+    uint32_t v[PP][16];
+#pragma unroll
+    for (int p = 0; p < PP; ++p) BS_TMEM_LD16(taddr + p * R, v[p]);
+    tmem_ld_wait();
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      float x = __uint_as_float(v[PP - 1][r]);
+#pragma unroll
+      for (int p = PP - 2; p >= 0; --p) x = fmaf(x, 0.0625f, __uint_as_float(v[p][r]));
+      s[r] = x;
+    }
+  } else {
+#pragma unroll
+    for (int r0 = 0; r0 < R; r0 += 32) {
+      uint32_t v[PP][32];
+#pragma unroll
+      for (int p = 0; p < PP; ++p) BS_TMEM_LD32(taddr + p * R + r0, v[p]);
+      tmem_ld_wait();
+#pragma unroll
+      for (int r = 0; r < 32; ++r) {
+        float x = __uint_as_float(v[PP - 1][r]);
+#pragma unroll
+        for (int p = PP - 2; p >= 0; --p) x = fmaf(x, 0.0625f, __uint_as_float(v[p][r]));
+        s[r0 + r] = x;
+      }
+    }
+  }
+}
+
+// e4m3 NaN (0x7F or 0xFF) among four codes: bytes whose low seven bits are all set.
+BS_DEVINL uint32_t nan_bytes(uint32_t v) { return ((v & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; }
+
+template <int R, int PP, int NC>
+__global__ void __launch_bounds__(kThreads, 1)
+    cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const Args a) {
+  using C = Cfg<R, PP, NC>;
+  constexpr int N = C::N;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint8_t* qbuf = smem + a.slots * kChunk;
+  uint8_t* pbuf = qbuf + 2 * C::kQBytes;
+  typename C::Tail& T = *reinterpret_cast<typename C::Tail*>(pbuf + 2 * C::kPBytes);
+  volatile int* abort_flag = &T.abort;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  if (tid == 0) {
+    for (int i = 0; i < a.slots; ++i) {
+      mbar_init(&T.full[i], 1);
+      mbar_init(&T.empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&T.s_full[i], 1);
+      mbar_init(&T.s_empty[i], 4);
+      mbar_init(&T.p_full[i], 4);
+      mbar_init(&T.o_full[i], 1);
+      mbar_init(&T.o_empty[i], 4);
+      mbar_init(&T.q_full[i], 4);
+    }
+    for (int i = 0; i < kSegRing; ++i) mbar_init(&T.l_full[i], 4);
+    T.abort = 0;
+    T.start_unit = 0;
+    T.start_off = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&tm_k);
+    if (!a.shared) tma_prefetch_desc(&tm_v);
+  }
+  if (warp == 1) {
+    tmem_alloc(&T.tmem, C::kTmem);
+    tmem_relinquish();
+  }
+  // columns that hold no row stay zero
+  for (int i = tid; i < 2 * C::kQBytes / 16; i += kThreads) reinterpret_cast<uint4*>(qbuf)[i] = make_uint4(0, 0, 0, 0);
+  for (int i = tid; i < 2 * C::kPBytes / 16; i += kThreads) reinterpret_cast<uint4*>(pbuf)[i] = make_uint4(0, 0, 0, 0);
+  for (int i = tid; i < kSegRing * NC * 128; i += kThreads) (&T.nanmin[0][0])[i] = 0x7FFFFFFF;
+  if (tid < kSegRing) T.nanseen[tid] = 0;
+  pdl_launch_dependents();
+  pdl_wait();
+
+  // ---- the share of this CTA: tiles [start, start + count) of all
+  const int units = a.B * a.RT;
+  auto unit_tiles = [&](int u, bool report) -> int64_t {
+    if (u >= units) return 0;
+    const int b = u / a.RT;
+    const Seq s = load_seq(a, b, report);
+    return (int64_t)a.Hkv * tiles_of(tile_limit(a, s, u - b * a.RT, R));
+  };
+  int64_t mine = 0;
+  for (int u = tid; u < units; u += kThreads) mine += unit_tiles(u, blockIdx.x == 0 && u % a.RT == 0);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+  if (lane == 0) T.scan[warp] = mine;
+  fence_proxy_async_smem();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  int64_t total = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) total += T.scan[w];
+  __syncthreads();
+  const int64_t per = (total + gridDim.x - 1) / gridDim.x;
+  const int64_t start = min(per * blockIdx.x, total);
+  const int64_t count = min(per, total - start);
+  if (blockIdx.x == 0 && tid == 0) a.plan[0] = per;
+  if (count > 0 || blockIdx.x == 0) {
+    int64_t before = 0;
+    for (int u0 = 0; u0 < units; u0 += kThreads) {
+      const int64_t w = unit_tiles(u0 + tid, false);
+      int64_t inc = w;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t x = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += x;
+      }
+      if (lane == 31) T.scan[warp] = inc;
+      __syncthreads();
+      int64_t base = before;
+      for (int i = 0; i < warp; ++i) base += T.scan[i];
+      for (int i = 0; i < kThreads / 32; ++i) before += T.scan[i];
+      const int64_t ex = base + inc - w;
+      if (count > 0 && w > 0 && start >= ex && start < ex + w) {
+        T.start_unit = u0 + tid;
+        T.start_off = start - ex;
+      }
+      if (blockIdx.x == 0 && u0 + tid < units) a.plan[1 + u0 + tid] = ex;
+      __syncthreads();
+      if (blockIdx.x != 0 && before > start) break;
+    }
+  }
+  __syncthreads();
+  const uint32_t tmem = T.tmem;
+  const int unit0 = T.start_unit;
+  const int64_t off0 = T.start_off;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer
+    Walk w;
+    w.start(a, R, unit0, off0, count);
+    const int ppt = kTok >> a.page_log2, page = 1 << a.page_log2;
+    uint32_t ci = 0;                   // chunks asked for so far
+    uint32_t tile = 0;
+    bool ok = true;
+    int v_pages = 0;                   // the previous tile's page row of this lane, for its values
+    bool v_pending = false;
+    const int oob = a.n_pages * a.Hkv; // a page row past the end: TMA fills zeros
+    auto chunks = [&](const CUtensorMap* m, int prow) {
+      for (int c = 0; c < NC && ok; ++c, ++ci) {
+        const uint32_t s = ci % a.slots, ph = (ci / a.slots) & 1;
+        ok = __all_sync(0xffffffffu, mbar_wait(&T.empty[s], ph ^ 1, abort_flag));
+        if (!ok) break;
+        if (lane == 0) mbar_arrive_expect_tx(&T.full[s], kChunk);
+        __syncwarp();
+        if (lane < ppt) tma_load_3d(smem + s * kChunk + lane * page * 128, m, &T.full[s], c * 128, 0, prow);
+        __syncwarp();
+      }
+    };
+    while (w.left > 0 && ok) {
+      const int t1 = w.seg_end(), t0 = w.t;
+      for (int t = t0; t < t1 && ok; ++t, ++tile) {
+        // this tile's pages and scales, one page per lane
+        int prow = oob;
+        float ks = 0.0f, vs = 0.0f;
+        bool there = false;
+        if (lane < ppt) {
+          const int64_t p = (int64_t)t * ppt + lane;
+          if ((p << a.page_log2) < w.limit) {
+            const int id = a.table[(int64_t)w.b * a.max_pages + p];
+            there = id >= 0 && id < a.n_pages;
+            if (there) {
+              prow = id * a.Hkv + w.h;
+              ks = a.k_scale[prow];
+              vs = a.shared ? ks : a.v_scale[prow];
+            } else {
+              bs_set_error(BS_ERR_BAD_INDEX);
+            }
+          }
+        }
+        float unit = fabsf(vs);
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) unit = fmaxf(unit, __shfl_xor_sync(0xffffffffu, unit, o));
+        const uint32_t valid = __ballot_sync(0xffffffffu, there) & 0xFFu;
+        // the first slot of the tile free: the entry's last reader is far behind
+        const uint32_t s = ci % a.slots, ph = (ci / a.slots) & 1;
+        ok = __all_sync(0xffffffffu, mbar_wait(&T.empty[s], ph ^ 1, abort_flag));
+        if (!ok) break;
+        Info& in = T.info[tile % kInfo];
+        if (lane < 8) {
+          in.ks[lane] = ks;
+          in.vs[lane] = vs;
+        }
+        if (lane == 0) {
+          // rows of the tile see at least the first row's tokens
+          const int low = row_limit(w.s, w.rt * R / a.G);
+          in.unit = unit;
+          in.valid = (int)valid;
+          in.t0 = t * kTok;
+          in.limit = w.limit;
+          in.first = t == t0;
+          in.last = t + 1 == t1;
+          in.mask = (t + 1) * kTok > low || valid != (1u << ppt) - 1u;
+          // chunk order: K0 K1 V0 K2 V1 ... V_last (shared: every chunk once)
+          in.vslot = (int)(a.shared ? ci : 2 * NC * (tile + 1) - (tile + 1 == (uint32_t)count ? NC : 0));
+        }
+        __syncwarp();
+        chunks(&tm_k, prow);
+        if (!a.shared) {
+          if (v_pending && ok) chunks(&tm_v, v_pages);
+          v_pages = prow;
+          v_pending = true;
+        }
+      }
+      w.next(a, R);
+    }
+    if (v_pending && ok) chunks(&tm_v, v_pages);
+    // on the way out after a timeout: the copies in flight still write this CTA's shared memory
+    if (!ok) {
+      const uint32_t n = min(ci, (uint32_t)a.slots);
+      for (uint32_t k = 0; k < n; ++k) {
+        const uint32_t i = ci - 1 - k;
+        uint64_t t0 = 0;
+        for (uint32_t j = 0; j < BS_SPIN_LIMIT; ++j) {
+          if (mbar_try_wait(&T.full[i % a.slots], (i / a.slots) & 1)) break;
+          if (bs_wait_expired(j, &t0)) break;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA
+    const uint32_t idesc_s = idesc_f8f6f4(0, 0, 128, N);
+    const uint32_t idesc_o = idesc_f8f6f4(0, 0, 128, N) | (1u << 15) | (1u << 16);   // A and B along M / N
+    const uint64_t dk = sdesc_k128_sw128(smem_u32(smem));
+    const uint64_t dv = sdesc_mn_sw128(smem_u32(smem));
+    const uint64_t dq = sdesc_k128_sw128(smem_u32(qbuf));
+    const uint64_t dp = sdesc_mn_plain(smem_u32(pbuf));
+    uint32_t ci = 0;                 // chunks consumed, in the producer's order
+    uint32_t vprev = 0;              // first value chunk of the previous tile (shared)
+    int seg = -1;
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, uint32_t ph) {
+      ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, ph, abort_flag));
+    };
+    for (int64_t i = 0; i <= count && ok && count > 0; ++i) {
+      uint32_t kfirst = ci;
+      if (i < count) {
+        const int sb = (int)(i % C::SB);
+        for (int c = 0; c < NC; ++c) wait(&T.full[(ci + c) % a.slots], ((ci + c) / a.slots) & 1);
+        if (!ok) break;
+        if (T.info[i % kInfo].first) {
+          ++seg;
+          wait(&T.q_full[seg & 1], (seg >> 1) & 1);
+        }
+        wait(&T.s_empty[sb], ((i / C::SB) & 1) ^ 1);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int c = 0; c < NC; ++c) {
+            const uint64_t da = dk + (uint64_t)(((ci + c) % a.slots) * kChunk >> 4);
+            const uint64_t db = dq + (uint64_t)(((seg & 1) * C::kQBytes + c * N * 128) >> 4);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) tc_mma_f8f6f4(tmem + sb * N, da + 2 * k, db + 2 * k, idesc_s, (c | k) != 0);
+          }
+          if (!a.shared)
+            for (int c = 0; c < NC; ++c) tc_commit(&T.empty[(ci + c) % a.slots]);
+          tc_commit(&T.s_full[sb]);
+        }
+        __syncwarp();
+        ci += NC;
+      }
+      if (i > 0) {
+        const int64_t j = i - 1;
+        const int pb = (int)(j & 1), ob = (int)(j % C::OB);
+        const uint32_t v0 = a.shared ? vprev : ci;
+        wait(&T.p_full[pb], (j >> 1) & 1);
+        wait(&T.o_empty[ob], ((j / C::OB) & 1) ^ 1);
+        if (!a.shared)
+          for (int c = 0; c < NC; ++c) wait(&T.full[(v0 + c) % a.slots], ((v0 + c) / a.slots) & 1);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int c = 0; c < NC; ++c) {
+            const uint32_t s = (v0 + c) % a.slots;
+            const uint64_t da = dv + (uint64_t)(s * kChunk >> 4);
+            const uint64_t db = dp + (uint64_t)(pb * C::kPBytes >> 4);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)        // 32 tokens each: 4096 bytes of V, 512 of P
+              tc_mma_f8f6f4(tmem + C::SB * N + (ob * NC + c) * N, da + (4096 >> 4) * k, db + (512 >> 4) * k, idesc_o, k != 0);
+            tc_commit(&T.empty[s]);
+          }
+          tc_commit(&T.o_full[ob]);
+        }
+        __syncwarp();
+        if (!a.shared) ci += NC;
+      }
+      vprev = kfirst;
+    }
+  } else if (warp < 6) {
+    // ------------------------------------------------------------ softmax: one token per thread
+    const int quad = warp & 3;
+    const int tok = quad * 32 + lane;
+    const int row = (warp - 2) * 32 + lane;      // < R: the row whose maximum this thread keeps
+    const uint32_t lane_base = (uint32_t)(quad * 32) << 16;
+    float l[R];
+    float m_old = -INFINITY;
+    int seg = -1;
+    bool dead = false;
+#pragma unroll
+    for (int r = 0; r < R; ++r) l[r] = 0.0f;
+    for (int64_t i = 0; i < count; ++i) {
+      const int sb = (int)(i % C::SB), pb = (int)(i & 1);
+      const Info& in = T.info[i % kInfo];
+      float s[R];
+      bool ok = __all_sync(0xffffffffu, mbar_wait(&T.s_full[sb], (i / C::SB) & 1, abort_flag)) && !dead;
+      bool first = false, last = false;
+      float ratio = 0.0f;
+      if (ok) {
+        tc_fence_after();
+        load_rows<R, PP>(tmem + lane_base + sb * N, s);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&T.s_empty[sb]);
+        first = in.first;
+        last = in.last;
+        if (first) {
+          ++seg;
+          m_old = -INFINITY;
+#pragma unroll
+          for (int r = 0; r < R; ++r) l[r] = 0.0f;
+        }
+        const int pg = tok >> a.page_log2;
+        const float ks = in.ks[pg];
+        ratio = in.unit > 0.0f ? 256.0f * (in.vs[pg] / in.unit) : 0.0f;
+        const float* qf = T.qf[seg & 1];
+#pragma unroll
+        for (int r = 0; r < R; ++r) s[r] *= qf[r] * ks;
+        if (in.mask) {
+          const int t = in.t0 + tok;
+          const bool there = (in.valid >> pg) & 1;
+          const int* lim = T.lim[seg & 1];
+#pragma unroll
+          for (int r = 0; r < R; ++r)
+            if (!there || t >= lim[r]) s[r] = -INFINITY;
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const float m = redux_max(s[r]);
+          if (lane == 0) T.wmax[quad][r] = m;
+        }
+      }
+      if (!group_all(ok)) break;
+      if (row < R) {
+        const float m = fmaxf(fmaxf(fmaxf(T.wmax[0][row], T.wmax[1][row]), fmaxf(T.wmax[2][row], T.wmax[3][row])), m_old);
+        const float use = m == -INFINITY ? 0.0f : m;     // no token seen yet
+        T.muse[row] = use;
+        T.alpha[i & 3][row] = exp2f(m_old - use);
+        m_old = m;
+        if (last) T.mfin[seg % kSegRing][row] = m;
+      }
+      group_sync();
+      const float* muse = T.muse;
+      const float* al = T.alpha[i & 3];
+      uint8_t* p = pbuf + pb * C::kPBytes + tok * 16;
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        s[r] = exp2f(s[r] - muse[r]);
+        l[r] = fmaf(l[r], al[r], s[r]);
+      }
+      if constexpr (R == 8) {
+        uint32_t w[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+        for (int r = 0; r < 8; r += 2) {
+          uint16_t c[PP];
+          split2<PP>(s[r] * ratio, s[r + 1] * ratio, c);
+#pragma unroll
+          for (int k = 0; k < PP; ++k) w[2 * k + (r >> 2)] |= (uint32_t)c[k] << (16 * ((r >> 1) & 1));
+        }
+        *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+        if (PP == 3) *reinterpret_cast<uint4*>(p + 2048) = make_uint4(w[4], w[5], 0, 0);
+      } else {
+#pragma unroll
+        for (int g = 0; g < R / 16; ++g) {
+          uint32_t w[PP][4];
+#pragma unroll
+          for (int r = 0; r < 16; r += 4) {
+            uint16_t c[PP], d[PP];
+            split2<PP>(s[g * 16 + r] * ratio, s[g * 16 + r + 1] * ratio, c);
+            split2<PP>(s[g * 16 + r + 2] * ratio, s[g * 16 + r + 3] * ratio, d);
+#pragma unroll
+            for (int k = 0; k < PP; ++k) w[k][r >> 2] = (uint32_t)c[k] | ((uint32_t)d[k] << 16);
+          }
+#pragma unroll
+          for (int k = 0; k < PP; ++k)
+            *reinterpret_cast<uint4*>(p + (k * (R / 16) + g) * 2048) = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
+        }
+      }
+      if (in.mask) {
+        // Values that some row must not see: 0 x NaN would reach its sum.  Rows that no query sees become zero; a NaN
+        // in a row that only some see becomes zero too, and is put back for those when the segment ends.
+        const int t = in.t0 + tok;
+        for (int c = 0; c < NC; ++c) {
+          const uint32_t v = (uint32_t)in.vslot + c;
+          if (!a.shared && !__all_sync(0xffffffffu, mbar_wait(&T.full[v % a.slots], (v / a.slots) & 1, abort_flag))) dead = true;
+          uint4* row16 = reinterpret_cast<uint4*>(smem + (v % a.slots) * kChunk + tok * 128);
+          for (int k = 0; k < 8; ++k) {
+            // the swizzle has the row's dims 16 k .. 16 k + 15 in this 16-byte unit
+            uint4* vr = row16 + (k ^ (tok & 7));
+            if (t >= in.limit) {
+              *vr = make_uint4(0, 0, 0, 0);
+            } else {
+              uint4 x = *vr;
+              uint32_t* xs = reinterpret_cast<uint32_t*>(&x);
+              if (nan_bytes(x.x) | nan_bytes(x.y) | nan_bytes(x.z) | nan_bytes(x.w)) {
+                T.nanseen[seg % kSegRing] = 1;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const uint32_t nb = nan_bytes(xs[e]);
+#pragma unroll
+                  for (int y = 0; y < 4; ++y)
+                    if ((nb >> (8 * y + 7)) & 1) {
+                      atomicMin(&T.nanmin[seg % kSegRing][c * 128 + 16 * k + 4 * e + y], t);
+                      xs[e] &= ~(0xFFu << (8 * y));
+                    }
+                }
+                *vr = x;
+              }
+            }
+          }
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&T.p_full[pb]);
+      if (last) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          float x = l[r];
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+          if (lane == 0) T.lsum[seg % kSegRing][quad][r] = x;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&T.l_full[seg % kSegRing]);
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ Q in, O out
+    const int quad = warp & 3;
+    const uint32_t lane_base = (uint32_t)(quad * 32) << 16;
+    const int wq = warp - 6;
+    // One warp per row: amax, power-of-two scale, terms, swizzled store.
+    auto stage = [&](const Walk& w, int buf) {
+      uint8_t* qb = qbuf + buf * C::kQBytes;
+      for (int r = wq; r < R; r += 4) {
+        const int rr = w.rt * R + r;
+        const int i = rr / a.G, g = rr - i * a.G;
+        const bool in = rr < a.S * a.G;
+        float f[NC][4];
+        float amax = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          const int d = c * 128 + lane * 4;
+          f[c][0] = f[c][1] = f[c][2] = f[c][3] = 0.0f;
+          if (in && d < a.D) {
+            const int64_t at = (int64_t)w.b * a.q_sb + (int64_t)i * a.q_ss + (int64_t)(w.h * a.G + g) * a.q_sh + d;
+            const uint2 v = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(a.q) + at);
+            const uint32_t u[2] = {v.x, v.y};
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              if (PP == 3) {
+                const float2 z = __half22float2(*reinterpret_cast<const __half2*>(&u[k]));
+                f[c][2 * k] = z.x;
+                f[c][2 * k + 1] = z.y;
+              } else {
+                f[c][2 * k] = __uint_as_float(u[k] << 16);
+                f[c][2 * k + 1] = __uint_as_float(u[k] & 0xFFFF0000u);
+              }
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) amax = fmaxf(amax, fabsf(f[c][k]));
+        }
+        amax = redux_max(amax);
+        // 2^e with amax * 2^e in [128, 256); zero rows, tiny ones and infinities keep to the exponents that exist
+        int e = 134 - (int)(__float_as_uint(amax) >> 23);
+        e = amax == 0.0f ? 0 : min(max(e, -120), 120);
+        float up = __uint_as_float((uint32_t)(127 + e) << 23);
+        const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+        if (amax == __uint_as_float(0x7F800000u)) up = __uint_as_float(0x7FC00000u);   // e4m3 would saturate it
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          uint16_t lo[PP], hi[PP];
+          split2<PP>(f[c][0] * up, f[c][1] * up, lo);
+          split2<PP>(f[c][2] * up, f[c][3] * up, hi);
+#pragma unroll
+          for (int p = 0; p < PP; ++p) {
+            const int n = p * R + r;
+            *reinterpret_cast<uint32_t*>(qb + c * N * 128 + n * 128 + ((lane * 4) ^ ((n & 7) << 4))) =
+                (uint32_t)lo[p] | ((uint32_t)hi[p] << 16);
+          }
+        }
+        if (lane == 0) {
+          T.qf[buf][r] = down * a.scale_log2;
+          T.lim[buf][r] = in ? row_limit(w.s, i) : 0;
+          T.off[buf][r] = in && i < w.s.nl ? (((int64_t)w.b * a.S + i) * a.H + w.h * a.G + g) * a.D : -1;
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&T.q_full[buf]);
+    };
+    Walk w;
+    w.start(a, R, unit0, off0, count);
+    if (w.left > 0) stage(w, 0);
+    int64_t i = 0;
+    bool ok = true;
+    for (int seg = 0; w.left > 0 && ok; ++seg) {
+      const int t0 = w.t, t1 = w.seg_end(), nt = w.nt;
+      w.next(a, R);
+      // the other Q buffer: its last products are behind the O tiles taken out before
+      if (w.left > 0) stage(w, (seg + 1) & 1);
+      float acc[NC][R];
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int r = 0; r < R; ++r) acc[c][r] = 0.0f;
+      for (int t = t0; t < t1; ++t, ++i) {
+        const int ob = (int)(i % C::OB);
+        ok = __all_sync(0xffffffffu, mbar_wait(&T.o_full[ob], (i / C::OB) & 1, abort_flag));
+        if (!ok) break;
+        tc_fence_after();
+        const float unit = T.info[i % kInfo].unit * (1.0f / 256.0f);
+        const float* al = T.alpha[i & 3];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          float o[R];
+          load_rows<R, PP>(tmem + lane_base + C::SB * N + (ob * NC + c) * N, o);
+#pragma unroll
+          for (int r = 0; r < R; ++r) acc[c][r] = fmaf(acc[c][r], al[r], o[r] * unit);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&T.o_empty[ob]);
+      }
+      if (!ok) break;
+      const int sr = seg % kSegRing;
+      ok = __all_sync(0xffffffffu, mbar_wait(&T.l_full[sr], (seg / kSegRing) & 1, abort_flag));
+      if (!ok) break;
+      const int buf = seg & 1;
+      if (T.nanseen[sr]) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          const int first_nan = T.nanmin[sr][c * 128 + quad * 32 + lane];
+#pragma unroll
+          for (int r = 0; r < R; ++r)
+            if (first_nan < T.lim[buf][r]) acc[c][r] = __uint_as_float(0x7FC00000u);
+          T.nanmin[sr][c * 128 + quad * 32 + lane] = 0x7FFFFFFF;
+        }
+      }
+      const bool whole = t0 == 0 && t1 == nt;
+      const int64_t slot = 2 * (int64_t)blockIdx.x + (seg == 0 ? 0 : 1);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const float lr = T.lsum[sr][0][r] + T.lsum[sr][1][r] + T.lsum[sr][2][r] + T.lsum[sr][3][r];
+        const float m = T.mfin[sr][r];
+        if (whole) {
+          const int64_t at = T.off[buf][r];
+          if (at < 0) continue;
+          float f = 1.0f, z = lr;
+          if (a.sink) {
+            const float sk = a.sink[(at / a.D) % a.H] * 1.4426950408889634f;
+            const float M = fmaxf(m, sk);
+            f = m == -INFINITY ? 0.0f : exp2f(m - M);
+            z = lr * f + (sk == -INFINITY ? 0.0f : exp2f(sk - M));
+          }
+          f = z == 0.0f ? 0.0f : f / z;
+#pragma unroll
+          for (int c = 0; c < NC; ++c) {
+            const int d = c * 128 + quad * 32 + lane;
+            if (d < a.D) {
+              const float x = acc[c][r] * f;
+              if (PP == 3) reinterpret_cast<__half*>(a.out)[at + d] = __float2half_rn(x);
+              else reinterpret_cast<__nv_bfloat16*>(a.out)[at + d] = __float2bfloat16_rn(x);
+            }
+          }
+        } else {
+          if (quad == 0 && lane == 0) {
+            a.part_ml[(slot * R + r) * 2] = m;
+            a.part_ml[(slot * R + r) * 2 + 1] = lr;
+          }
+#pragma unroll
+          for (int c = 0; c < NC; ++c) a.part_o[(slot * R + r) * (NC * 128) + c * 128 + quad * 32 + lane] = acc[c][r];
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, C::kTmem);
+  }
+}
+
+// One warp per row: joins the partial results of heads that several CTAs share, and writes zeros for rows that see
+// nothing (empty sequences, padded query tokens).
+template <typename T>
+__global__ void __launch_bounds__(256) merge_kernel(const Args a, int R, int DC, int64_t rows) {
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const int64_t per = a.plan[0];
+  for (int64_t id = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 5; id < rows; id += (int64_t)gridDim.x * 8) {
+    const int r = (int)(id % R);
+    const int64_t item = id / R;
+    const int h = (int)(item % a.Hkv);
+    const int unit = (int)(item / a.Hkv);
+    const int b = unit / a.RT, rt = unit - b * a.RT;
+    const int rr = rt * R + r;
+    if (rr >= a.S * a.G) continue;
+    const int i = rr / a.G, g = rr - i * a.G;
+    const Seq s = load_seq(a, b, false);
+    const int nt = tiles_of(tile_limit(a, s, rt, R));
+    T* out = reinterpret_cast<T*>(a.out) + (((int64_t)b * a.S + i) * a.H + h * a.G + g) * a.D;
+    if (row_limit(s, i) == 0) {
+      for (int d = lane; d < a.D; d += 32) out[d] = bs_from_f32<T>(0.0f);
+      continue;
+    }
+    const int64_t first = a.plan[1 + unit] + (int64_t)h * nt;
+    const int64_t c0 = first / per, c1 = (first + nt - 1) / per;
+    if (c0 == c1) continue;                    // one CTA had it all
+    float M = -INFINITY, sk = -INFINITY;
+    if (a.sink) M = sk = a.sink[h * a.G + g] * 1.4426950408889634f;
+    // a CTA's first segment is in its slot 0, its last one in slot 1
+    auto slot = [&](int64_t c) { return 2 * c + (c * per >= first ? 0 : 1); };
+    for (int64_t c = c0 + lane; c <= c1; c += 32) M = fmaxf(M, a.part_ml[(slot(c) * R + r) * 2]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    const float use = M == -INFINITY ? 0.0f : M;
+    float z = sk == -INFINITY ? 0.0f : exp2f(sk - use);
+    for (int64_t c = c0; c <= c1; ++c) {
+      const float* ml = a.part_ml + (slot(c) * R + r) * 2;
+      z += ml[1] * exp2f(ml[0] - use);
+    }
+    const float f = z == 0.0f ? 0.0f : 1.0f / z;
+    for (int d = lane; d < a.D; d += 32) {
+      float acc = 0.0f;
+      for (int64_t c = c0; c <= c1; ++c) {
+        const int64_t at = slot(c) * R + r;
+        acc = fmaf(a.part_o[at * DC + d], exp2f(a.part_ml[at * 2] - use), acc);
+      }
+      out[d] = bs_from_f32<T>(acc * f);
+    }
+  }
+}
+
+bool make_map(CUtensorMap* m, const void* cache, int64_t D, int64_t page, int64_t rows) {
+  auto enc = moe::encode_fn();
+  if (!enc) return false;
+  cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)page, (cuuint64_t)rows};
+  cuuint64_t strides[2] = {(cuuint64_t)D, (cuuint64_t)(D * page)};
+  cuuint32_t box[3] = {128u, (cuuint32_t)page, 1u};          // dims past D are filled with zeros
+  cuuint32_t estr[3] = {1u, 1u, 1u};
+  return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(cache), dims, strides, box, estr,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Largest row tile: what TMEM, registers and shared memory carry.
+__host__ __device__ constexpr int most_rows(int PP, int NC) {
+  return NC == 1 ? (PP == 3 ? 32 : 64) : NC == 2 ? 32 : (PP == 3 ? 16 : 32);
+}
+// Rows of a tile: the smallest R that holds a kv head's rows, up to that.
+int rows_per_tile(int64_t rows, int NC, int f16) {
+  const int most = most_rows(f16 ? 3 : 2, NC);
+  int R = 8;
+  while (R < most && R < rows) R *= 2;
+  return R;
+}
+
+int sm_count() {
+  static int slots[hostcache::kMaxDevices];
+  const int n = hostcache::device_attr(slots, cudaDevAttrMultiProcessorCount);
+  return n > 0 ? n : 148;
+}
+
+struct Layout {
+  int R, NC, RT, grid;
+  size_t plan, ml, o, total;
+};
+Layout layout(int64_t B, int64_t S, int H, int Hkv, int D, int f16) {
+  Layout l;
+  l.NC = (D + 127) / 128;
+  const int64_t rows = S * (H / Hkv);
+  l.R = rows_per_tile(rows, l.NC, f16);
+  l.RT = (int)((rows + l.R - 1) / l.R);
+  l.grid = sm_count();
+  auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+  l.plan = up((1 + (size_t)B * l.RT) * 8);
+  l.ml = up((size_t)2 * l.grid * l.R * 2 * 4);
+  l.o = (size_t)2 * l.grid * l.R * l.NC * 128 * 4;
+  l.total = l.plan + l.ml + l.o;
+  return l;
+}
+
+template <int R, int PP, int NC>
+cudaError_t launch(const CUtensorMap& mk, const CUtensorMap& mv, Args a, int grid, cudaStream_t st) {
+  using C = Cfg<R, PP, NC>;
+  auto kern = cache_attn_kernel<R, PP, NC>;
+  // as many chunks as fit, with two tiles at least (the next tile's keys arrive before this one's values are used up)
+  int slots = kMaxSlots;
+  while (C::smem(slots) > 227 * 1024) --slots;
+  if (slots < 2 * NC) return cudaErrorInvalidConfiguration;
+  a.slots = slots;
+  static int done[hostcache::kMaxDevices];
+  cudaError_t e = (cudaError_t)hostcache::get(done, [&] {
+    return (int)cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::smem(slots));
+  });
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = C::smem(slots);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, mk, mv, a);
+}
+
+template <int PP, int NC>
+cudaError_t launch_r(int R, const CUtensorMap& mk, const CUtensorMap& mv, const Args& a, int grid, cudaStream_t st) {
+  if (R == 8) return launch<8, PP, NC>(mk, mv, a, grid, st);
+  if (R == 16) return launch<16, PP, NC>(mk, mv, a, grid, st);
+  if constexpr (most_rows(PP, NC) >= 32)
+    if (R == 32) return launch<32, PP, NC>(mk, mv, a, grid, st);
+  if constexpr (most_rows(PP, NC) >= 64)
+    if (R == 64) return launch<64, PP, NC>(mk, mv, a, grid, st);
+  return cudaErrorInvalidConfiguration;
+}
+
+}  // namespace cattn
+
+size_t bs_cache_attn_ws(int64_t B, int64_t S, int H, int Hkv, int D, int f16) {
+  return cattn::layout(B, S, H, Hkv, D, f16).total;
+}
+
+// 0 ok, BS_ERR_UNSUPPORTED (descriptor), or a CUDA error in *cerr
+int bs_launch_cache_attn(cattn::Args a, const void* k_cache, const void* v_cache, int f16, void* ws, cudaStream_t st,
+                         cudaError_t* cerr) {
+  *cerr = cudaSuccess;
+  const cattn::Layout l = cattn::layout(a.B, a.S, a.H, a.Hkv, a.D, f16);
+  a.RT = l.RT;
+  a.plan = (int64_t*)ws;
+  a.part_ml = (float*)((char*)ws + l.plan);
+  a.part_o = (float*)((char*)ws + l.plan + l.ml);
+  const int64_t page = (int64_t)1 << a.page_log2;
+  CUtensorMap mk, mv;
+  if (!cattn::make_map(&mk, k_cache, a.D, page, (int64_t)a.n_pages * a.Hkv)) return BS_ERR_UNSUPPORTED;
+  if (!cattn::make_map(&mv, a.shared ? k_cache : v_cache, a.D, page, (int64_t)a.n_pages * a.Hkv)) return BS_ERR_UNSUPPORTED;
+  cudaError_t e;
+  if (f16)
+    e = l.NC == 1 ? cattn::launch_r<3, 1>(l.R, mk, mv, a, l.grid, st) : l.NC == 2 ? cattn::launch_r<3, 2>(l.R, mk, mv, a, l.grid, st)
+      : l.NC == 3 ? cattn::launch_r<3, 3>(l.R, mk, mv, a, l.grid, st) : cattn::launch_r<3, 4>(l.R, mk, mv, a, l.grid, st);
+  else
+    e = l.NC == 1 ? cattn::launch_r<2, 1>(l.R, mk, mv, a, l.grid, st) : l.NC == 2 ? cattn::launch_r<2, 2>(l.R, mk, mv, a, l.grid, st)
+      : l.NC == 3 ? cattn::launch_r<2, 3>(l.R, mk, mv, a, l.grid, st) : cattn::launch_r<2, 4>(l.R, mk, mv, a, l.grid, st);
+  if (e != cudaSuccess) {
+    *cerr = e;
+    return BS_ERR_CUDA;
+  }
+  const int64_t rows = (int64_t)a.B * a.RT * a.Hkv * l.R;
+  cudaLaunchConfig_t cfg = {};
+  const int64_t want = (rows + 7) / 8;
+  cfg.gridDim = dim3((unsigned)(want < 148 * 8 ? want : 148 * 8));
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = f16 ? cudaLaunchKernelEx(&cfg, cattn::merge_kernel<__half>, a, l.R, l.NC * 128, rows)
+          : cudaLaunchKernelEx(&cfg, cattn::merge_kernel<__nv_bfloat16>, a, l.R, l.NC * 128, rows);
+  *cerr = e;
+  return e == cudaSuccess ? 0 : BS_ERR_CUDA;
+}

@@ -11,8 +11,9 @@
  *   - enqueues work on the stream and returns without synchronising;
  *   - returns 0 on success or a BS_ERR_* code, with a message available from
  *     bs_last_error() (thread-local).  No C++ exception crosses the ABI.
- * Device-side failures (a bounded wait that ran out) are recorded in a
- * device word and reported by bs_device_error_check().
+ * Device-side failures (a bounded wait that ran out; a page index or length
+ * in device memory that is out of range) are recorded in a device word and
+ * reported by bs_device_error_check().
  *
  * Layouts (all row-major, contiguous):
  *   bf16/f16/f32 activations [rows, K]; e4m3 codes one byte each;
@@ -46,7 +47,8 @@ enum {
   BS_ERR_UNSUPPORTED = 2,
   BS_ERR_CUDA = 3,
   BS_ERR_DEVICE_TIMEOUT = 4,
-  BS_ERR_DEVICE_FAULT = 5
+  BS_ERR_DEVICE_FAULT = 5,
+  BS_ERR_BAD_INDEX = 6 /* a page index or length in device memory is out of range */
 };
 
 /* Library version (major*10000 + minor*100 + patch). */
@@ -346,6 +348,83 @@ int bs_ep_moe_forward(const void* x, const float* logits, int64_t T, int64_t max
 /* out[t] = bf16(sum_k w[t,k] * y[pos_of[t,k]]) */
 int bs_moe_combine(const void* y, const int* pos_of, const float* w, int64_t T, int topk, int H, void* out,
                    void* stream);
+
+/*
+ * RMS norm with the residual's addition.  x, residual (or NULL), weight, h:
+ * bf16, f16 or f32, one type for all; x [rows, H], weight [H].
+ * h = x + residual, rounded to the type (written only with a residual; may be
+ * x or residual itself); y = h * weight / sqrt(mean(h^2) + eps) in fp32.
+ * bs_rms_norm writes y in the type (H a multiple of 8, up to 16384);
+ * bs_rms_norm_quant writes e4m3 codes [rows, H] and scales [rows, H/128]
+ * (f32 or e8m0; s = max(amax, 1e-4)/448 over 128 values, rounded up to a power
+ * of two when pow2), H a multiple of 128 up to 16384: the operands of
+ * bs_fp8_gemm and bs_fp4_gemm.
+ */
+int bs_rms_norm(const void* x, const void* residual, const void* weight, int dtype, int64_t rows, int64_t H, float eps,
+                void* h, void* y, void* stream);
+int bs_rms_norm_quant(const void* x, const void* residual, const void* weight, int dtype, int64_t rows, int64_t H,
+                      float eps, int pow2, void* h, void* y, void* s, int s_dtype, void* stream);
+
+/*
+ * Rotary positions on dims [offset, offset + rope_dim) of each head: pair i
+ * turns by positions[token] * freqs[i] radians (freqs fp64 [rope_dim/2];
+ * positions int64 when pos_int64, else int32, any sign), backwards when
+ * inverse, times scale.  Pairs are (x[2i], x[2i+1]), or with half
+ * (x[i], x[i + rope_dim/2]).  x, out: bf16, f16 or f32 [tokens, H, D] with the
+ * last dim contiguous and the given strides in elements; out may be x (the
+ * other dims are then not touched) but must not overlap it otherwise.
+ * rope_dim a multiple of 16 up to 512; offset and D multiples of 8.
+ */
+int bs_rope(const void* x, int dtype, int64_t tokens, int H, int D, int64_t x_tok_stride, int64_t x_head_stride,
+            const void* positions, int pos_int64, const double* freqs, int rope_dim, int offset, int half, int inverse,
+            float scale, void* out, int64_t out_tok_stride, int64_t out_head_stride, void* stream);
+
+/*
+ * Appends keys and values to a paged e4m3 cache.
+ *   k, v       [B, S, Hkv, D] bf16, f16 or f32, last dim contiguous, strides
+ *              {batch, token, head} in elements; v NULL: keys only (a latent
+ *              cache whose values are its keys)
+ *   k_cache, v_cache  [n_pages, Hkv, page, D] e4m3; k_scale, v_scale
+ *              [n_pages, Hkv] fp32; page 16, 32, 64 or 128; D a multiple of
+ *              16 up to 512
+ *   block_table  int32 [B, max_pages]; start  int32 [B], tokens already
+ *              cached; new_lens  int32 [B] or NULL: how many of the S are real
+ * Token i of sequence b goes to position start[b] + i.  A page's scale is the
+ * smallest power of two that holds its values' amax (at least 1e-4) in 448;
+ * if it has to grow, the page's earlier codes are rounded again to the larger
+ * scale.  Writing a page's slot 0 starts it anew; slots behind the new tokens
+ * are left as they are.  Non-finite values are stored as NaN and do not count
+ * for the scale.  Two sequences of a call must not write to the same page.
+ * A page index or length out of range writes nothing there and is reported
+ * by bs_device_error_check().
+ */
+int bs_cache_append(const void* k, const void* v, int dtype, int64_t B, int64_t S, int Hkv, int D,
+                    const int64_t* k_strides, const int64_t* v_strides, void* k_cache, void* v_cache, float* k_scale,
+                    float* v_scale, int64_t n_pages, int page, const int* block_table, int64_t max_pages,
+                    const int* start, const int* new_lens, void* stream);
+
+/*
+ * Attention over that cache: q [B, S, H, D] (bf16 or f16, strides {batch,
+ * token, head} in elements, multiples of 4) -> out [B, S, H, D] contiguous.
+ * seq_lens int32 [B] counts all cached tokens, the S (or new_lens[b]) newest
+ * included; query token i sees the first seq_lens[b] - new_lens[b] + i + 1.
+ * Query heads h*H/Hkv .. share kv head h.  v_cache NULL: the values are the
+ * keys.  Any finite or NaN scales are taken (fp32 [n_pages, Hkv]).
+ * attn_sink fp32 [H] or NULL: a logit per head that takes softmax weight and
+ * adds no value.  A row that sees nothing is zero, padded query tokens too.
+ * Softmax statistics and sums in fp32; weights and queries enter the tensor
+ * cores as sums of two (bf16) or three (f16) e4m3 terms.  Results do not
+ * depend on any order of execution.  A page index or length out of range
+ * reads as absent and is reported by bs_device_error_check().
+ * The workspace may be reused once the call's work is done; calls that may
+ * overlap on the GPU need one each.
+ */
+size_t bs_cache_attn_workspace_size(int64_t B, int64_t S, int H, int Hkv, int D, int dtype);
+int bs_cache_attn(const void* q, int dtype, int64_t B, int64_t S, int H, int Hkv, int D, const int64_t* q_strides,
+                  const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale, int64_t n_pages,
+                  int page, const int* block_table, int64_t max_pages, const int* seq_lens, const int* new_lens,
+                  const float* attn_sink, float softmax_scale, void* out, void* workspace, size_t workspace_bytes,
+                  void* stream);
 
 #ifdef __cplusplus
 }
