@@ -32,17 +32,17 @@
 // head's tokens, both sides leave partial results (unnormalised O, max, sum)
 // and a second kernel joins them.  Lengths are read on the device only.
 //
-// Roles (10 warps): TMA producer; MMA issuer; four softmax warps, one token
-// per thread; four warps that stage Q and accumulate O, one head dim per
-// thread and 128-dim chunk.  Shared memory: a ring of 16 KB chunks, two Q
-// buffers (this segment's and the next one's), two P buffers.
+// Roles: one warpgroup with the TMA producer and the MMA issuer; one or (from
+// 32 rows on) two softmax warpgroups, each with its share of the rows; one
+// that stages Q and accumulates O, one head dim per thread and 128-dim chunk.
+// Shared memory: a ring of 16 KB chunks, Q (this segment's and, where it fits,
+// the next one's), two P buffers.
 #include "common.cuh"
 
 namespace cattn {
 
 constexpr int kTok = 128;
 constexpr int kChunk = kTok * 128;
-constexpr int kThreads = 320;
 constexpr int kInfo = 16;          // tile info ring: above the tiles between the producer and the accumulators
 constexpr int kSegRing = 5;        // row sums of finished segments: the softmax warps run at most four segments ahead
 constexpr int kMaxSlots = 12;
@@ -63,7 +63,6 @@ struct Args {
   int B, S, H, Hkv, G, D, RT, page_log2, max_pages, n_pages;
   float scale_log2;                // softmax scale x log2(e)
   int shared;                      // values are the keys' codes
-  int slots;                       // chunks in the ring
 };
 
 // Lengths of one sequence as the kernels use them; what is out of range reads as nothing and is recorded.
@@ -97,6 +96,7 @@ struct Walk {
   int unit, h, t, nt;
   int64_t left;
   int b, rt, limit;
+  bool fresh;                       // nothing of this segment has been taken yet
   Seq s;
   BS_DEVINL void enter(const Args& a, int R) {
     b = unit / a.RT;
@@ -109,6 +109,7 @@ struct Walk {
     unit = unit0;
     left = n;
     h = t = nt = 0;
+    fresh = true;
     if (left > 0) {
       enter(a, R);
       h = (int)(off / nt);
@@ -119,6 +120,7 @@ struct Walk {
   BS_DEVINL void next(const Args& a, int R) {
     left -= seg_end() - t;
     t = 0;
+    fresh = true;
     if (left <= 0) return;
     if (++h == a.Hkv) {
       h = 0;
@@ -131,21 +133,26 @@ struct Walk {
 };
 
 struct Info {                       // one tile, from the producer
-  float ks[8], vs[8];               // per page of the tile; a page that is not there has valid bit 0
-  float unit;                       // largest |vs|
+  float ks[8];                      // per page of the tile
+  float vr[8];                      // 256 x value scale / unit
+  float unit;                       // largest |value scale|
   int valid;                        // bits of the pages that are there
   int t0;                           // first token
   int limit;                        // tokens that any row sees
   int first, last;                  // of its segment
-  int vslot;                        // running index of its first value chunk
   int mask;                         // some row does not see all of the tile
+  int pad;
 };
 
 template <int R, int PP, int NC>
 struct Cfg {
   static constexpr int N = R * PP % 16 ? R * PP + 8 : R * PP;      // columns of one MMA
+  static constexpr int WG = R >= 32 ? 2 : 1;                       // softmax warpgroups
+  static constexpr int RW = R / WG;                                // rows of each
+  static constexpr int kThreads = 128 * (2 + WG);
   static constexpr int kQBytes = NC * N * 128;
   static constexpr int kPBytes = N * kTok;
+  static constexpr int QB = kQBytes >= 32768 ? 1 : 2;              // Q buffers
   static constexpr int OB = 2 * N + 2 * NC * N <= 512 ? 2 : 1;     // O buffers
   static constexpr int SB = 2 * N + OB * NC * N <= 512 ? 2 : 1;    // S buffers
   static constexpr int kCols = SB * N + OB * NC * N;
@@ -153,10 +160,10 @@ struct Cfg {
   static_assert(kCols <= 512 && N % 16 == 0 && N <= 256, "TMEM");
   struct Tail {                     // behind the ring, Q and P
     Info info[kInfo];
-    float qf[2][R];                 // 2^-k x scale x log2(e) of each row
+    float qf[2][R];                 // 2^-k x |scale| x log2(e) of each row
     int lim[2][R];                  // tokens each row sees
     int64_t off[2][R];              // element offset of the row's output, -1: no row
-    float wmax[4][R], muse[R], alpha[4][R];
+    float wmax[2][4][R], alpha[4][R];
     float lsum[kSegRing][4][R], mfin[kSegRing][R];
     int nanmin[kSegRing][NC * 128]; // first token with a NaN value in partly hidden tiles
     int nanseen[kSegRing];
@@ -164,11 +171,16 @@ struct Cfg {
     uint64_t s_full[2], s_empty[2], p_full[2], o_full[2], o_empty[2], q_full[2], l_full[kSegRing];
     uint32_t tmem;
     int abort;
-    int64_t scan[12];
-    int64_t start_off, total;
+    int64_t scan[16];
+    int64_t start_off;
     int start_unit;
   };
-  static constexpr int smem(int slots) { return 1024 + slots * kChunk + 2 * kQBytes + 2 * kPBytes + (int)sizeof(Tail); }
+  static constexpr int kFixed = 1024 + QB * kQBytes + 2 * kPBytes + (int)sizeof(Tail);
+  static constexpr int kFit = (227 * 1024 - kFixed) / kChunk;
+  static constexpr int kSlots = kFit < kMaxSlots ? kFit : kMaxSlots;
+  // two tiles at least: the next tile's keys are used before this one's values
+  static_assert(kSlots >= 2 * NC, "ring");
+  static constexpr int kSmem = kFixed + kSlots * kChunk;
 };
 
 // Descriptor of a 128-token x 128-byte tile (128B swizzle) read along tokens: M is the byte within a row, K the row.
@@ -197,34 +209,82 @@ BS_DEVINL float redux_max(float v) {
   asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
   return r;
 }
-// Barrier of the four softmax warps that also says whether all of them are still alive.
-BS_DEVINL bool group_all(bool ok) {
+// Barrier of a softmax warpgroup that also says whether all of it is still alive.
+BS_DEVINL bool group_all(int id, bool ok) {
   uint32_t r;
-  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.and.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-               : "=r"(r)
-               : "r"((uint32_t)ok)
-               : "memory");
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.and.pred q, %2, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"((uint32_t)ok), "r"(id)
+      : "memory");
   return r != 0;
 }
-BS_DEVINL void group_sync() { asm volatile("barrier.cta.sync 1, 128;" ::: "memory"); }
+template <int N>
+BS_DEVINL void reg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+BS_DEVINL void reg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 
-// Two e4m3 codes -> two floats.
-BS_DEVINL float2 e4m3x2_to_f32(uint16_t c) {
+// 2^x to 2 ulp; exponents below -126 give 0.
+BS_DEVINL float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// Two e4m3 codes -> f16 (exact).
+BS_DEVINL __half2 e4m3x2_to_h2(uint16_t c) {
   uint32_t h;
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(c));
-  return __half22float2(*reinterpret_cast<__half2*>(&h));
+  return *reinterpret_cast<__half2*>(&h);
 }
-// The PP terms of two values.
+BS_DEVINL uint16_t h2_to_e4m3x2(__half2 v) {
+  uint16_t c;
+  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(c) : "r"(*reinterpret_cast<uint32_t*>(&v)));
+  return c;
+}
+// The PP terms of two values, in fp32 (Q).
 template <int PP>
 BS_DEVINL void split2(float x, float y, uint16_t* c) {
 #pragma unroll
   for (int p = 0; p < PP; ++p) {
     c[p] = bs_cvt_e4m3x2(x, y);
     if (p + 1 < PP) {
-      const float2 b = e4m3x2_to_f32(c[p]);
+      const float2 b = __half22float2(e4m3x2_to_h2(c[p]));
       x = (x - b.x) * 16.0f;
       y = (y - b.y) * 16.0f;
     }
+  }
+}
+// The same from f16 (P): rounding to f16 first costs 2^-12 of the value at most, and three terms then hold its 11 bits;
+// differences of a value and its nearest e4m3 neighbour are exact.
+template <int PP>
+BS_DEVINL void split2h(float x, float y, uint16_t* c) {
+  __half2 v = __floats2half2_rn(x, y);
+#pragma unroll
+  for (int p = 0; p < PP; ++p) {
+    c[p] = h2_to_e4m3x2(v);
+    if (p + 1 < PP) v = __hmul2(__hsub2(v, e4m3x2_to_h2(c[p])), __float2half2_rn(16.0f));
+  }
+}
+
+// 16 TMEM lanes x 8 K columns: v[4g + 2i + j] is lane (thread / 4) + 8i, column 8g + 2 (thread % 4) + j.
+template <int K>
+BS_DEVINL void tmem_ld16x256(uint32_t taddr, uint32_t* v) {
+  if constexpr (K == 1) {
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x1.b32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+                 : "r"(taddr));
+  } else if constexpr (K == 2) {
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+                 : "r"(taddr));
+  } else {
+    static_assert(K == 4, "16x256b.x4");
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(taddr));
   }
 }
 
@@ -278,32 +338,33 @@ BS_DEVINL void load_rows(uint32_t taddr, float* s) {
 BS_DEVINL uint32_t nan_bytes(uint32_t v) { return ((v & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; }
 
 template <int R, int PP, int NC>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, 1)
     cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const Args a) {
   using C = Cfg<R, PP, NC>;
-  constexpr int N = C::N;
+  constexpr int N = C::N, kThreads = C::kThreads;
+  constexpr uint32_t SLOTS = C::kSlots;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  uint8_t* qbuf = smem + a.slots * kChunk;
-  uint8_t* pbuf = qbuf + 2 * C::kQBytes;
+  uint8_t* qbuf = smem + SLOTS * kChunk;
+  uint8_t* pbuf = qbuf + C::QB * C::kQBytes;
   typename C::Tail& T = *reinterpret_cast<typename C::Tail*>(pbuf + 2 * C::kPBytes);
   volatile int* abort_flag = &T.abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (tid == 0) {
-    for (int i = 0; i < a.slots; ++i) {
+    for (int i = 0; i < (int)SLOTS; ++i) {
       mbar_init(&T.full[i], 1);
       mbar_init(&T.empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&T.s_full[i], 1);
-      mbar_init(&T.s_empty[i], 4);
-      mbar_init(&T.p_full[i], 4);
+      mbar_init(&T.s_empty[i], 4 * C::WG);
+      mbar_init(&T.p_full[i], 4 * C::WG);
       mbar_init(&T.o_full[i], 1);
       mbar_init(&T.o_empty[i], 4);
       mbar_init(&T.q_full[i], 4);
     }
-    for (int i = 0; i < kSegRing; ++i) mbar_init(&T.l_full[i], 4);
+    for (int i = 0; i < kSegRing; ++i) mbar_init(&T.l_full[i], 4 * C::WG);
     T.abort = 0;
     T.start_unit = 0;
     T.start_off = 0;
@@ -316,8 +377,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_relinquish();
   }
   // columns that hold no row stay zero
-  for (int i = tid; i < 2 * C::kQBytes / 16; i += kThreads) reinterpret_cast<uint4*>(qbuf)[i] = make_uint4(0, 0, 0, 0);
-  for (int i = tid; i < 2 * C::kPBytes / 16; i += kThreads) reinterpret_cast<uint4*>(pbuf)[i] = make_uint4(0, 0, 0, 0);
+  if (N != R * PP) {
+    for (int i = tid; i < C::QB * C::kQBytes / 16; i += kThreads) reinterpret_cast<uint4*>(qbuf)[i] = make_uint4(0, 0, 0, 0);
+    for (int i = tid; i < 2 * C::kPBytes / 16; i += kThreads) reinterpret_cast<uint4*>(pbuf)[i] = make_uint4(0, 0, 0, 0);
+  }
   for (int i = tid; i < kSegRing * NC * 128; i += kThreads) (&T.nanmin[0][0])[i] = 0x7FFFFFFF;
   if (tid < kSegRing) T.nanseen[tid] = 0;
   pdl_launch_dependents();
@@ -346,7 +409,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   const int64_t per = (total + gridDim.x - 1) / gridDim.x;
   const int64_t start = min(per * blockIdx.x, total);
-  const int64_t count = min(per, total - start);
+  const int count = (int)min(per, total - start);
   if (blockIdx.x == 0 && tid == 0) a.plan[0] = per;
   if (count > 0 || blockIdx.x == 0) {
     int64_t before = 0;
@@ -377,156 +440,162 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = T.tmem;
   const int unit0 = T.start_unit;
   const int64_t off0 = T.start_off;
+  // Chunks go through the ring as K0 K1 V0 K2 V1 ... V_last, or each tile's once when the values are the keys.
+  auto k_chunk = [&](uint32_t i) -> uint32_t { return a.shared ? i * NC : i == 0 ? 0 : 2 * NC * i - NC; };
+  auto v_chunk = [&](uint32_t i) -> uint32_t {
+    return a.shared ? i * NC : 2 * NC * (i + 1) - (i + 1 == (uint32_t)count ? NC : 0);
+  };
+  // Registers move from the issuing warpgroup to the accumulators: 56 + 2 x 120 + 216 = 4 x 128.
+  constexpr bool kSplitRegs = C::WG == 2;
 
-  if (warp == 0) {
-    // ------------------------------------------------------------ producer
-    Walk w;
-    w.start(a, R, unit0, off0, count);
-    const int ppt = kTok >> a.page_log2, page = 1 << a.page_log2;
-    uint32_t ci = 0;                   // chunks asked for so far
-    uint32_t tile = 0;
-    bool ok = true;
-    int v_pages = 0;                   // the previous tile's page row of this lane, for its values
-    bool v_pending = false;
-    const int oob = a.n_pages * a.Hkv; // a page row past the end: TMA fills zeros
-    auto chunks = [&](const CUtensorMap* m, int prow) {
-      for (int c = 0; c < NC && ok; ++c, ++ci) {
-        const uint32_t s = ci % a.slots, ph = (ci / a.slots) & 1;
-        ok = __all_sync(0xffffffffu, mbar_wait(&T.empty[s], ph ^ 1, abort_flag));
-        if (!ok) break;
-        if (lane == 0) mbar_arrive_expect_tx(&T.full[s], kChunk);
-        __syncwarp();
-        if (lane < ppt) tma_load_3d(smem + s * kChunk + lane * page * 128, m, &T.full[s], c * 128, 0, prow);
-        __syncwarp();
-      }
-    };
-    while (w.left > 0 && ok) {
-      const int t1 = w.seg_end(), t0 = w.t;
-      for (int t = t0; t < t1 && ok; ++t, ++tile) {
-        // this tile's pages and scales, one page per lane
-        int prow = oob;
-        float ks = 0.0f, vs = 0.0f;
+  if (warp < 4) {
+    if constexpr (kSplitRegs) reg_dec<56>();
+    if (warp == 0) {
+      // ---------------------------------------------------------- producer
+      const int ppt = kTok >> a.page_log2, page = 1 << a.page_log2;
+      const int per_batch = 32 / ppt;            // tiles whose pages fit the lanes
+      const int oob = a.n_pages * a.Hkv;         // a page row past the end: TMA fills zeros
+      // Page rows and scales of the next tiles, one page per lane, loaded while the previous batch is sent.
+      struct Batch {
+        int prow, n, t, limit, low, first, last;
+        uint32_t there;
+        float ks, vs;
+      };
+      Walk w;
+      w.start(a, R, unit0, off0, count);
+      auto load = [&](Batch& o) {
+        o.n = 0;
+        if (w.left <= 0) return;
+        const int end = w.seg_end();
+        o.t = w.t;
+        o.n = min(end - w.t, per_batch);
+        o.limit = w.limit;
+        o.low = row_limit(w.s, w.rt * R / a.G);      // rows of the tile see at least the first row's tokens
+        o.first = w.fresh;
+        o.last = w.t + o.n == end;
+        o.prow = oob;
+        o.ks = o.vs = 0.0f;
         bool there = false;
-        if (lane < ppt) {
-          const int64_t p = (int64_t)t * ppt + lane;
-          if ((p << a.page_log2) < w.limit) {
-            const int id = a.table[(int64_t)w.b * a.max_pages + p];
-            there = id >= 0 && id < a.n_pages;
-            if (there) {
-              prow = id * a.Hkv + w.h;
-              ks = a.k_scale[prow];
-              vs = a.shared ? ks : a.v_scale[prow];
-            } else {
-              bs_set_error(BS_ERR_BAD_INDEX);
-            }
+        const int64_t p = (int64_t)o.t * ppt + lane;
+        if (lane < o.n * ppt && (p << a.page_log2) < w.limit) {
+          const int id = a.table[(int64_t)w.b * a.max_pages + p];
+          there = id >= 0 && id < a.n_pages;
+          if (there) {
+            o.prow = id * a.Hkv + w.h;
+            o.ks = a.k_scale[o.prow];
+            o.vs = a.shared ? o.ks : a.v_scale[o.prow];
+          } else {
+            bs_set_error(BS_ERR_BAD_INDEX);
           }
         }
-        float unit = fabsf(vs);
-#pragma unroll
-        for (int o = 4; o > 0; o >>= 1) unit = fmaxf(unit, __shfl_xor_sync(0xffffffffu, unit, o));
-        const uint32_t valid = __ballot_sync(0xffffffffu, there) & 0xFFu;
-        // the first slot of the tile free: the entry's last reader is far behind
-        const uint32_t s = ci % a.slots, ph = (ci / a.slots) & 1;
-        ok = __all_sync(0xffffffffu, mbar_wait(&T.empty[s], ph ^ 1, abort_flag));
-        if (!ok) break;
-        Info& in = T.info[tile % kInfo];
-        if (lane < 8) {
-          in.ks[lane] = ks;
-          in.vs[lane] = vs;
+        o.there = __ballot_sync(0xffffffffu, there);
+        if (o.last) {
+          w.next(a, R);
+        } else {
+          w.t += o.n;
+          w.left -= o.n;
+          w.fresh = false;
         }
-        if (lane == 0) {
-          // rows of the tile see at least the first row's tokens
-          const int low = row_limit(w.s, w.rt * R / a.G);
-          in.unit = unit;
-          in.valid = (int)valid;
-          in.t0 = t * kTok;
-          in.limit = w.limit;
-          in.first = t == t0;
-          in.last = t + 1 == t1;
-          in.mask = (t + 1) * kTok > low || valid != (1u << ppt) - 1u;
-          // chunk order: K0 K1 V0 K2 V1 ... V_last (shared: every chunk once)
-          in.vslot = (int)(a.shared ? ci : 2 * NC * (tile + 1) - (tile + 1 == (uint32_t)count ? NC : 0));
-        }
-        __syncwarp();
-        chunks(&tm_k, prow);
-        if (!a.shared) {
-          if (v_pending && ok) chunks(&tm_v, v_pages);
-          v_pages = prow;
-          v_pending = true;
-        }
-      }
-      w.next(a, R);
-    }
-    if (v_pending && ok) chunks(&tm_v, v_pages);
-    // on the way out after a timeout: the copies in flight still write this CTA's shared memory
-    if (!ok) {
-      const uint32_t n = min(ci, (uint32_t)a.slots);
-      for (uint32_t k = 0; k < n; ++k) {
-        const uint32_t i = ci - 1 - k;
-        uint64_t t0 = 0;
-        for (uint32_t j = 0; j < BS_SPIN_LIMIT; ++j) {
-          if (mbar_try_wait(&T.full[i % a.slots], (i / a.slots) & 1)) break;
-          if (bs_wait_expired(j, &t0)) break;
-        }
-      }
-    }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------ MMA
-    const uint32_t idesc_s = idesc_f8f6f4(0, 0, 128, N);
-    const uint32_t idesc_o = idesc_f8f6f4(0, 0, 128, N) | (1u << 15) | (1u << 16);   // A and B along M / N
-    const uint64_t dk = sdesc_k128_sw128(smem_u32(smem));
-    const uint64_t dv = sdesc_mn_sw128(smem_u32(smem));
-    const uint64_t dq = sdesc_k128_sw128(smem_u32(qbuf));
-    const uint64_t dp = sdesc_mn_plain(smem_u32(pbuf));
-    uint32_t ci = 0;                 // chunks consumed, in the producer's order
-    uint32_t vprev = 0;              // first value chunk of the previous tile (shared)
-    int seg = -1;
-    bool ok = true;
-    auto wait = [&](uint64_t* bar, uint32_t ph) {
-      ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, ph, abort_flag));
-    };
-    for (int64_t i = 0; i <= count && ok && count > 0; ++i) {
-      uint32_t kfirst = ci;
-      if (i < count) {
-        const int sb = (int)(i % C::SB);
-        for (int c = 0; c < NC; ++c) wait(&T.full[(ci + c) % a.slots], ((ci + c) / a.slots) & 1);
-        if (!ok) break;
-        if (T.info[i % kInfo].first) {
-          ++seg;
-          wait(&T.q_full[seg & 1], (seg >> 1) & 1);
-        }
-        wait(&T.s_empty[sb], ((i / C::SB) & 1) ^ 1);
-        if (!ok) break;
-        tc_fence_after();
-        if (elect_one()) {
-#pragma unroll
-          for (int c = 0; c < NC; ++c) {
-            const uint64_t da = dk + (uint64_t)(((ci + c) % a.slots) * kChunk >> 4);
-            const uint64_t db = dq + (uint64_t)(((seg & 1) * C::kQBytes + c * N * 128) >> 4);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) tc_mma_f8f6f4(tmem + sb * N, da + 2 * k, db + 2 * k, idesc_s, (c | k) != 0);
+      };
+      uint32_t slot = 0, phase = 1, sent = 0;
+      bool ok = true;
+      auto chunks = [&](const CUtensorMap* m, int prow) {
+        for (int c = 0; c < NC && ok; ++c) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&T.empty[slot], phase, abort_flag));
+          if (!ok) break;
+          if (lane == 0) mbar_arrive_expect_tx(&T.full[slot], kChunk);
+          __syncwarp();
+          if (lane < ppt) tma_load_3d(smem + slot * kChunk + lane * page * 128, m, &T.full[slot], c * 128, 0, prow);
+          __syncwarp();
+          ++sent;
+          if (++slot == SLOTS) {
+            slot = 0;
+            phase ^= 1;
           }
-          if (!a.shared)
-            for (int c = 0; c < NC; ++c) tc_commit(&T.empty[(ci + c) % a.slots]);
-          tc_commit(&T.s_full[sb]);
         }
-        __syncwarp();
-        ci += NC;
+      };
+      Batch cur, nxt;
+      load(cur);
+      load(nxt);
+      int v_prow = 0;                            // the previous tile's page row of this lane, for its values
+      bool v_pending = false;
+      uint32_t tile = 0;
+      while (cur.n > 0 && ok) {
+        for (int k = 0; k < cur.n && ok; ++k, ++tile) {
+          const int src = (k * ppt + (lane & (ppt - 1))) & 31;
+          const int prow = __shfl_sync(0xffffffffu, cur.prow, src);
+          const float ks = __shfl_sync(0xffffffffu, cur.ks, src), vs = __shfl_sync(0xffffffffu, cur.vs, src);
+          const uint32_t valid = (cur.there >> (k * ppt)) & ((1u << ppt) - 1u);
+          float unit = fabsf(vs);
+#pragma unroll
+          for (int o = 4; o > 0; o >>= 1) unit = fmaxf(unit, __shfl_xor_sync(0xffffffffu, unit, o));
+          // the first slot of the tile free: the entry's last reader is far behind
+          ok = __all_sync(0xffffffffu, mbar_wait(&T.empty[slot], phase, abort_flag));
+          if (!ok) break;
+          Info& in = T.info[tile % kInfo];
+          if (lane < 8) {
+            in.ks[lane] = ks;
+            in.vr[lane] = unit > 0.0f ? 256.0f * (vs / unit) : 0.0f;
+          }
+          if (lane == 0) {
+            const int t = cur.t + k;
+            in.unit = unit;
+            in.valid = (int)valid;
+            in.t0 = t * kTok;
+            in.limit = cur.limit;
+            in.first = cur.first && k == 0;
+            in.last = cur.last && k + 1 == cur.n;
+            in.mask = (t + 1) * kTok > cur.low || valid != (1u << ppt) - 1u;
+          }
+          __syncwarp();
+          chunks(&tm_k, prow);
+          if (!a.shared) {
+            if (v_pending && ok) chunks(&tm_v, v_prow);
+            v_prow = prow;
+            v_pending = true;
+          }
+        }
+        cur = nxt;
+        load(nxt);
       }
-      if (i > 0) {
-        const int64_t j = i - 1;
-        const int pb = (int)(j & 1), ob = (int)(j % C::OB);
-        const uint32_t v0 = a.shared ? vprev : ci;
+      if (v_pending && ok) chunks(&tm_v, v_prow);
+      // on the way out after a timeout: the copies in flight still write this CTA's shared memory
+      if (!ok) {
+        const uint32_t n = min(sent, SLOTS);
+        for (uint32_t k = 0; k < n; ++k) {
+          const uint32_t i = sent - 1 - k;
+          uint64_t t0 = 0;
+          for (uint32_t j = 0; j < BS_SPIN_LIMIT; ++j) {
+            if (mbar_try_wait(&T.full[i % SLOTS], (i / SLOTS) & 1)) break;
+            if (bs_wait_expired(j, &t0)) break;
+          }
+        }
+      }
+    } else if (warp == 1) {
+      // ---------------------------------------------------------- MMA
+      constexpr uint32_t idesc_s = idesc_f8f6f4(0, 0, 128, N);
+      constexpr uint32_t idesc_o = idesc_s | (1u << 15) | (1u << 16);   // A and B along M / N
+      const uint64_t dk = sdesc_k128_sw128(smem_u32(smem));
+      const uint64_t dv = sdesc_mn_sw128(smem_u32(smem));
+      const uint64_t dq = sdesc_k128_sw128(smem_u32(qbuf));
+      const uint64_t dp = sdesc_mn_plain(smem_u32(pbuf));
+      int seg = -1;
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, uint32_t ph) {
+        ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, ph, abort_flag));
+      };
+      auto products_pv = [&](uint32_t j) {
+        const uint32_t pb = j & 1, ob = j % C::OB, v0 = v_chunk(j);
         wait(&T.p_full[pb], (j >> 1) & 1);
         wait(&T.o_empty[ob], ((j / C::OB) & 1) ^ 1);
         if (!a.shared)
-          for (int c = 0; c < NC; ++c) wait(&T.full[(v0 + c) % a.slots], ((v0 + c) / a.slots) & 1);
-        if (!ok) break;
+          for (uint32_t c = 0; c < NC; ++c) wait(&T.full[(v0 + c) % SLOTS], ((v0 + c) / SLOTS) & 1);
+        if (!ok) return;
         tc_fence_after();
         if (elect_one()) {
 #pragma unroll
           for (int c = 0; c < NC; ++c) {
-            const uint32_t s = (v0 + c) % a.slots;
+            const uint32_t s = (v0 + c) % SLOTS;
             const uint64_t da = dv + (uint64_t)(s * kChunk >> 4);
             const uint64_t db = dp + (uint64_t)(pb * C::kPBytes >> 4);
 #pragma unroll
@@ -537,117 +606,174 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc_commit(&T.o_full[ob]);
         }
         __syncwarp();
-        if (!a.shared) ci += NC;
+      };
+      for (uint32_t i = 0; i <= (uint32_t)count && ok && count > 0; ++i) {
+        bool pv_done = i == 0;
+        if (i < (uint32_t)count) {
+          const uint32_t sb = i % C::SB, k0 = k_chunk(i);
+          for (uint32_t c = 0; c < NC; ++c) wait(&T.full[(k0 + c) % SLOTS], ((k0 + c) / SLOTS) & 1);
+          if (!ok) break;
+          if (T.info[i % kInfo].first) {
+            ++seg;
+            // with one Q buffer the next segment's rows come in when the last O tile of this one is out
+            if (C::QB == 1 && !pv_done) {
+              products_pv(i - 1);
+              pv_done = true;
+            }
+            wait(&T.q_full[seg % C::QB], (seg / C::QB) & 1);
+          }
+          wait(&T.s_empty[sb], ((i / C::SB) & 1) ^ 1);
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_one()) {
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+              const uint64_t da = dk + (uint64_t)(((k0 + c) % SLOTS) * kChunk >> 4);
+              const uint64_t db = dq + (uint64_t)(((seg % C::QB) * C::kQBytes + c * N * 128) >> 4);
+#pragma unroll
+              for (int k = 0; k < 4; ++k) tc_mma_f8f6f4(tmem + sb * N, da + 2 * k, db + 2 * k, idesc_s, (c | k) != 0);
+              if (!a.shared) tc_commit(&T.empty[(k0 + c) % SLOTS]);
+            }
+            tc_commit(&T.s_full[sb]);
+          }
+          __syncwarp();
+        }
+        if (!pv_done) products_pv(i - 1);
       }
-      vprev = kfirst;
     }
-  } else if (warp < 6) {
-    // ------------------------------------------------------------ softmax: one token per thread
-    const int quad = warp & 3;
-    const int tok = quad * 32 + lane;
-    const int row = (warp - 2) * 32 + lane;      // < R: the row whose maximum this thread keeps
-    const uint32_t lane_base = (uint32_t)(quad * 32) << 16;
-    float l[R];
-    float m_old = -INFINITY;
+  } else if (warp < 4 + 4 * C::WG) {
+    // ------------------------------------------------------------ softmax
+    // A thread holds tokens tok0 + 8k (k = 0..3) of rows row0 + 8g + {0, 1} (g < K).
+    if constexpr (kSplitRegs) reg_dec<120>();
+    constexpr int RW = C::RW, K = RW / 8;
+    const int wg = (warp >> 2) - 1, quad = warp & 3;
+    const int tok0 = quad * 32 + (lane >> 2);
+    const int row0 = wg * RW + 2 * (lane & 3);
+    const uint32_t t_lane = tmem + ((uint32_t)(quad * 32) << 16) + wg * RW;
+    float l[K][2], m[K][2], qf[K][2];
     int seg = -1;
     bool dead = false;
-#pragma unroll
-    for (int r = 0; r < R; ++r) l[r] = 0.0f;
-    for (int64_t i = 0; i < count; ++i) {
-      const int sb = (int)(i % C::SB), pb = (int)(i & 1);
+    for (int i = 0; i < count; ++i) {
+      const int sb = i % C::SB, pb = i & 1;
       const Info& in = T.info[i % kInfo];
-      float s[R];
-      bool ok = __all_sync(0xffffffffu, mbar_wait(&T.s_full[sb], (i / C::SB) & 1, abort_flag)) && !dead;
-      bool first = false, last = false;
-      float ratio = 0.0f;
+      const bool ok = __all_sync(0xffffffffu, mbar_wait(&T.s_full[sb], (i / C::SB) & 1, abort_flag)) && !dead;
+      float s[K][4][2];
       if (ok) {
         tc_fence_after();
-        load_rows<R, PP>(tmem + lane_base + sb * N, s);
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&T.s_empty[sb]);
-        first = in.first;
-        last = in.last;
-        if (first) {
-          ++seg;
-          m_old = -INFINITY;
+        {
+          uint32_t v[2][PP][4 * K];
 #pragma unroll
-          for (int r = 0; r < R; ++r) l[r] = 0.0f;
-        }
-        const int pg = tok >> a.page_log2;
-        const float ks = in.ks[pg];
-        ratio = in.unit > 0.0f ? 256.0f * (in.vs[pg] / in.unit) : 0.0f;
-        const float* qf = T.qf[seg & 1];
+          for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int r = 0; r < R; ++r) s[r] *= qf[r] * ks;
-        if (in.mask) {
-          const int t = in.t0 + tok;
-          const bool there = (in.valid >> pg) & 1;
-          const int* lim = T.lim[seg & 1];
+            for (int p = 0; p < PP; ++p) tmem_ld16x256<K>(t_lane + ((uint32_t)(16 * h) << 16) + sb * N + p * R, v[h][p]);
+          if (in.first) {
+            ++seg;
 #pragma unroll
-          for (int r = 0; r < R; ++r)
-            if (!there || t >= lim[r]) s[r] = -INFINITY;
-        }
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-          const float m = redux_max(s[r]);
-          if (lane == 0) T.wmax[quad][r] = m;
-        }
-      }
-      if (!group_all(ok)) break;
-      if (row < R) {
-        const float m = fmaxf(fmaxf(fmaxf(T.wmax[0][row], T.wmax[1][row]), fmaxf(T.wmax[2][row], T.wmax[3][row])), m_old);
-        const float use = m == -INFINITY ? 0.0f : m;     // no token seen yet
-        T.muse[row] = use;
-        T.alpha[i & 3][row] = exp2f(m_old - use);
-        m_old = m;
-        if (last) T.mfin[seg % kSegRing][row] = m;
-      }
-      group_sync();
-      const float* muse = T.muse;
-      const float* al = T.alpha[i & 3];
-      uint8_t* p = pbuf + pb * C::kPBytes + tok * 16;
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        s[r] = exp2f(s[r] - muse[r]);
-        l[r] = fmaf(l[r], al[r], s[r]);
-      }
-      if constexpr (R == 8) {
-        uint32_t w[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-#pragma unroll
-        for (int r = 0; r < 8; r += 2) {
-          uint16_t c[PP];
-          split2<PP>(s[r] * ratio, s[r + 1] * ratio, c);
-#pragma unroll
-          for (int k = 0; k < PP; ++k) w[2 * k + (r >> 2)] |= (uint32_t)c[k] << (16 * ((r >> 1) & 1));
-        }
-        *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-        if (PP == 3) *reinterpret_cast<uint4*>(p + 2048) = make_uint4(w[4], w[5], 0, 0);
-      } else {
-#pragma unroll
-        for (int g = 0; g < R / 16; ++g) {
-          uint32_t w[PP][4];
-#pragma unroll
-          for (int r = 0; r < 16; r += 4) {
-            uint16_t c[PP], d[PP];
-            split2<PP>(s[g * 16 + r] * ratio, s[g * 16 + r + 1] * ratio, c);
-            split2<PP>(s[g * 16 + r + 2] * ratio, s[g * 16 + r + 3] * ratio, d);
-#pragma unroll
-            for (int k = 0; k < PP; ++k) w[k][r >> 2] = (uint32_t)c[k] | ((uint32_t)d[k] << 16);
+            for (int g = 0; g < K; ++g) {
+              const float2 f = *reinterpret_cast<const float2*>(&T.qf[seg & 1][row0 + 8 * g]);
+              qf[g][0] = f.x;
+              qf[g][1] = f.y;
+              m[g][0] = m[g][1] = -INFINITY;
+              l[g][0] = l[g][1] = 0.0f;
+            }
           }
+          float ks[4];
 #pragma unroll
-          for (int k = 0; k < PP; ++k)
-            *reinterpret_cast<uint4*>(p + (k * (R / 16) + g) * 2048) = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
+          for (int k = 0; k < 4; ++k) ks[k] = in.ks[(tok0 + 8 * k) >> a.page_log2];
+          tmem_ld_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&T.s_empty[sb]);
+#pragma unroll
+          for (int g = 0; g < K; ++g)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                const int at = 4 * g + 2 * (k & 1) + j;
+                float x = __uint_as_float(v[k >> 1][PP - 1][at]);
+#pragma unroll
+                for (int p = PP - 2; p >= 0; --p) x = fmaf(x, 0.0625f, __uint_as_float(v[k >> 1][p][at]));
+                s[g][k][j] = x * ks[k];
+              }
+        }
+        if (in.mask) {
+#pragma unroll
+          for (int g = 0; g < K; ++g) {
+            const int2 lim = *reinterpret_cast<const int2*>(&T.lim[seg & 1][row0 + 8 * g]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int tok = tok0 + 8 * k, t = in.t0 + tok;
+              const bool there = (in.valid >> (tok >> a.page_log2)) & 1;
+              if (!there || t >= lim.x) s[g][k][0] = -INFINITY;
+              if (!there || t >= lim.y) s[g][k][1] = -INFINITY;
+            }
+          }
+        }
+#pragma unroll
+        for (int g = 0; g < K; ++g) {
+          float x[2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            x[j] = fmaxf(fmaxf(s[g][0][j], s[g][1][j]), fmaxf(s[g][2][j], s[g][3][j]));
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) x[j] = fmaxf(x[j], __shfl_xor_sync(0xffffffffu, x[j], o));
+          }
+          if (lane < 4)
+            *reinterpret_cast<float2*>(&T.wmax[i & 1][quad][row0 + 8 * g]) = make_float2(x[0] * qf[g][0], x[1] * qf[g][1]);
         }
       }
-      if (in.mask) {
+      // one barrier a tile: wmax has two buffers
+      if (!group_all(1 + wg, ok)) break;
+      const bool last = in.last;
+#pragma unroll
+      for (int g = 0; g < K; ++g) {
+        float2 x[4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) x[w] = *reinterpret_cast<const float2*>(&T.wmax[i & 1][w][row0 + 8 * g]);
+        float al[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float t = j ? fmaxf(fmaxf(x[0].y, x[1].y), fmaxf(x[2].y, x[3].y))
+                            : fmaxf(fmaxf(x[0].x, x[1].x), fmaxf(x[2].x, x[3].x));
+          const float now = fmaxf(m[g][j], t);
+          const float use = now == -INFINITY ? 0.0f : now;       // no token seen yet
+          al[j] = ex2(m[g][j] - use);
+          m[g][j] = now;
+          float sum = 0.0f;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            s[g][k][j] = ex2(fmaf(s[g][k][j], qf[g][j], -use));
+            sum += s[g][k][j];
+          }
+          l[g][j] = fmaf(l[g][j], al[j], sum);
+        }
+        if (quad == 0 && lane < 4) *reinterpret_cast<float2*>(&T.alpha[i & 3][row0 + 8 * g]) = make_float2(al[0], al[1]);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int tok = tok0 + 8 * k;
+        const float ratio = in.vr[tok >> a.page_log2];
+        uint8_t* p = pbuf + pb * C::kPBytes + tok * 16;
+#pragma unroll
+        for (int g = 0; g < K; ++g) {
+          uint16_t c[PP];
+          split2h<PP>(s[g][k][0] * ratio, s[g][k][1] * ratio, c);
+#pragma unroll
+          for (int t = 0; t < PP; ++t) {
+            const int n = t * R + row0 + 8 * g;
+            *reinterpret_cast<uint16_t*>(p + (n >> 4) * 2048 + (n & 15)) = c[t];
+          }
+        }
+      }
+      if (in.mask && wg == 0) {
         // Values that some row must not see: 0 x NaN would reach its sum.  Rows that no query sees become zero; a NaN
         // in a row that only some see becomes zero too, and is put back for those when the segment ends.
-        const int t = in.t0 + tok;
+        const int tok = quad * 32 + lane, t = in.t0 + tok;
         for (int c = 0; c < NC; ++c) {
-          const uint32_t v = (uint32_t)in.vslot + c;
-          if (!a.shared && !__all_sync(0xffffffffu, mbar_wait(&T.full[v % a.slots], (v / a.slots) & 1, abort_flag))) dead = true;
-          uint4* row16 = reinterpret_cast<uint4*>(smem + (v % a.slots) * kChunk + tok * 128);
+          const uint32_t v = v_chunk(i) + c;
+          if (!a.shared && !__all_sync(0xffffffffu, mbar_wait(&T.full[v % SLOTS], (v / SLOTS) & 1, abort_flag))) dead = true;
+          uint4* row16 = reinterpret_cast<uint4*>(smem + (v % SLOTS) * kChunk + tok * 128);
           for (int k = 0; k < 8; ++k) {
             // the swizzle has the row's dims 16 k .. 16 k + 15 in this 16-byte unit
             uint4* vr = row16 + (k ^ (tok & 7));
@@ -679,11 +805,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) mbar_arrive(&T.p_full[pb]);
       if (last) {
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-          float x = l[r];
+        for (int g = 0; g < K; ++g) {
+          float x[2];
 #pragma unroll
-          for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-          if (lane == 0) T.lsum[seg % kSegRing][quad][r] = x;
+          for (int j = 0; j < 2; ++j) {
+            x[j] = l[g][j];
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) x[j] += __shfl_xor_sync(0xffffffffu, x[j], o);
+          }
+          if (lane < 4) {
+            *reinterpret_cast<float2*>(&T.lsum[seg % kSegRing][quad][row0 + 8 * g]) = make_float2(x[0], x[1]);
+            if (quad == 0) *reinterpret_cast<float2*>(&T.mfin[seg % kSegRing][row0 + 8 * g]) = make_float2(m[g][0], m[g][1]);
+          }
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&T.l_full[seg % kSegRing]);
@@ -691,13 +824,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     // ------------------------------------------------------------ Q in, O out
+    if constexpr (kSplitRegs) reg_inc<216>();
     const int quad = warp & 3;
     const uint32_t lane_base = (uint32_t)(quad * 32) << 16;
-    const int wq = warp - 6;
     // One warp per row: amax, power-of-two scale, terms, swizzled store.
-    auto stage = [&](const Walk& w, int buf) {
-      uint8_t* qb = qbuf + buf * C::kQBytes;
-      for (int r = wq; r < R; r += 4) {
+    auto stage = [&](const Walk& w, int seg) {
+      uint8_t* qb = qbuf + (seg % C::QB) * C::kQBytes;
+      const int buf = seg & 1;
+      for (int r = quad; r < R; r += 4) {
         const int rr = w.rt * R + r;
         const int i = rr / a.G, g = rr - i * a.G;
         const bool in = rr < a.S * a.G;
@@ -733,6 +867,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         float up = __uint_as_float((uint32_t)(127 + e) << 23);
         const float down = __uint_as_float((uint32_t)(127 - e) << 23);
         if (amax == __uint_as_float(0x7F800000u)) up = __uint_as_float(0x7FC00000u);   // e4m3 would saturate it
+        if (a.scale_log2 < 0.0f) up = -up;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
           uint16_t lo[PP], hi[PP];
@@ -746,32 +881,33 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         if (lane == 0) {
-          T.qf[buf][r] = down * a.scale_log2;
+          // not zero: a hidden token's -inf times it has to stay -inf
+          T.qf[buf][r] = fmaxf(down * fabsf(a.scale_log2), 1e-35f);
           T.lim[buf][r] = in ? row_limit(w.s, i) : 0;
           T.off[buf][r] = in && i < w.s.nl ? (((int64_t)w.b * a.S + i) * a.H + w.h * a.G + g) * a.D : -1;
         }
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&T.q_full[buf]);
+      if (lane == 0) mbar_arrive(&T.q_full[seg % C::QB]);
     };
     Walk w;
     w.start(a, R, unit0, off0, count);
     if (w.left > 0) stage(w, 0);
-    int64_t i = 0;
+    int i = 0;
     bool ok = true;
     for (int seg = 0; w.left > 0 && ok; ++seg) {
       const int t0 = w.t, t1 = w.seg_end(), nt = w.nt;
       w.next(a, R);
       // the other Q buffer: its last products are behind the O tiles taken out before
-      if (w.left > 0) stage(w, (seg + 1) & 1);
+      if (C::QB == 2 && w.left > 0) stage(w, seg + 1);
       float acc[NC][R];
 #pragma unroll
       for (int c = 0; c < NC; ++c)
 #pragma unroll
         for (int r = 0; r < R; ++r) acc[c][r] = 0.0f;
       for (int t = t0; t < t1; ++t, ++i) {
-        const int ob = (int)(i % C::OB);
+        const int ob = i % C::OB;
         ok = __all_sync(0xffffffffu, mbar_wait(&T.o_full[ob], (i / C::OB) & 1, abort_flag));
         if (!ok) break;
         tc_fence_after();
@@ -789,6 +925,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive(&T.o_empty[ob]);
       }
       if (!ok) break;
+      if (C::QB == 1 && w.left > 0) stage(w, seg + 1);
       const int sr = seg % kSegRing;
       ok = __all_sync(0xffffffffu, mbar_wait(&T.l_full[sr], (seg / kSegRing) & 1, abort_flag));
       if (!ok) break;
@@ -949,23 +1086,18 @@ Layout layout(int64_t B, int64_t S, int H, int Hkv, int D, int f16) {
 }
 
 template <int R, int PP, int NC>
-cudaError_t launch(const CUtensorMap& mk, const CUtensorMap& mv, Args a, int grid, cudaStream_t st) {
+cudaError_t launch(const CUtensorMap& mk, const CUtensorMap& mv, const Args& a, int grid, cudaStream_t st) {
   using C = Cfg<R, PP, NC>;
   auto kern = cache_attn_kernel<R, PP, NC>;
-  // as many chunks as fit, with two tiles at least (the next tile's keys arrive before this one's values are used up)
-  int slots = kMaxSlots;
-  while (C::smem(slots) > 227 * 1024) --slots;
-  if (slots < 2 * NC) return cudaErrorInvalidConfiguration;
-  a.slots = slots;
   static int done[hostcache::kMaxDevices];
   cudaError_t e = (cudaError_t)hostcache::get(done, [&] {
-    return (int)cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::smem(slots));
+    return (int)cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
   });
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = C::smem(slots);
+  cfg.blockDim = dim3(C::kThreads);
+  cfg.dynamicSmemBytes = C::kSmem;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
