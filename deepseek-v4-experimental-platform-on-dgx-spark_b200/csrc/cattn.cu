@@ -32,7 +32,8 @@
 // head's tokens, both sides leave partial results (unnormalised O, max, sum)
 // and a second kernel joins them.  Lengths are read on the device only.
 //
-// Roles: one warpgroup with the TMA producer and the MMA issuer; one or (from
+// Roles: one warpgroup with the TMA producer and an issuer for each of the two
+// products; one or (from
 // 32 rows on) two softmax warpgroups, each with its share of the rows; one
 // that stages Q and accumulates O, one head dim per thread and 128-dim chunk.
 // Shared memory: a ring of 16 KB chunks, Q (this segment's and, where it fits,
@@ -168,7 +169,7 @@ struct Cfg {
     int nanmin[kSegRing][NC * 128]; // first token with a NaN value in partly hidden tiles
     int nanseen[kSegRing];
     uint64_t full[kMaxSlots], empty[kMaxSlots];
-    uint64_t s_full[2], s_empty[2], p_full[2], o_full[2], o_empty[2], q_full[2], l_full[kSegRing];
+    uint64_t s_full[2], s_empty[2], p_full[2], p_empty[2], o_full[2], o_empty[2], q_full[2], l_full[kSegRing], v_ready;
     uint32_t tmem;
     int abort;
     int64_t scan[16];
@@ -176,10 +177,17 @@ struct Cfg {
     int start_unit;
   };
   static constexpr int kFixed = 1024 + QB * kQBytes + 2 * kPBytes + (int)sizeof(Tail);
-  static constexpr int kFit = (227 * 1024 - kFixed) / kChunk;
+  // Two CTAs an SM for the small row tiles of a decode step: a tile's chain of waits (keys, S, maximum, P, O) is longer
+  // than its bytes take, and two such chains overlap.
+  static constexpr int kCtas = NC == 1 && R <= 16 ? 2 : 1;
+  static_assert(kCtas * kTmem <= 512, "TMEM of the resident CTAs");
+  static constexpr int kFit = ((kCtas == 2 ? 113 : 227) * 1024 - kFixed) / kChunk;
   static constexpr int kSlots = kFit < kMaxSlots ? kFit : kMaxSlots;
-  // two tiles at least: the next tile's keys are used before this one's values
-  static_assert(kSlots >= 2 * NC, "ring");
+  // Separate rings for keys and values: each product's issuer then sees every phase of the barriers it waits for.  (In
+  // one ring of mixed chunks a slot's previous phase could belong to the other product, still incomplete, and a parity
+  // wait takes a phase two ahead for one that is over.)  Values that are the keys use one ring of all slots.
+  static constexpr int kVSlots = kSlots / 2, kKSlots = kSlots - kVSlots;
+  static_assert(kVSlots >= NC && kSlots + 4 <= kInfo, "rings");
   static constexpr int kSmem = kFixed + kSlots * kChunk;
 };
 
@@ -202,6 +210,19 @@ BS_DEVINL uint64_t sdesc_mn_plain(uint32_t addr) {
   d |= (uint64_t)(2048 >> 4) << 32;
   d |= (uint64_t)1 << 46;
   return d;
+}
+
+// mbar_wait behind a non-suspending probe.  A phase that is over costs 7 cycles this way and 70 with try_wait.
+BS_DEVINL bool wait_quick(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  return mbar_test_wait(bar, parity) || mbar_wait(bar, parity, abort);
+}
+// A whole warp waits, each lane for its own barrier (lanes with active = false for none).  The first probe does not
+// diverge; lanes that have to wait for good then do so one after another.
+BS_DEVINL bool warp_wait(uint64_t* bar, uint32_t parity, bool active, volatile int* abort) {
+  bool ok = !active || mbar_test_wait(bar, parity);
+  if (__all_sync(0xffffffffu, ok)) return true;
+  if (!ok) ok = mbar_wait(bar, parity, abort);
+  return __all_sync(0xffffffffu, ok);
 }
 
 BS_DEVINL float redux_max(float v) {
@@ -338,7 +359,7 @@ BS_DEVINL void load_rows(uint32_t taddr, float* s) {
 BS_DEVINL uint32_t nan_bytes(uint32_t v) { return ((v & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; }
 
 template <int R, int PP, int NC>
-__global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, 1)
+__global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCtas)
     cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const Args a) {
   using C = Cfg<R, PP, NC>;
   constexpr int N = C::N, kThreads = C::kThreads;
@@ -360,11 +381,13 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, 1)
       mbar_init(&T.s_full[i], 1);
       mbar_init(&T.s_empty[i], 4 * C::WG);
       mbar_init(&T.p_full[i], 4 * C::WG);
+      mbar_init(&T.p_empty[i], 1);
       mbar_init(&T.o_full[i], 1);
       mbar_init(&T.o_empty[i], 4);
       mbar_init(&T.q_full[i], 4);
     }
     for (int i = 0; i < kSegRing; ++i) mbar_init(&T.l_full[i], 4 * C::WG);
+    mbar_init(&T.v_ready, 1);
     T.abort = 0;
     T.start_unit = 0;
     T.start_off = 0;
@@ -440,11 +463,12 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, 1)
   const uint32_t tmem = T.tmem;
   const int unit0 = T.start_unit;
   const int64_t off0 = T.start_off;
-  // Chunks go through the ring as K0 K1 V0 K2 V1 ... V_last, or each tile's once when the values are the keys.
-  auto k_chunk = [&](uint32_t i) -> uint32_t { return a.shared ? i * NC : i == 0 ? 0 : 2 * NC * i - NC; };
-  auto v_chunk = [&](uint32_t i) -> uint32_t {
-    return a.shared ? i * NC : 2 * NC * (i + 1) - (i + 1 == (uint32_t)count ? NC : 0);
-  };
+  // Slot of a running chunk number (tile x NC + c) and the parity of its phase.
+  constexpr uint32_t KS = C::kKSlots, VS = C::kVSlots;
+  auto k_slot = [&](uint32_t n) -> uint32_t { return a.shared ? n % SLOTS : n % KS; };
+  auto k_par = [&](uint32_t n) -> uint32_t { return (a.shared ? n / SLOTS : n / KS) & 1; };
+  auto v_slot = [&](uint32_t n) -> uint32_t { return a.shared ? n % SLOTS : KS + n % VS; };
+  auto v_par = [&](uint32_t n) -> uint32_t { return (a.shared ? n / SLOTS : n / VS) & 1; };
   // Registers move from the issuing warpgroup to the accumulators: 56 + 2 x 120 + 216 = 4 x 128.
   constexpr bool kSplitRegs = C::WG == 2;
 
@@ -497,21 +521,26 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, 1)
           w.fresh = false;
         }
       };
-      uint32_t slot = 0, phase = 1, sent = 0;
+      uint32_t k_sent = 0, v_sent = 0;           // chunks
       bool ok = true;
-      auto chunks = [&](const CUtensorMap* m, int prow) {
+      auto chunk = [&](const CUtensorMap* m, uint32_t slot, uint32_t parity, int x, int prow) {
+        ok = ok && __all_sync(0xffffffffu, wait_quick(&T.empty[slot], parity ^ 1, abort_flag));
+        if (!ok) return;
+        if (lane == 0) mbar_arrive_expect_tx(&T.full[slot], kChunk);
+        __syncwarp();
+        if (lane < ppt) tma_load_3d(smem + slot * kChunk + lane * page * 128, m, &T.full[slot], x, 0, prow);
+        __syncwarp();
+      };
+      auto k_chunks = [&](int prow) {
         for (int c = 0; c < NC && ok; ++c) {
-          ok = __all_sync(0xffffffffu, mbar_wait(&T.empty[slot], phase, abort_flag));
-          if (!ok) break;
-          if (lane == 0) mbar_arrive_expect_tx(&T.full[slot], kChunk);
-          __syncwarp();
-          if (lane < ppt) tma_load_3d(smem + slot * kChunk + lane * page * 128, m, &T.full[slot], c * 128, 0, prow);
-          __syncwarp();
-          ++sent;
-          if (++slot == SLOTS) {
-            slot = 0;
-            phase ^= 1;
-          }
+          chunk(&tm_k, k_slot(k_sent), k_par(k_sent), c * 128, prow);
+          k_sent += ok;
+        }
+      };
+      auto v_chunks = [&](int prow) {
+        for (int c = 0; c < NC && ok; ++c) {
+          chunk(&tm_v, v_slot(v_sent), v_par(v_sent), c * 128, prow);
+          v_sent += ok;
         }
       };
       Batch cur, nxt;
@@ -530,7 +559,7 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, 1)
 #pragma unroll
           for (int o = 4; o > 0; o >>= 1) unit = fmaxf(unit, __shfl_xor_sync(0xffffffffu, unit, o));
           // the first slot of the tile free: the entry's last reader is far behind
-          ok = __all_sync(0xffffffffu, mbar_wait(&T.empty[slot], phase, abort_flag));
+          ok = __all_sync(0xffffffffu, wait_quick(&T.empty[k_slot(k_sent)], k_par(k_sent) ^ 1, abort_flag));
           if (!ok) break;
           Info& in = T.info[tile % kInfo];
           if (lane < 8) {
@@ -548,9 +577,9 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, 1)
             in.mask = (t + 1) * kTok > cur.low || valid != (1u << ppt) - 1u;
           }
           __syncwarp();
-          chunks(&tm_k, prow);
+          k_chunks(prow);
           if (!a.shared) {
-            if (v_pending && ok) chunks(&tm_v, v_prow);
+            if (v_pending && ok) v_chunks(v_prow);
             v_prow = prow;
             v_pending = true;
           }
@@ -558,87 +587,81 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, 1)
         cur = nxt;
         load(nxt);
       }
-      if (v_pending && ok) chunks(&tm_v, v_prow);
+      if (v_pending && ok) v_chunks(v_prow);
       // on the way out after a timeout: the copies in flight still write this CTA's shared memory
       if (!ok) {
-        const uint32_t n = min(sent, SLOTS);
-        for (uint32_t k = 0; k < n; ++k) {
-          const uint32_t i = sent - 1 - k;
+        auto drain = [&](uint32_t slot, uint32_t parity) {
           uint64_t t0 = 0;
-          for (uint32_t j = 0; j < BS_SPIN_LIMIT; ++j) {
-            if (mbar_try_wait(&T.full[i % SLOTS], (i / SLOTS) & 1)) break;
-            if (bs_wait_expired(j, &t0)) break;
-          }
-        }
+          for (uint32_t j = 0; j < BS_SPIN_LIMIT; ++j)
+            if (mbar_try_wait(&T.full[slot], parity) || bs_wait_expired(j, &t0)) break;
+        };
+        const uint32_t nk = min(k_sent, a.shared ? SLOTS : KS), nv = min(v_sent, VS);
+        for (uint32_t k = 1; k <= nk; ++k) drain(k_slot(k_sent - k), k_par(k_sent - k));
+        for (uint32_t k = 1; k <= nv; ++k) drain(v_slot(v_sent - k), v_par(v_sent - k));
       }
     } else if (warp == 1) {
-      // ---------------------------------------------------------- MMA
-      constexpr uint32_t idesc_s = idesc_f8f6f4(0, 0, 128, N);
-      constexpr uint32_t idesc_o = idesc_s | (1u << 15) | (1u << 16);   // A and B along M / N
+      // ---------------------------------------------------------- S = K Q^T
+      // One lane per barrier: the waits of a tile one after another, in one warp for both products, took longer than
+      // its products (1925 cycles a tile of 128 x 128).
+      constexpr uint32_t idesc = idesc_f8f6f4(0, 0, 128, N);
       const uint64_t dk = sdesc_k128_sw128(smem_u32(smem));
-      const uint64_t dv = sdesc_mn_sw128(smem_u32(smem));
       const uint64_t dq = sdesc_k128_sw128(smem_u32(qbuf));
-      const uint64_t dp = sdesc_mn_plain(smem_u32(pbuf));
       int seg = -1;
-      bool ok = true;
-      auto wait = [&](uint64_t* bar, uint32_t ph) {
-        ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, ph, abort_flag));
-      };
-      auto products_pv = [&](uint32_t j) {
-        const uint32_t pb = j & 1, ob = j % C::OB, v0 = v_chunk(j);
-        wait(&T.p_full[pb], (j >> 1) & 1);
-        wait(&T.o_empty[ob], ((j / C::OB) & 1) ^ 1);
-        if (!a.shared)
-          for (uint32_t c = 0; c < NC; ++c) wait(&T.full[(v0 + c) % SLOTS], ((v0 + c) / SLOTS) & 1);
-        if (!ok) return;
+      for (uint32_t i = 0; i < (uint32_t)count; ++i) {
+        const uint32_t sb = i % C::SB;
+        const uint32_t at = i * NC + min(lane, NC - 1);
+        if (!warp_wait(lane < NC ? &T.full[k_slot(at)] : &T.s_empty[sb], lane < NC ? k_par(at) : ((i / C::SB) & 1) ^ 1,
+                       lane <= NC, abort_flag))
+          break;
+        if (T.info[i % kInfo].first) {
+          ++seg;
+          if (!warp_wait(&T.q_full[seg % C::QB], (seg / C::QB) & 1, true, abort_flag)) break;
+        }
         tc_fence_after();
         if (elect_one()) {
 #pragma unroll
           for (int c = 0; c < NC; ++c) {
-            const uint32_t s = (v0 + c) % SLOTS;
-            const uint64_t da = dv + (uint64_t)(s * kChunk >> 4);
-            const uint64_t db = dp + (uint64_t)(pb * C::kPBytes >> 4);
+            const uint32_t slot = k_slot(i * NC + c);
+            const uint64_t da = dk + (uint64_t)(slot * kChunk >> 4);
+            const uint64_t db = dq + (uint64_t)(((seg % C::QB) * C::kQBytes + c * N * 128) >> 4);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) tc_mma_f8f6f4(tmem + sb * N, da + 2 * k, db + 2 * k, idesc, (c | k) != 0);
+            if (!a.shared) tc_commit(&T.empty[slot]);
+          }
+          tc_commit(&T.s_full[sb]);
+        }
+        __syncwarp();
+      }
+    } else if (warp == 2) {
+      // ---------------------------------------------------------- O = V^T P^T
+      constexpr uint32_t idesc = idesc_f8f6f4(0, 0, 128, N) | (1u << 15) | (1u << 16);   // A and B along M / N
+      const uint64_t dv = sdesc_mn_sw128(smem_u32(smem));
+      const uint64_t dp = sdesc_mn_plain(smem_u32(pbuf));
+      for (uint32_t i = 0; i < (uint32_t)count; ++i) {
+        const uint32_t pb = i & 1, ob = i % C::OB;
+        const uint32_t at = i * NC + min(lane, NC - 1);
+        if (!warp_wait(&T.full[v_slot(at)], v_par(at), lane < NC, abort_flag)) break;
+        // the softmax warps look the values of a partly hidden tile over before they hand in its weights
+        if (lane == 0 && T.info[i % kInfo].mask) mbar_arrive(&T.v_ready);
+        __syncwarp();
+        if (!warp_wait(lane ? &T.o_empty[ob] : &T.p_full[pb], lane ? ((i / C::OB) & 1) ^ 1 : (i >> 1) & 1, lane < 2, abort_flag))
+          break;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t db = dp + (uint64_t)(pb * C::kPBytes >> 4);
+#pragma unroll
+          for (int c = 0; c < NC; ++c) {
+            const uint32_t slot = v_slot(i * NC + c);
+            const uint64_t da = dv + (uint64_t)(slot * kChunk >> 4);
 #pragma unroll
             for (int k = 0; k < 4; ++k)        // 32 tokens each: 4096 bytes of V, 512 of P
-              tc_mma_f8f6f4(tmem + C::SB * N + (ob * NC + c) * N, da + (4096 >> 4) * k, db + (512 >> 4) * k, idesc_o, k != 0);
-            tc_commit(&T.empty[s]);
+              tc_mma_f8f6f4(tmem + C::SB * N + (ob * NC + c) * N, da + (4096 >> 4) * k, db + (512 >> 4) * k, idesc, k != 0);
+            tc_commit(&T.empty[slot]);
           }
+          tc_commit(&T.p_empty[pb]);
           tc_commit(&T.o_full[ob]);
         }
         __syncwarp();
-      };
-      for (uint32_t i = 0; i <= (uint32_t)count && ok && count > 0; ++i) {
-        bool pv_done = i == 0;
-        if (i < (uint32_t)count) {
-          const uint32_t sb = i % C::SB, k0 = k_chunk(i);
-          for (uint32_t c = 0; c < NC; ++c) wait(&T.full[(k0 + c) % SLOTS], ((k0 + c) / SLOTS) & 1);
-          if (!ok) break;
-          if (T.info[i % kInfo].first) {
-            ++seg;
-            // with one Q buffer the next segment's rows come in when the last O tile of this one is out
-            if (C::QB == 1 && !pv_done) {
-              products_pv(i - 1);
-              pv_done = true;
-            }
-            wait(&T.q_full[seg % C::QB], (seg / C::QB) & 1);
-          }
-          wait(&T.s_empty[sb], ((i / C::SB) & 1) ^ 1);
-          if (!ok) break;
-          tc_fence_after();
-          if (elect_one()) {
-#pragma unroll
-            for (int c = 0; c < NC; ++c) {
-              const uint64_t da = dk + (uint64_t)(((k0 + c) % SLOTS) * kChunk >> 4);
-              const uint64_t db = dq + (uint64_t)(((seg % C::QB) * C::kQBytes + c * N * 128) >> 4);
-#pragma unroll
-              for (int k = 0; k < 4; ++k) tc_mma_f8f6f4(tmem + sb * N, da + 2 * k, db + 2 * k, idesc_s, (c | k) != 0);
-              if (!a.shared) tc_commit(&T.empty[(k0 + c) % SLOTS]);
-            }
-            tc_commit(&T.s_full[sb]);
-          }
-          __syncwarp();
-        }
-        if (!pv_done) products_pv(i - 1);
       }
     }
   } else if (warp < 4 + 4 * C::WG) {
@@ -651,12 +674,14 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, 1)
     const int row0 = wg * RW + 2 * (lane & 3);
     const uint32_t t_lane = tmem + ((uint32_t)(quad * 32) << 16) + wg * RW;
     float l[K][2], m[K][2], qf[K][2];
-    int seg = -1;
+    int seg = -1, masked = 0;
     bool dead = false;
     for (int i = 0; i < count; ++i) {
       const int sb = i % C::SB, pb = i & 1;
       const Info& in = T.info[i % kInfo];
-      const bool ok = __all_sync(0xffffffffu, mbar_wait(&T.s_full[sb], (i / C::SB) & 1, abort_flag)) && !dead;
+      const bool ok = warp_wait(lane ? &T.p_empty[pb] : &T.s_full[sb], lane ? ((i >> 1) & 1) ^ 1 : (i / C::SB) & 1,
+                                lane < 2, abort_flag) &&
+                      !dead;
       float s[K][4][2];
       if (ok) {
         tc_fence_after();
@@ -770,10 +795,9 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, 1)
         // Values that some row must not see: 0 x NaN would reach its sum.  Rows that no query sees become zero; a NaN
         // in a row that only some see becomes zero too, and is put back for those when the segment ends.
         const int tok = quad * 32 + lane, t = in.t0 + tok;
-        for (int c = 0; c < NC; ++c) {
-          const uint32_t v = v_chunk(i) + c;
-          if (!a.shared && !__all_sync(0xffffffffu, mbar_wait(&T.full[v % SLOTS], (v / SLOTS) & 1, abort_flag))) dead = true;
-          uint4* row16 = reinterpret_cast<uint4*>(smem + (v % SLOTS) * kChunk + tok * 128);
+        dead = !__all_sync(0xffffffffu, wait_quick(&T.v_ready, masked++ & 1, abort_flag));
+        for (int c = 0; c < NC && !dead; ++c) {
+          uint4* row16 = reinterpret_cast<uint4*>(smem + v_slot(i * NC + c) * kChunk + tok * 128);
           for (int k = 0; k < 8; ++k) {
             // the swizzle has the row's dims 16 k .. 16 k + 15 in this 16-byte unit
             uint4* vr = row16 + (k ^ (tok & 7));
@@ -908,7 +932,7 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, 1)
         for (int r = 0; r < R; ++r) acc[c][r] = 0.0f;
       for (int t = t0; t < t1; ++t, ++i) {
         const int ob = i % C::OB;
-        ok = __all_sync(0xffffffffu, mbar_wait(&T.o_full[ob], (i / C::OB) & 1, abort_flag));
+        ok = __all_sync(0xffffffffu, wait_quick(&T.o_full[ob], (i / C::OB) & 1, abort_flag));
         if (!ok) break;
         tc_fence_after();
         const float unit = T.info[i % kInfo].unit * (1.0f / 256.0f);
@@ -1076,7 +1100,7 @@ Layout layout(int64_t B, int64_t S, int H, int Hkv, int D, int f16) {
   const int64_t rows = S * (H / Hkv);
   l.R = rows_per_tile(rows, l.NC, f16);
   l.RT = (int)((rows + l.R - 1) / l.R);
-  l.grid = sm_count();
+  l.grid = sm_count() * (l.NC == 1 && l.R <= 16 ? 2 : 1);
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
   l.plan = up((1 + (size_t)B * l.RT) * 8);
   l.ml = up((size_t)2 * l.grid * l.R * 2 * 4);

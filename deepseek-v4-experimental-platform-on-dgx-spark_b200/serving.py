@@ -32,23 +32,32 @@ __all__ = ["rms_norm", "rms_norm_quant", "rope", "rope_freqs", "cache_append", "
 _I64x3 = ctypes.c_int64 * 3
 
 
-def _same_device(*ts: Optional[torch.Tensor]) -> torch.device:
-    dev = ts[0].device
-    if dev.type != "cuda":
+# Host time counts where a decode step is not captured into a graph: these two are what
+# torch.cuda.current_stream(...).cuda_stream and torch.cuda.current_device() end in, without 2 us of wrapping.
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
+
+
+def _device_of(*ts: Optional[torch.Tensor]) -> int:
+    """The index of the CUDA device that all the tensors are on."""
+    index = ts[0].get_device()
+    if index < 0:
         raise RuntimeError("bsgemm ops run on CUDA tensors only (no CPU fallback)")
     for t in ts:
-        if t is not None and t.device != dev:
-            raise ValueError(f"tensors on {dev} and {t.device}")
-    return dev
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"tensors on {ts[0].device} and {t.device}")
+    return index
 
 
-def _call(dev: torch.device, fn, *args) -> None:
-    """The library call on the current stream of ``dev``, with that device current."""
-    if dev.index == torch.cuda.current_device():
-        _lib.check(fn(*args, torch.cuda.current_stream(dev).cuda_stream))
+def _call(index: int, fn, *args) -> None:
+    """The library call on the current stream of device ``index``, with that device current."""
+    if index == _current_device():
+        status = fn(*args, _raw_stream(index))
+        if status:
+            _lib.check(status)
     else:
-        with torch.cuda.device(dev):
-            _lib.check(fn(*args, torch.cuda.current_stream(dev).cuda_stream))
+        with torch.cuda.device(index):
+            _lib.check(fn(*args, _raw_stream(index)))
 
 
 def _ptr(t: Optional[torch.Tensor]):
@@ -56,20 +65,21 @@ def _ptr(t: Optional[torch.Tensor]):
 
 
 def _norm_args(x, weight, residual):
-    dev = _same_device(x, weight, residual)
-    if x.dtype not in _X_DT:
-        raise TypeError(f"rms_norm: x is {x.dtype}, expected bf16, f16 or fp32")
-    if weight.dtype != x.dtype or (residual is not None and residual.dtype != x.dtype):
+    dev = _device_of(x, weight, residual)
+    dt = x.dtype
+    if dt not in _X_DT:
+        raise TypeError(f"rms_norm: x is {dt}, expected bf16, f16 or fp32")
+    if weight.dtype != dt or (residual is not None and residual.dtype != dt):
         raise TypeError("rms_norm: x, weight and residual must have one type")
-    H = x.size(-1)
-    if weight.shape != (H,):
-        raise ValueError(f"rms_norm: weight {tuple(weight.shape)} does not match H={H}")
-    if residual is not None and residual.shape != x.shape:
-        raise ValueError(f"rms_norm: residual {tuple(residual.shape)} does not match x {tuple(x.shape)}")
+    shape = x.shape
+    if not shape or weight.shape != shape[-1:]:
+        raise ValueError(f"rms_norm: weight {tuple(weight.shape)} does not match x {tuple(shape)}")
+    if residual is not None and residual.shape != shape:
+        raise ValueError(f"rms_norm: residual {tuple(residual.shape)} does not match x {tuple(shape)}")
     xc = x.contiguous()
-    rc = None if residual is None else residual.contiguous()
-    h = None if residual is None else torch.empty(x.shape, dtype=x.dtype, device=dev)
-    return dev, H, xc.numel() // H if H else 0, xc, weight.contiguous(), rc, h
+    H = shape[-1]
+    return (dev, _X_DT[dt], H, xc.numel() // H if H else 0, xc, weight.contiguous(),
+            None if residual is None else residual.contiguous(), None if residual is None else torch.empty_like(xc))
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: Optional[torch.Tensor] = None):
@@ -82,10 +92,9 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual:
     with a residual.
     """
     t0 = _time.perf_counter()
-    dev, H, rows, xc, wc, rc, h = _norm_args(x, weight, residual)
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    _call(dev, _lib.load().bs_rms_norm, xc.data_ptr(), _ptr(rc), wc.data_ptr(), _X_DT[x.dtype], rows, H, eps, _ptr(h),
-          y.data_ptr())
+    dev, dt, H, rows, xc, wc, rc, h = _norm_args(x, weight, residual)
+    y = torch.empty_like(xc)
+    _call(dev, _lib.load().bs_rms_norm, xc.data_ptr(), _ptr(rc), wc.data_ptr(), dt, rows, H, eps, _ptr(h), y.data_ptr())
     _tally("rms_norm", t0)
     return y if h is None else (y, h)
 
@@ -102,12 +111,12 @@ def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, res
     t0 = _time.perf_counter()
     if scale_dtype not in (torch.float32, torch.float8_e8m0fnu):
         raise NotImplementedError(f"rms_norm_quant: scale_dtype {scale_dtype} not supported")
-    dev, H, rows, xc, wc, rc, h = _norm_args(x, weight, residual)
+    dev, dt, H, rows, xc, wc, rc, h = _norm_args(x, weight, residual)
     if H % 128 != 0:
         raise NotImplementedError(f"rms_norm_quant: H={H} is not a multiple of 128")
-    y = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=dev)
-    s = torch.empty(*x.shape[:-1], H // 128, dtype=scale_dtype, device=dev)
-    _call(dev, _lib.load().bs_rms_norm_quant, xc.data_ptr(), _ptr(rc), wc.data_ptr(), _X_DT[x.dtype], rows, H, eps,
+    y = torch.empty_like(xc, dtype=torch.float8_e4m3fn)
+    s = xc.new_empty((*x.shape[:-1], H // 128), dtype=scale_dtype)
+    _call(dev, _lib.load().bs_rms_norm_quant, xc.data_ptr(), _ptr(rc), wc.data_ptr(), dt, rows, H, eps,
           0 if scale_fmt is None else 1, _ptr(h), y.data_ptr(), s.data_ptr(),
           _lib.DT_F32 if scale_dtype == torch.float32 else _lib.DT_E8M0)
     _tally("rms_norm_quant", t0)
@@ -159,32 +168,34 @@ def rope(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, layout: 
     D multiples of 8.
     """
     t0 = _time.perf_counter()
-    dev = _same_device(x, positions, freqs)
-    if x.dtype not in _X_DT:
+    dev = _device_of(x, positions, freqs)
+    dt = _X_DT.get(x.dtype)
+    if dt is None:
         raise TypeError(f"rope: x is {x.dtype}, expected bf16, f16 or fp32")
-    if positions.dtype not in (torch.int64, torch.int32):
+    if positions.dtype != torch.int64 and positions.dtype != torch.int32:
         raise TypeError(f"rope: positions are {positions.dtype}, expected int64 or int32")
     if freqs.dtype != torch.float64 or freqs.dim() != 1:
         raise TypeError("rope: freqs must be a float64 vector")
     if layout not in ("interleaved", "half"):
         raise ValueError(f"rope: layout {layout!r}: expected 'interleaved' or 'half'")
-    if x.dim() < 2 or positions.shape != x.shape[:-2]:
-        raise ValueError(f"rope: positions {tuple(positions.shape)} do not match x {tuple(x.shape)}")
-    H, D = x.shape[-2:]
-    e = 16 // x.element_size()
-    xt = x
-    # one token stride: the leading dims collapse into one, heads and dims stay
-    tok = _token_stride(x)
-    if tok is None or x.stride(-1) != 1 or x.stride(-2) % e or tok % e or x.data_ptr() % 16:
-        if inplace:
-            raise ValueError("rope: an in-place x needs contiguous 16-byte aligned dims and one stride over its tokens")
-        xt = x.contiguous()
-        tok = H * D
-    out = xt if inplace else torch.empty(x.shape, dtype=x.dtype, device=dev)
-    _call(dev, _lib.load().bs_rope, xt.data_ptr(), _X_DT[x.dtype], positions.numel(), H, D, tok, xt.stride(-2),
-          positions.contiguous().data_ptr(), 1 if positions.dtype == torch.int64 else 0, freqs.contiguous().data_ptr(),
-          2 * freqs.numel(), offset, 1 if layout == "half" else 0, 1 if inverse else 0, scale, out.data_ptr(),
-          tok if inplace else H * D, xt.stride(-2) if inplace else D)
+    shape = x.shape
+    if len(shape) < 2 or positions.shape != shape[:-2]:
+        raise ValueError(f"rope: positions {tuple(positions.shape)} do not match x {tuple(shape)}")
+    H, D = shape[-2:]
+    xt, tok, head = x, H * D, D
+    if not x.is_contiguous() or x.data_ptr() % 16:
+        e = 16 // x.element_size()
+        # one token stride: the leading dims collapse into one, heads and dims stay
+        tok, head = _token_stride(x), x.stride(-2)
+        if tok is None or x.stride(-1) != 1 or head % e or tok % e or x.data_ptr() % 16:
+            if inplace:
+                raise ValueError("rope: an in-place x needs contiguous 16-byte aligned dims and one stride over its tokens")
+            xt, tok, head = x.clone(memory_format=torch.contiguous_format), H * D, D
+    out = xt if inplace else torch.empty_like(x, memory_format=torch.contiguous_format)
+    pc, fc = positions.contiguous(), freqs.contiguous()
+    _call(dev, _lib.load().bs_rope, xt.data_ptr(), dt, pc.numel(), H, D, tok, head, pc.data_ptr(),
+          1 if pc.dtype == torch.int64 else 0, fc.data_ptr(), 2 * fc.numel(), offset, 1 if layout == "half" else 0,
+          1 if inverse else 0, scale, out.data_ptr(), tok if inplace else H * D, head if inplace else D)
     _tally("rope", t0)
     return out
 
@@ -224,9 +235,9 @@ def _check_index(name, what, t, shape):
 def _strided(x: torch.Tensor, unit: int, align: int) -> torch.Tensor:
     """x, or a contiguous copy where its strides do not keep vectors of ``unit`` elements whole."""
     s = x.stride()
-    if s[3] == 1 and s[0] % unit == 0 and s[1] % unit == 0 and s[2] % unit == 0 and x.data_ptr() % align == 0:
+    if s[3] == 1 and not (s[0] % unit or s[1] % unit or s[2] % unit or x.data_ptr() % align):
         return x
-    return x.contiguous()
+    return x.clone(memory_format=torch.contiguous_format)
 
 
 def cache_append(k: torch.Tensor, v: Optional[torch.Tensor], k_cache: torch.Tensor, v_cache: Optional[torch.Tensor],
@@ -248,7 +259,7 @@ def cache_append(k: torch.Tensor, v: Optional[torch.Tensor], k_cache: torch.Tens
     they were.  Sequences of one call must not write to the same page.
     """
     t0 = _time.perf_counter()
-    dev = _same_device(k, v, k_cache, v_cache, k_scale, v_scale, block_table, start, new_lens)
+    dev = _device_of(k, v, k_cache, v_cache, k_scale, v_scale, block_table, start, new_lens)
     if k.dim() != 4:
         raise ValueError(f"cache_append: k {tuple(k.shape)}, expected [B, S, Hkv, D]")
     B, S, Hkv, D = k.shape
@@ -281,7 +292,8 @@ def cache_append(k: torch.Tensor, v: Optional[torch.Tensor], k_cache: torch.Tens
 @functools.lru_cache(maxsize=4096)
 def _attn_workspace(index: int, B: int, S: int, H: int, Hkv: int, D: int, dt: int) -> int:
     with torch.cuda.device(index):
-        return _lib.load().bs_cache_attn_workspace_size(B, S, H, Hkv, D, dt)
+        n = _lib.load().bs_cache_attn_workspace_size(B, S, H, Hkv, D, dt)
+    return (max(n, 256) + 3) // 4 * 4
 
 
 def cache_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: Optional[torch.Tensor], k_scale: torch.Tensor,
@@ -301,7 +313,7 @@ def cache_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: Optional[torch.T
     it.
     """
     t0 = _time.perf_counter()
-    dev = _same_device(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, attn_sink, new_lens)
+    dev = _device_of(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, attn_sink, new_lens)
     if q.dim() != 4:
         raise ValueError(f"cache_attn: q {tuple(q.shape)}, expected [B, S, H, D]")
     B, S, H, D = q.shape
@@ -329,16 +341,15 @@ def cache_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: Optional[torch.T
         if attn_sink.shape != (H,):
             raise ValueError(f"cache_attn: attn_sink {tuple(attn_sink.shape)}, expected ({H},)")
         sink = attn_sink.float().contiguous()
-    out = torch.empty(B, S, H, D, dtype=q.dtype, device=dev)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if out.numel() == 0:
         return out
     qc = _strided(q, 4, 8)
     dt = _X_DT[q.dtype]
-    nbytes = _attn_workspace(dev.index, B, S, H, Hkv, D, dt)
-    ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=dev)
+    ws = bt.new_empty(_attn_workspace(dev, B, S, H, Hkv, D, dt) // 4)
     _call(dev, _lib.load().bs_cache_attn, qc.data_ptr(), dt, B, S, H, Hkv, D, _I64x3(*qc.stride()[:3]),
           k_cache.data_ptr(), _ptr(v_cache), k_scale.data_ptr(), _ptr(v_scale), k_cache.size(0), k_cache.size(2),
           bt.data_ptr(), bt.size(1), sl.data_ptr(), _ptr(nl), _ptr(sink), softmax_scale, out.data_ptr(), ws.data_ptr(),
-          ws.numel())
+          4 * ws.numel())
     _tally("cache_attn", t0)
     return out

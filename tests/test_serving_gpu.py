@@ -317,6 +317,26 @@ ATTN = [
 ]
 
 
-@pytest.mark.parametrize("case", ATTN, ids=lambda c: "-".join(str(x) for x in c).replace(" ", ""))
+# enough tokens that every CTA works through many tiles of several sequences
+ATTN_LONG = [
+    ([9000, 7777, 1, 128, 4000, 6001], 1, 32, 8, 128, 64, "bf16", False, False),
+    ([20000, 17], 1, 64, 8, 128, 128, "f16", False, True),
+    ([5000] * 7 + [4999], 1, 64, 4, 128, 32, "bf16", False, False),
+    ([9001, 8000], 1, 96, 8, 64, 16, "f16", False, False),
+    ([30000, 20000], 1, 64, 2, 128, 64, "bf16", False, True),
+    ([30000, 20000], 1, 48, 2, 112, 64, "f16", False, False),
+    ([30000, 123], 33, 8, 4, 128, 64, "bf16", False, False),
+    ([12000, 12345], 1, 24, 8, 256, 64, "bf16", False, False),
+    ([12000, 12345], 1, 64, 4, 256, 128, "f16", False, False),
+    ([9999, 10000], 1, 32, 4, 384, 64, "bf16", False, False),
+    ([8000, 9000, 300], 1, 64, 2, 512, 64, "bf16", False, False),
+    ([8000, 9000, 300], 1, 16, 2, 512, 16, "f16", False, False),
+    ([20000, 15000, 1, 40000], 1, 64, 1, 512, 64, "bf16", True, True),
+    ([20000, 15000, 40000], 1, 8, 1, 512, 128, "bf16", True, False),
+    ([20000, 15000, 40000], 1, 64, 1, 512, 64, "f16", True, False),
+]
+
+
+@pytest.mark.parametrize("case", ATTN + ATTN_LONG, ids=lambda c: "-".join(str(x) for x in c).replace(" ", ""))
 def test_cache_attn(pkg, case):
     run_attn(pkg, *case)
