@@ -744,7 +744,7 @@ static int norm_common(const void* x, const void* residual, const void* weight, 
     return fail(BS_ERR_INVALID_ARG, "%s: pointers must be 16-byte aligned", name);
   rmsn::Args a = {};
   a.x = x; a.res = residual; a.w = weight; a.h = h; a.y = y; a.s = s;
-  a.rows = rows; a.H = (int)H; a.eps = eps; a.s_e8m0 = s_dtype == BS_DT_E8M0; a.pow2 = pow2;
+  a.rows = rows; a.H = (int)H; a.inv_h = 1.0 / (double)H; a.eps = eps; a.s_e8m0 = s_dtype == BS_DT_E8M0; a.pow2 = pow2;
   return cuda_status(bs_launch_rms_norm(a, dtype, codes, (cudaStream_t)stream), name);
 }
 
@@ -768,7 +768,8 @@ int bs_rope(const void* x, int dtype, int64_t tokens, int H, int D, int64_t x_to
   if (rope_dim % 16 != 0 || rope_dim > 2 * rope::kMaxPairs || offset % 8 != 0 || D % 8 != 0)
     return fail(BS_ERR_UNSUPPORTED, "rope: rope_dim=%d (a multiple of 16 up to %d), offset=%d and D=%d (multiples of 8)",
                 rope_dim, 2 * rope::kMaxPairs, offset, D);
-  if (tokens > 0x7fffffff || H > 65535) return fail(BS_ERR_UNSUPPORTED, "rope: %lld tokens of %d heads", (long long)tokens, H);
+  if (tokens > 0x7fffffff || H > 65535 || D > 65536)
+    return fail(BS_ERR_UNSUPPORTED, "rope: %lld tokens of %d heads of %d", (long long)tokens, H, D);
   if (tokens == 0) return BS_OK;
   if (!x || !positions || !freqs || !out) return fail(BS_ERR_INVALID_ARG, "rope: null pointer");
   const int e = 16 / elem_bytes(dtype);

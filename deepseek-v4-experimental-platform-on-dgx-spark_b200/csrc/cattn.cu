@@ -159,13 +159,13 @@ struct Cfg {
   static constexpr int kCols = SB * N + OB * NC * N;
   static constexpr int kTmem = kCols <= 32 ? 32 : kCols <= 64 ? 64 : kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
   static_assert(kCols <= 512 && N % 16 == 0 && N <= 256, "TMEM");
-  struct Tail {                     // behind the ring, Q and P
+  struct alignas(16) Tail {         // behind the ring, Q and P
     Info info[kInfo];
     float qf[2][R];                 // 2^-k x |scale| x log2(e) of each row
     int lim[2][R];                  // tokens each row sees
     int64_t off[2][R];              // element offset of the row's output, -1: no row
-    float wmax[2][4][R], alpha[4][R];
-    float lsum[kSegRing][4][R], mfin[kSegRing][R];
+    float wmax[2][R][4], alpha[4][R];
+    float lsum[kSegRing][4][R], mfin[kSegRing][R], fin[2][R];
     int nanmin[kSegRing][NC * 128]; // first token with a NaN value in partly hidden tiles
     int nanseen[kSegRing];
     uint64_t full[kMaxSlots], empty[kMaxSlots];
@@ -230,7 +230,7 @@ BS_DEVINL float redux_max(float v) {
   asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
   return r;
 }
-// Barrier of a softmax warpgroup that also says whether all of it is still alive.
+// Barrier of one warpgroup that also says whether all of it is still alive.
 BS_DEVINL bool group_all(int id, bool ok) {
   uint32_t r;
   asm volatile(
@@ -240,10 +240,45 @@ BS_DEVINL bool group_all(int id, bool ok) {
       : "memory");
   return r != 0;
 }
+BS_DEVINL float lds_f32(uint32_t addr) {
+  float v;
+  asm("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+BS_DEVINL int64_t lds_s64(uint32_t addr) {
+  int64_t v;
+  asm("ld.shared.s64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
+  return v;
+}
 template <int N>
 BS_DEVINL void reg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
 BS_DEVINL void reg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// Two fp32 operations in one instruction.
+BS_DEVINL float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+BS_DEVINL float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+BS_DEVINL float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+BS_DEVINL float2 both(float x) { return make_float2(x, x); }
 
 // 2^x to 2 ulp; exponents below -126 give 0.
 BS_DEVINL float ex2(float x) {
@@ -469,11 +504,13 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
   auto k_par = [&](uint32_t n) -> uint32_t { return (a.shared ? n / SLOTS : n / KS) & 1; };
   auto v_slot = [&](uint32_t n) -> uint32_t { return a.shared ? n % SLOTS : KS + n % VS; };
   auto v_par = [&](uint32_t n) -> uint32_t { return (a.shared ? n / SLOTS : n / VS) & 1; };
-  // Registers move from the issuing warpgroup to the accumulators: 56 + 2 x 120 + 216 = 4 x 128.
+  // Registers move from the issuing warpgroup to the accumulators; the four shares add up to the launch's 4 x 128.
   constexpr bool kSplitRegs = C::WG == 2;
+  constexpr int kIssueRegs = NC * R > 64 ? 72 : 120, kSoftRegs = NC * R > 64 ? 112 : 120, kAccRegs = NC * R > 64 ? 216 : 152;
+  static_assert(kIssueRegs + 2 * kSoftRegs + kAccRegs == 512, "registers");
 
   if (warp < 4) {
-    if constexpr (kSplitRegs) reg_dec<56>();
+    if constexpr (kSplitRegs) reg_dec<kIssueRegs>();
     if (warp == 0) {
       // ---------------------------------------------------------- producer
       const int ppt = kTok >> a.page_log2, page = 1 << a.page_log2;
@@ -667,13 +704,13 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
   } else if (warp < 4 + 4 * C::WG) {
     // ------------------------------------------------------------ softmax
     // A thread holds tokens tok0 + 8k (k = 0..3) of rows row0 + 8g + {0, 1} (g < K).
-    if constexpr (kSplitRegs) reg_dec<120>();
+    if constexpr (kSplitRegs) reg_dec<kSoftRegs>();
     constexpr int RW = C::RW, K = RW / 8;
     const int wg = (warp >> 2) - 1, quad = warp & 3;
     const int tok0 = quad * 32 + (lane >> 2);
     const int row0 = wg * RW + 2 * (lane & 3);
     const uint32_t t_lane = tmem + ((uint32_t)(quad * 32) << 16) + wg * RW;
-    float l[K][2], m[K][2], qf[K][2];
+    float2 l[K], m[K], qf[K];
     int seg = -1, masked = 0;
     bool dead = false;
     for (int i = 0; i < count; ++i) {
@@ -682,7 +719,7 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
       const bool ok = warp_wait(lane ? &T.p_empty[pb] : &T.s_full[sb], lane ? ((i >> 1) & 1) ^ 1 : (i / C::SB) & 1,
                                 lane < 2, abort_flag) &&
                       !dead;
-      float s[K][4][2];
+      float2 s[K][4];
       if (ok) {
         tc_fence_after();
         {
@@ -695,11 +732,9 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
             ++seg;
 #pragma unroll
             for (int g = 0; g < K; ++g) {
-              const float2 f = *reinterpret_cast<const float2*>(&T.qf[seg & 1][row0 + 8 * g]);
-              qf[g][0] = f.x;
-              qf[g][1] = f.y;
-              m[g][0] = m[g][1] = -INFINITY;
-              l[g][0] = l[g][1] = 0.0f;
+              qf[g] = *reinterpret_cast<const float2*>(&T.qf[seg & 1][row0 + 8 * g]);
+              m[g] = both(-INFINITY);
+              l[g] = both(0.0f);
             }
           }
           float ks[4];
@@ -712,15 +747,16 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
 #pragma unroll
           for (int g = 0; g < K; ++g)
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
+            for (int k = 0; k < 4; ++k) {
+              const int at = 4 * g + 2 * (k & 1);
+              auto term = [&](int p) {
+                return make_float2(__uint_as_float(v[k >> 1][p][at]), __uint_as_float(v[k >> 1][p][at + 1]));
+              };
+              float2 x = term(PP - 1);
 #pragma unroll
-              for (int j = 0; j < 2; ++j) {
-                const int at = 4 * g + 2 * (k & 1) + j;
-                float x = __uint_as_float(v[k >> 1][PP - 1][at]);
-#pragma unroll
-                for (int p = PP - 2; p >= 0; --p) x = fmaf(x, 0.0625f, __uint_as_float(v[k >> 1][p][at]));
-                s[g][k][j] = x * ks[k];
-              }
+              for (int p = PP - 2; p >= 0; --p) x = fma2(x, both(0.0625f), term(p));
+              s[g][k] = mul2(x, both(ks[k]));
+            }
         }
         if (in.mask) {
 #pragma unroll
@@ -730,60 +766,67 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
             for (int k = 0; k < 4; ++k) {
               const int tok = tok0 + 8 * k, t = in.t0 + tok;
               const bool there = (in.valid >> (tok >> a.page_log2)) & 1;
-              if (!there || t >= lim.x) s[g][k][0] = -INFINITY;
-              if (!there || t >= lim.y) s[g][k][1] = -INFINITY;
+              if (!there || t >= lim.x) s[g][k].x = -INFINITY;
+              if (!there || t >= lim.y) s[g][k].y = -INFINITY;
             }
           }
         }
+        // Maxima of the thread's 2K rows over the warp's 32 tokens, in a butterfly that halves the rows with the lanes:
+        // lane group (lane / 4) % 2K ends up with row 8 (v / 2) + v % 2 of v = that number.
+        float x[2 * K];
 #pragma unroll
         for (int g = 0; g < K; ++g) {
-          float x[2];
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            x[j] = fmaxf(fmaxf(s[g][0][j], s[g][1][j]), fmaxf(s[g][2][j], s[g][3][j]));
-#pragma unroll
-            for (int o = 4; o < 32; o <<= 1) x[j] = fmaxf(x[j], __shfl_xor_sync(0xffffffffu, x[j], o));
-          }
-          if (lane < 4)
-            *reinterpret_cast<float2*>(&T.wmax[i & 1][quad][row0 + 8 * g]) = make_float2(x[0] * qf[g][0], x[1] * qf[g][1]);
+          x[2 * g] = fmaxf(fmaxf(s[g][0].x, s[g][1].x), fmaxf(s[g][2].x, s[g][3].x));
+          x[2 * g + 1] = fmaxf(fmaxf(s[g][0].y, s[g][1].y), fmaxf(s[g][2].y, s[g][3].y));
         }
+        int n = 2 * K;
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) {
+          if (n > 1) {
+            const bool odd = lane & o;
+#pragma unroll
+            for (int q = 0; q < n / 2; ++q)
+              x[q] = fmaxf(odd ? x[2 * q + 1] : x[2 * q], __shfl_xor_sync(0xffffffffu, odd ? x[2 * q] : x[2 * q + 1], o));
+            n /= 2;
+          } else {
+            x[0] = fmaxf(x[0], __shfl_xor_sync(0xffffffffu, x[0], o));
+          }
+        }
+        const int v = (lane >> 2) & (2 * K - 1);
+        if (lane < 8 * K) T.wmax[i & 1][row0 + 8 * (v >> 1) + (v & 1)][quad] = x[0];
       }
       // one barrier a tile: wmax has two buffers
       if (!group_all(1 + wg, ok)) break;
       const bool last = in.last;
 #pragma unroll
       for (int g = 0; g < K; ++g) {
-        float2 x[4];
+        const float4 x = *reinterpret_cast<const float4*>(T.wmax[i & 1][row0 + 8 * g]);
+        const float4 y = *reinterpret_cast<const float4*>(T.wmax[i & 1][row0 + 8 * g + 1]);
+        const float2 top = mul2(make_float2(fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)), fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w))), qf[g]);
+        const float2 now = make_float2(fmaxf(m[g].x, top.x), fmaxf(m[g].y, top.y));
+        // rows that have seen no token yet: -inf - 0
+        const float2 use = make_float2(now.x == -INFINITY ? 0.0f : now.x, now.y == -INFINITY ? 0.0f : now.y);
+        const float2 al = make_float2(ex2(m[g].x - use.x), ex2(m[g].y - use.y));
+        m[g] = now;
+        const float2 neg = make_float2(-use.x, -use.y);
 #pragma unroll
-        for (int w = 0; w < 4; ++w) x[w] = *reinterpret_cast<const float2*>(&T.wmax[i & 1][w][row0 + 8 * g]);
-        float al[2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float t = j ? fmaxf(fmaxf(x[0].y, x[1].y), fmaxf(x[2].y, x[3].y))
-                            : fmaxf(fmaxf(x[0].x, x[1].x), fmaxf(x[2].x, x[3].x));
-          const float now = fmaxf(m[g][j], t);
-          const float use = now == -INFINITY ? 0.0f : now;       // no token seen yet
-          al[j] = ex2(m[g][j] - use);
-          m[g][j] = now;
-          float sum = 0.0f;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            s[g][k][j] = ex2(fmaf(s[g][k][j], qf[g][j], -use));
-            sum += s[g][k][j];
-          }
-          l[g][j] = fmaf(l[g][j], al[j], sum);
+        for (int k = 0; k < 4; ++k) {
+          const float2 e = fma2(s[g][k], qf[g], neg);
+          s[g][k] = make_float2(ex2(e.x), ex2(e.y));
         }
-        if (quad == 0 && lane < 4) *reinterpret_cast<float2*>(&T.alpha[i & 3][row0 + 8 * g]) = make_float2(al[0], al[1]);
+        l[g] = fma2(l[g], al, add2(add2(s[g][0], s[g][1]), add2(s[g][2], s[g][3])));
+        if (quad == 0 && lane < 4) *reinterpret_cast<float2*>(&T.alpha[i & 3][row0 + 8 * g]) = al;
       }
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int tok = tok0 + 8 * k;
-        const float ratio = in.vr[tok >> a.page_log2];
+        const float2 ratio = both(in.vr[tok >> a.page_log2]);
         uint8_t* p = pbuf + pb * C::kPBytes + tok * 16;
 #pragma unroll
         for (int g = 0; g < K; ++g) {
           uint16_t c[PP];
-          split2h<PP>(s[g][k][0] * ratio, s[g][k][1] * ratio, c);
+          const float2 w = mul2(s[g][k], ratio);
+          split2h<PP>(w.x, w.y, c);
 #pragma unroll
           for (int t = 0; t < PP; ++t) {
             const int n = t * R + row0 + 8 * g;
@@ -830,16 +873,13 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
       if (last) {
 #pragma unroll
         for (int g = 0; g < K; ++g) {
-          float x[2];
+          float2 x = l[g];
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            x[j] = l[g][j];
-#pragma unroll
-            for (int o = 4; o < 32; o <<= 1) x[j] += __shfl_xor_sync(0xffffffffu, x[j], o);
-          }
+          for (int o = 4; o < 32; o <<= 1)
+            x = add2(x, make_float2(__shfl_xor_sync(0xffffffffu, x.x, o), __shfl_xor_sync(0xffffffffu, x.y, o)));
           if (lane < 4) {
-            *reinterpret_cast<float2*>(&T.lsum[seg % kSegRing][quad][row0 + 8 * g]) = make_float2(x[0], x[1]);
-            if (quad == 0) *reinterpret_cast<float2*>(&T.mfin[seg % kSegRing][row0 + 8 * g]) = make_float2(m[g][0], m[g][1]);
+            *reinterpret_cast<float2*>(&T.lsum[seg % kSegRing][quad][row0 + 8 * g]) = x;
+            if (quad == 0) *reinterpret_cast<float2*>(&T.mfin[seg % kSegRing][row0 + 8 * g]) = m[g];
           }
         }
         __syncwarp();
@@ -848,67 +888,79 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
     }
   } else {
     // ------------------------------------------------------------ Q in, O out
-    if constexpr (kSplitRegs) reg_inc<216>();
+    if constexpr (kSplitRegs) reg_inc<kAccRegs>();
     const int quad = warp & 3;
     const uint32_t lane_base = (uint32_t)(quad * 32) << 16;
-    // One warp per row: amax, power-of-two scale, terms, swizzled store.
+    // One warp per row: amax, power-of-two scale, terms, swizzled store.  The loads of RB rows go out together.
+    constexpr int RB = R / 4 < 4 ? R / 4 : NC > 2 ? 2 : 4;
     auto stage = [&](const Walk& w, int seg) {
       uint8_t* qb = qbuf + (seg % C::QB) * C::kQBytes;
       const int buf = seg & 1;
-      for (int r = quad; r < R; r += 4) {
-        const int rr = w.rt * R + r;
-        const int i = rr / a.G, g = rr - i * a.G;
-        const bool in = rr < a.S * a.G;
-        float f[NC][4];
-        float amax = 0.0f;
+      for (int r0 = quad; r0 < R; r0 += 4 * RB) {
+        uint2 raw[RB][NC];
+        int64_t off[RB];
+        int lim[RB];
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          const int d = c * 128 + lane * 4;
-          f[c][0] = f[c][1] = f[c][2] = f[c][3] = 0.0f;
-          if (in && d < a.D) {
-            const int64_t at = (int64_t)w.b * a.q_sb + (int64_t)i * a.q_ss + (int64_t)(w.h * a.G + g) * a.q_sh + d;
-            const uint2 v = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(a.q) + at);
-            const uint32_t u[2] = {v.x, v.y};
+        for (int k = 0; k < RB; ++k) {
+          const int rr = w.rt * R + r0 + 4 * k;
+          const int i = rr / a.G, head = w.h * a.G + rr - i * a.G;
+          const bool in = rr < a.S * a.G;
+          lim[k] = in ? row_limit(w.s, i) : 0;
+          off[k] = in && i < w.s.nl ? (((int64_t)w.b * a.S + i) * a.H + head) * a.D : -1;
+          const uint16_t* q = reinterpret_cast<const uint16_t*>(a.q) + (int64_t)w.b * a.q_sb + (int64_t)i * a.q_ss +
+                              (int64_t)head * a.q_sh + lane * 4;
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
+          for (int c = 0; c < NC; ++c)
+            raw[k][c] = in && c * 128 + lane * 4 < a.D ? *reinterpret_cast<const uint2*>(q + c * 128) : make_uint2(0, 0);
+        }
+#pragma unroll
+        for (int k = 0; k < RB; ++k) {
+          const int r = r0 + 4 * k;
+          float f[NC][4];
+          float amax = 0.0f;
+#pragma unroll
+          for (int c = 0; c < NC; ++c) {
+            const uint32_t u[2] = {raw[k][c].x, raw[k][c].y};
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
               if (PP == 3) {
-                const float2 z = __half22float2(*reinterpret_cast<const __half2*>(&u[k]));
-                f[c][2 * k] = z.x;
-                f[c][2 * k + 1] = z.y;
+                const float2 z = __half22float2(*reinterpret_cast<const __half2*>(&u[e]));
+                f[c][2 * e] = z.x;
+                f[c][2 * e + 1] = z.y;
               } else {
-                f[c][2 * k] = __uint_as_float(u[k] << 16);
-                f[c][2 * k + 1] = __uint_as_float(u[k] & 0xFFFF0000u);
+                f[c][2 * e] = __uint_as_float(u[e] << 16);
+                f[c][2 * e + 1] = __uint_as_float(u[e] & 0xFFFF0000u);
               }
             }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) amax = fmaxf(amax, fabsf(f[c][e]));
           }
+          amax = redux_max(amax);
+          // 2^e with amax * 2^e in [128, 256); zero rows, tiny ones and infinities keep to the exponents that exist
+          int e = 134 - (int)(__float_as_uint(amax) >> 23);
+          e = amax == 0.0f ? 0 : min(max(e, -120), 120);
+          float up = __uint_as_float((uint32_t)(127 + e) << 23);
+          const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+          if (amax == __uint_as_float(0x7F800000u)) up = __uint_as_float(0x7FC00000u);   // e4m3 would saturate it
+          if (a.scale_log2 < 0.0f) up = -up;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) amax = fmaxf(amax, fabsf(f[c][k]));
-        }
-        amax = redux_max(amax);
-        // 2^e with amax * 2^e in [128, 256); zero rows, tiny ones and infinities keep to the exponents that exist
-        int e = 134 - (int)(__float_as_uint(amax) >> 23);
-        e = amax == 0.0f ? 0 : min(max(e, -120), 120);
-        float up = __uint_as_float((uint32_t)(127 + e) << 23);
-        const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-        if (amax == __uint_as_float(0x7F800000u)) up = __uint_as_float(0x7FC00000u);   // e4m3 would saturate it
-        if (a.scale_log2 < 0.0f) up = -up;
+          for (int c = 0; c < NC; ++c) {
+            uint16_t lo[PP], hi[PP];
+            split2<PP>(f[c][0] * up, f[c][1] * up, lo);
+            split2<PP>(f[c][2] * up, f[c][3] * up, hi);
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          uint16_t lo[PP], hi[PP];
-          split2<PP>(f[c][0] * up, f[c][1] * up, lo);
-          split2<PP>(f[c][2] * up, f[c][3] * up, hi);
-#pragma unroll
-          for (int p = 0; p < PP; ++p) {
-            const int n = p * R + r;
-            *reinterpret_cast<uint32_t*>(qb + c * N * 128 + n * 128 + ((lane * 4) ^ ((n & 7) << 4))) =
-                (uint32_t)lo[p] | ((uint32_t)hi[p] << 16);
+            for (int p = 0; p < PP; ++p) {
+              const int n = p * R + r;
+              *reinterpret_cast<uint32_t*>(qb + c * N * 128 + n * 128 + ((lane * 4) ^ ((n & 7) << 4))) =
+                  (uint32_t)lo[p] | ((uint32_t)hi[p] << 16);
+            }
           }
-        }
-        if (lane == 0) {
-          // not zero: a hidden token's -inf times it has to stay -inf
-          T.qf[buf][r] = fmaxf(down * fabsf(a.scale_log2), 1e-35f);
-          T.lim[buf][r] = in ? row_limit(w.s, i) : 0;
-          T.off[buf][r] = in && i < w.s.nl ? (((int64_t)w.b * a.S + i) * a.H + w.h * a.G + g) * a.D : -1;
+          if (lane == 0) {
+            // not zero: a hidden token's -inf times it has to stay -inf
+            T.qf[buf][r] = fmaxf(down * fabsf(a.scale_log2), 1e-35f);
+            T.lim[buf][r] = lim[k];
+            T.off[buf][r] = off[k];
+          }
         }
       }
       fence_proxy_async_smem();
@@ -933,7 +985,7 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
       for (int t = t0; t < t1; ++t, ++i) {
         const int ob = i % C::OB;
         ok = __all_sync(0xffffffffu, wait_quick(&T.o_full[ob], (i / C::OB) & 1, abort_flag));
-        if (!ok) break;
+        if (!ok) break;               // out of the tile loop; the group's barrier below ends the role
         tc_fence_after();
         const float unit = T.info[i % kInfo].unit * (1.0f / 256.0f);
         const float* al = T.alpha[i & 3];
@@ -942,18 +994,44 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
           float o[R];
           load_rows<R, PP>(tmem + lane_base + C::SB * N + (ob * NC + c) * N, o);
 #pragma unroll
-          for (int r = 0; r < R; ++r) acc[c][r] = fmaf(acc[c][r], al[r], o[r] * unit);
+          for (int r = 0; r < R; r += 2) {
+            const float2 x = fma2(make_float2(acc[c][r], acc[c][r + 1]), *reinterpret_cast<const float2*>(al + r),
+                                  mul2(make_float2(o[r], o[r + 1]), both(unit)));
+            acc[c][r] = x.x;
+            acc[c][r + 1] = x.y;
+          }
         }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&T.o_empty[ob]);
       }
-      if (!ok) break;
-      if (C::QB == 1 && w.left > 0) stage(w, seg + 1);
-      const int sr = seg % kSegRing;
-      ok = __all_sync(0xffffffffu, mbar_wait(&T.l_full[sr], (seg / kSegRing) & 1, abort_flag));
-      if (!ok) break;
-      const int buf = seg & 1;
+      if (C::QB == 1 && ok && w.left > 0) stage(w, seg + 1);
+      const int sr = seg % kSegRing, buf = seg & 1;
+      ok = ok && __all_sync(0xffffffffu, wait_quick(&T.l_full[sr], (seg / kSegRing) & 1, abort_flag));
+      const bool whole = t0 == 0 && t1 == nt;
+      const int64_t slot = 2 * (int64_t)blockIdx.x + (seg == 0 ? 0 : 1);
+      // Row r's factor (1 over its sum), once, by thread r; partial results keep their sum and maximum instead.
+      const int row = quad * 32 + lane;
+      if (ok && row < R) {
+        const float lr = T.lsum[sr][0][row] + T.lsum[sr][1][row] + T.lsum[sr][2][row] + T.lsum[sr][3][row];
+        const float m = T.mfin[sr][row];
+        float f = 1.0f;
+        if (!whole) {
+          *reinterpret_cast<float2*>(&a.part_ml[(slot * R + row) * 2]) = make_float2(m, lr);
+        } else {
+          const int64_t at = T.off[buf][row];
+          float z = lr;
+          if (a.sink && at >= 0) {
+            const float sk = a.sink[(at / a.D) % a.H] * 1.4426950408889634f;
+            const float M = fmaxf(m, sk);
+            f = m == -INFINITY ? 0.0f : exp2f(m - M);
+            z = lr * f + (sk == -INFINITY ? 0.0f : exp2f(sk - M));
+          }
+          f = z == 0.0f ? 0.0f : f / z;
+        }
+        T.fin[buf][row] = f;
+      }
+      if (!group_all(3, ok)) break;
       if (T.nanseen[sr]) {
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
@@ -964,40 +1042,31 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
           T.nanmin[sr][c * 128 + quad * 32 + lane] = 0x7FFFFFFF;
         }
       }
-      const bool whole = t0 == 0 && t1 == nt;
-      const int64_t slot = 2 * (int64_t)blockIdx.x + (seg == 0 ? 0 : 1);
+      // Shared memory is read by its 32-bit address here: loads through T are generic ones, which wait for the global
+      // stores before them (1000 cycles a row, 60000 at the end of a segment of 64 rows).
+      const uint32_t fin = smem_u32(&T.fin[buf][0]), off = smem_u32(&T.off[buf][0]);
+      const int d0 = quad * 32 + lane;
+      if (whole) {
+        uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + d0;
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const float lr = T.lsum[sr][0][r] + T.lsum[sr][1][r] + T.lsum[sr][2][r] + T.lsum[sr][3][r];
-        const float m = T.mfin[sr][r];
-        if (whole) {
-          const int64_t at = T.off[buf][r];
+        for (int r = 0; r < R; ++r) {
+          const int64_t at = lds_s64(off + 8 * r);
+          const float f = lds_f32(fin + 4 * r);
           if (at < 0) continue;
-          float f = 1.0f, z = lr;
-          if (a.sink) {
-            const float sk = a.sink[(at / a.D) % a.H] * 1.4426950408889634f;
-            const float M = fmaxf(m, sk);
-            f = m == -INFINITY ? 0.0f : exp2f(m - M);
-            z = lr * f + (sk == -INFINITY ? 0.0f : exp2f(sk - M));
-          }
-          f = z == 0.0f ? 0.0f : f / z;
 #pragma unroll
           for (int c = 0; c < NC; ++c) {
-            const int d = c * 128 + quad * 32 + lane;
-            if (d < a.D) {
+            if (c * 128 + d0 < a.D) {
               const float x = acc[c][r] * f;
-              if (PP == 3) reinterpret_cast<__half*>(a.out)[at + d] = __float2half_rn(x);
-              else reinterpret_cast<__nv_bfloat16*>(a.out)[at + d] = __float2bfloat16_rn(x);
+              out[at + c * 128] = PP == 3 ? __half_as_ushort(__float2half_rn(x)) : __bfloat16_as_ushort(__float2bfloat16_rn(x));
             }
           }
-        } else {
-          if (quad == 0 && lane == 0) {
-            a.part_ml[(slot * R + r) * 2] = m;
-            a.part_ml[(slot * R + r) * 2 + 1] = lr;
-          }
-#pragma unroll
-          for (int c = 0; c < NC; ++c) a.part_o[(slot * R + r) * (NC * 128) + c * 128 + quad * 32 + lane] = acc[c][r];
         }
+      } else {
+        float* po = a.part_o + slot * (R * NC * 128) + d0;
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int c = 0; c < NC; ++c) po[r * (NC * 128) + c * 128] = acc[c][r];
       }
     }
   }

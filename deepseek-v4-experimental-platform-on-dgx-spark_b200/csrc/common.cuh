@@ -154,6 +154,13 @@ BS_DEVINL float bs_e4m3_to_f32(uint8_t c) {
   return float(v);
 }
 
+// n / d for n < 2^16 and d < 2^16: multiply by ceil(2^32 / d) (d = 1: 0, which means n itself).
+struct BsDiv {
+  uint32_t d, m;
+};
+inline BsDiv bs_make_div(uint32_t d) { return {d, d == 1 ? 0u : (uint32_t)((0x100000000ull + d - 1) / d)}; }
+BS_DEVINL uint32_t bs_div(uint32_t n, const BsDiv& v) { return v.m ? __umulhi(n, v.m) : n; }
+
 // NaN-preserving clamp (torch.clamp keeps NaN; fminf/fmaxf would not).
 BS_DEVINL float bs_clamp(float v, float lo, float hi) { return v > hi ? hi : (v < lo ? lo : v); }
 

@@ -15,13 +15,15 @@
 //
 // One CTA per (sequence, page it touches, head, key or value): it owns that
 // page and head, so there are no atomics and the result does not depend on any
-// order.  Two passes over its new rows: amax, then codes (the second reads
-// hit the caches).  HBM-bound for prompts, latency for single tokens.
+// order.  Its new rows are read once into registers, the loads going out
+// before the page's index and old scale are known; rows that do not fit there
+// (long pages of wide heads) are read twice, the second time out of L2.
+// HBM-bound for prompts, three dependent loads' latency for single tokens.
 #include "common.cuh"
 
 namespace kvc {
 
-constexpr int kThreads = 128;
+constexpr int kU = 8;             // 16-byte vectors of new rows in registers
 
 struct Args {
   const void* src[2];           // k, v: [B, S, Hkv, D], last dim contiguous
@@ -32,6 +34,7 @@ struct Args {
   const int* start;             // [B] cached tokens before the new ones
   const int* new_lens;          // [B] or null
   int B, S, Hkv, D, page_log2, max_pages, n_pages, span;   // span: pages a sequence touches at most
+  BsDiv vrow;                   // 16-byte vectors of a row
 };
 
 // Smallest power of two s with amax / s <= 448 = 1.75 * 2^8, exactly: compare amax's significand with 1.75.
@@ -41,20 +44,81 @@ BS_DEVINL float pow2_scale(float amax) {
   return __uint_as_float((uint32_t)e << 23);
 }
 
+// Codes of a vector: x / s for a power of two s (exact) or, where the page came with another scale, any s.  `odd`: there
+// are infinities among the new rows, which become NaN (the conversion would saturate them).
 template <typename T>
-__global__ void __launch_bounds__(kThreads) append_kernel(Args a) {
+BS_DEVINL void put_codes(uint8_t* dst, const uint4& raw, float s, float inv, bool pow2, bool odd) {
   constexpr int E = 16 / (int)sizeof(T);
-  __shared__ float red[kThreads / 32];
+  float f[E];
+  unpack<T>(raw, f);
+  if (pow2) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) f[e] *= inv;
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e) f[e] = __fdiv_rn(f[e], s);
+  }
+  if (odd) {
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (fabsf(f[e]) == __uint_as_float(0x7F800000u)) f[e] = __uint_as_float(0x7FC00000u);
+  }
+  uint32_t q[E / 4];
+#pragma unroll
+  for (int e = 0; e < E / 4; ++e)
+    q[e] = bs_cvt_e4m3x2(f[4 * e], f[4 * e + 1]) | ((uint32_t)bs_cvt_e4m3x2(f[4 * e + 2], f[4 * e + 3]) << 16);
+  if constexpr (E == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(q[0], q[1]);
+  else *reinterpret_cast<uint32_t*>(dst) = q[0];
+}
+
+// Largest magnitude of a vector as bits (of T, for two values of 16 bits at once in both halves): for numbers without
+// their sign integer order is float order, and infinities and NaN come out on top.
+template <typename T>
+BS_DEVINL uint32_t top_of(const uint4& v, uint32_t top) {
+  if constexpr (sizeof(T) == 2) {
+    constexpr uint32_t k = 0x7FFF7FFFu;
+    top = max_u16x2(top, max_u16x2(max_u16x2(v.x & k, v.y & k), max_u16x2(v.z & k, v.w & k)));
+  } else {
+    constexpr uint32_t k = 0x7FFFFFFFu;
+    top = max(top, max(max(v.x & k, v.y & k), max(v.z & k, v.w & k)));
+  }
+  return top;
+}
+template <typename T>
+BS_DEVINL float top_value(uint32_t top) {
+  if constexpr (sizeof(T) == 4) return __uint_as_float(top);
+  const uint16_t b = (uint16_t)max(top & 0xFFFFu, top >> 16);
+  return bs_to_f32<T>(*reinterpret_cast<const T*>(&b));
+}
+// Largest finite magnitude (vectors with infinities or NaN).
+template <typename T>
+BS_DEVINL float finite_top(const uint4& raw, float amax) {
+  constexpr int E = 16 / (int)sizeof(T);
+  float f[E];
+  unpack<T>(raw, f);
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const float v = fabsf(f[e]);
+    if (v < __uint_as_float(0x7F800000u)) amax = fmaxf(amax, v);
+  }
+  return amax;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(512, 2) append_kernel(const Args a) {
+  constexpr int E = 16 / (int)sizeof(T);
+  __shared__ float red[16];
   pdl_wait();
-  int64_t u = blockIdx.x;
-  const int h = (int)(u % a.Hkv);
-  u /= a.Hkv;
-  const int j = (int)(u % a.span);
-  const int b = (int)(u / a.span);
+  const int nthr = blockDim.x;
+  unsigned u = blockIdx.x;
+  const int h = (int)(u % (unsigned)a.Hkv);
+  u /= (unsigned)a.Hkv;
+  const int j = (int)(u % (unsigned)a.span);
+  const int b = (int)(u / (unsigned)a.span);
   const int w = blockIdx.y;
   const int page = 1 << a.page_log2;
-  int start = a.start[b];
-  int nl = a.new_lens ? a.new_lens[b] : a.S;
+  const int start = a.start[b];
+  const int nl = a.new_lens ? a.new_lens[b] : a.S;
   if (start < 0 || nl < 0 || nl > a.S) {      // not a length: nothing of this sequence is written
     if (threadIdx.x == 0) bs_set_error(BS_ERR_BAD_INDEX);
     return;
@@ -64,32 +128,52 @@ __global__ void __launch_bounds__(kThreads) append_kernel(Args a) {
   const int64_t lo = max((int64_t)start, first), hi = min((int64_t)start + nl, first + page);
   if (lo >= hi) return;
   const int id = pg < a.max_pages ? a.table[(int64_t)b * a.max_pages + pg] : -1;
+  const int m = (int)(hi - lo), before = (int)(lo - first);
+  const int vrow = (int)a.vrow.d, nvec = m * vrow;   // 16-byte vectors
+  const T* src = reinterpret_cast<const T*>(a.src[w]) + b * a.sb[w] + (lo - start) * a.ss[w] + h * a.sh[w];
+  const int64_t ss = a.ss[w];
+  auto vec = [&](int i) {
+    const int r = (int)bs_div(i, a.vrow);
+    return *reinterpret_cast<const uint4*>(src + r * ss + (i - r * vrow) * E);
+  };
+  // a thread's vectors are threadIdx.x + k nthr; the first kU stay in registers
+  uint4 raw[kU];
+#pragma unroll
+  for (int k = 0; k < kU; ++k) {
+    const int i = threadIdx.x + k * nthr;
+    if (i < nvec) raw[k] = vec(i);
+  }
   if (id < 0 || id >= a.n_pages) {
     if (threadIdx.x == 0) bs_set_error(BS_ERR_BAD_INDEX);
     return;
   }
-  const int m = (int)(hi - lo), before = (int)(lo - first);
-  const int vrow = a.D / E;                   // 16-byte vectors per row
-  const T* src = reinterpret_cast<const T*>(a.src[w]) + b * a.sb[w] + (lo - start) * a.ss[w] + h * a.sh[w];
-  float amax = 0.0f;
-  for (int i = threadIdx.x; i < m * vrow; i += kThreads) {
-    const int r = i / vrow, d = (i - r * vrow) * E;
-    float f[E];
-    unpack<T>(*reinterpret_cast<const uint4*>(src + r * a.ss[w] + d), f);
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const float v = fabsf(f[e]);
-      if (v < __uint_as_float(0x7F800000u)) amax = fmaxf(amax, v);
-    }
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = amax;
   const int64_t sat = (int64_t)id * a.Hkv + h;
   const float old = a.scale[w][sat];
-  __syncthreads();                            // also: every thread has read the old scale
+  uint32_t top = 0;
 #pragma unroll
-  for (int k = 0; k < kThreads / 32; ++k) amax = fmaxf(amax, red[k]);
+  for (int k = 0; k < kU; ++k)
+    if ((int)threadIdx.x + k * nthr < nvec) top = top_of<T>(raw[k], top);
+#pragma unroll 4
+  for (int i = threadIdx.x + kU * nthr; i < nvec; i += nthr) top = top_of<T>(vec(i), top);
+  auto over_cta = [&](float x) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) x = nan_max(x, __shfl_xor_sync(0xffffffffu, x, o));
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = x;
+    __syncthreads();
+    for (int k = 0; k < (nthr >> 5); ++k) x = nan_max(x, red[k]);
+    return x;
+  };
+  float amax = over_cta(top_value<T>(top));   // its barrier: every thread has read the old scale
+  const bool odd = !(amax < __uint_as_float(0x7F800000u));
+  if (odd) {                                  // the same for the whole CTA
+    amax = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kU; ++k)
+      if ((int)threadIdx.x + k * nthr < nvec) amax = finite_top<T>(raw[k], amax);
+    for (int i = threadIdx.x + kU * nthr; i < nvec; i += nthr) amax = finite_top<T>(vec(i), amax);
+    __syncthreads();
+    amax = over_cta(amax);
+  }
   float s = pow2_scale(amax);
   uint8_t* dst = a.cache[w] + sat * ((int64_t)a.D << a.page_log2);
   if (before > 0) {
@@ -97,7 +181,8 @@ __global__ void __launch_bounds__(kThreads) append_kernel(Args a) {
     if (s > old) {
       const float f = __fdiv_rn(old, s);
       const int n16 = before * a.D / 16;
-      for (int i = threadIdx.x; i < n16; i += kThreads) {
+#pragma unroll 4
+      for (int i = threadIdx.x; i < n16; i += nthr) {
         uint4 c = reinterpret_cast<uint4*>(dst)[i];
         uint32_t* p = reinterpret_cast<uint32_t*>(&c);
 #pragma unroll
@@ -111,33 +196,31 @@ __global__ void __launch_bounds__(kThreads) append_kernel(Args a) {
     }
   }
   if (threadIdx.x == 0) a.scale[w][sat] = s;
-  dst += (int64_t)before * a.D;
-  for (int i = threadIdx.x; i < m * vrow; i += kThreads) {
-    const int r = i / vrow, d = (i - r * vrow) * E;
-    float f[E];
-    unpack<T>(*reinterpret_cast<const uint4*>(src + r * a.ss[w] + d), f);
+  dst += (int64_t)before * a.D;               // the new rows lie one behind the other there
+  const bool pow2 = (__float_as_uint(s) & 0x7FFFFFu) == 0 && s >= 1.1754944e-38f && s < 1.7e38f;
+  const float inv = pow2 ? bs_inv_pow2(s) : 0.0f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      f[e] = __fdiv_rn(f[e], s);
-      if (fabsf(f[e]) == __uint_as_float(0x7F800000u)) f[e] = __uint_as_float(0x7FC00000u);
-    }
-    uint32_t q[E / 4];
-#pragma unroll
-    for (int e = 0; e < E / 4; ++e)
-      q[e] = bs_cvt_e4m3x2(f[4 * e], f[4 * e + 1]) | ((uint32_t)bs_cvt_e4m3x2(f[4 * e + 2], f[4 * e + 3]) << 16);
-    uint32_t* o = reinterpret_cast<uint32_t*>(dst + (int64_t)r * a.D + d);
-    if constexpr (E == 8) *reinterpret_cast<uint2*>(o) = make_uint2(q[0], q[1]);
-    else *o = q[0];
+  for (int k = 0; k < kU; ++k) {
+    const int i = threadIdx.x + k * nthr;
+    if (i < nvec) put_codes<T>(dst + i * E, raw[k], s, inv, pow2, odd);
   }
+#pragma unroll 4
+  for (int i = threadIdx.x + kU * nthr; i < nvec; i += nthr) put_codes<T>(dst + i * E, vec(i), s, inv, pow2, odd);
   pdl_launch_dependents();
 }
 
 }  // namespace kvc
 
-cudaError_t bs_launch_cache_append(const kvc::Args& a, int dtype, int both, cudaStream_t st) {
+cudaError_t bs_launch_cache_append(kvc::Args a, int dtype, int both, cudaStream_t st) {
+  // threads: one 16-byte vector of a page's new rows in each of the kU registers, from a warp to 512
+  const int E = dtype == BS_DT_F32 ? 4 : 8, page = 1 << a.page_log2;
+  a.vrow = bs_make_div(a.D / E);
+  const int64_t vecs = (int64_t)(a.S < page ? a.S : page) * a.D / E;
+  int threads = 32;
+  while (threads < 512 && (int64_t)threads * kvc::kU < vecs) threads *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((int64_t)a.B * a.span * a.Hkv), both ? 2 : 1);
-  cfg.blockDim = dim3(kvc::kThreads);
+  cfg.blockDim = dim3(threads);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -13,16 +13,16 @@
 // and only that fraction, in [-1/2, 1/2) turns, is rounded to fp32 for
 // sincospif.  What is left of the error is freq's own 2^-53.
 //
-// HBM-bound: a CTA takes one token and a range of its heads, loads its 16-byte
-// vectors first, computes the token's n/2 cos/sin pairs into shared memory
-// while they are in flight, and rotates and stores.
+// HBM-bound: a CTA takes a few tokens (or, when there are few, a range of one
+// token's heads), loads its 16-byte vectors first, computes the tokens' cos/sin
+// pairs into shared memory while they are in flight, rotates and stores.
 #include "common.cuh"
 
 namespace rope {
 
 constexpr int kThreads = 256;
 constexpr int kMaxPairs = 256;
-constexpr int kU = 4;           // 16-byte vectors (pairs of vectors in the half layout) in flight per thread
+constexpr int kCs = 1024;        // cos/sin pairs of a CTA's tokens
 
 struct Args {
   const void* x;
@@ -34,74 +34,80 @@ struct Args {
   const double* freq;           // [n/2] radians per position
   int64_t tokens;
   int H, D, n, offset;
-  int heads_per_cta;
+  int tokens_per_cta, heads_per_cta;
   float scale;
   int inverse, copy;            // copy: the unrotated dims go to out as well
+  BsDiv per_head, per_token, pairs;
 };
 
-// One task of a head: a rotated vector (or pair of vectors), or a vector to copy.
-template <typename T, bool HALF>
-__global__ void __launch_bounds__(kThreads) rope_kernel(Args a) {
+// One task: a rotated vector of 16 bytes (in the half layout a pair of them), or a vector to copy.  U tasks per thread
+// and pass are in flight.
+template <typename T, bool HALF, int U>
+__global__ void __launch_bounds__(kThreads) rope_kernel(const Args a) {
   constexpr int E = 16 / (int)sizeof(T);               // elements per vector
-  __shared__ float2 cs[kMaxPairs];
+  __shared__ float2 cs[kCs];
   pdl_wait();
-  const int64_t tok = blockIdx.x;
+  const int64_t tok0 = (int64_t)blockIdx.x * a.tokens_per_cta;
+  const int nt = (int)min((int64_t)a.tokens_per_cta, a.tokens - tok0);
   const int h0 = blockIdx.y * a.heads_per_cta;
   const int nh = min(a.heads_per_cta, a.H - h0);
   const int nrot = HALF ? a.n / (2 * E) : a.n / E;
-  const int per_head = nrot + (a.copy ? (a.D - a.n) / E : 0);
-  const int tasks = nh * per_head;
-  const T* x = reinterpret_cast<const T*>(a.x) + tok * a.x_tok + h0 * a.x_head;
-  T* out = reinterpret_cast<T*>(a.out) + tok * a.o_tok + h0 * a.o_head;
-
-  auto where = [&](int task, int& h, int& j, int& d) {   // head, index of the rotated vector (-1: copy), first dim
-    h = task / per_head;
-    const int k = task - h * per_head;
-    if (k < nrot) {
-      j = k;
-      d = a.offset + k * E;
-    } else {
-      j = -1;
-      const int e = (k - nrot) * E;
-      d = e < a.offset ? e : e + a.n;
-    }
-  };
+  const int per_token = nh * (int)a.per_head.d;
+  const int tasks = nt * per_token;
+  const T* x = reinterpret_cast<const T*>(a.x) + tok0 * a.x_tok + h0 * a.x_head;
+  T* out = reinterpret_cast<T*>(a.out) + tok0 * a.o_tok + h0 * a.o_head;
+  const int np = a.n / 2;
   bool first = true;
-  for (int base = 0; base < tasks; base += kThreads * kU) {
-    uint4 lo[kU], hi[kU];
+  for (int base = 0; base < tasks; base += kThreads * U) {
+    uint4 lo[U], hi[HALF ? U : 1];
+    int64_t to[U];
+    int at[U];                       // first cos/sin pair, or -1: copy
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
+    for (int u = 0; u < U; ++u) {
       const int task = base + u * kThreads + threadIdx.x;
       if (task < tasks) {
-        int h, j, d;
-        where(task, h, j, d);
-        lo[u] = *reinterpret_cast<const uint4*>(x + h * a.x_head + d);
-        if (HALF && j >= 0) hi[u] = *reinterpret_cast<const uint4*>(x + h * a.x_head + d + a.n / 2);
+        // per_token is the divisor of a full range of heads; a CTA with several tokens has all of them
+        const int t = nt > 1 ? bs_div(task, a.per_token) : 0;
+        const int in = task - t * per_token;
+        const int h = bs_div(in, a.per_head);
+        const int k = in - h * (int)a.per_head.d;
+        int d;
+        if (k < nrot) {
+          d = a.offset + k * E;
+          at[u] = t * np + (HALF ? k * E : k * E / 2);
+        } else {
+          const int e = (k - nrot) * E;
+          d = e < a.offset ? e : e + a.n;
+          at[u] = -1;
+        }
+        const T* p = x + t * a.x_tok + h * a.x_head + d;
+        to[u] = t * a.o_tok + h * a.o_head + d;
+        lo[u] = *reinterpret_cast<const uint4*>(p);
+        if (HALF && at[u] >= 0) hi[u] = *reinterpret_cast<const uint4*>(p + np);
       }
     }
     if (first) {
       first = false;
-      if (threadIdx.x < a.n / 2) {
-        const int64_t p = a.pos64 ? a.pos64[tok] : (int64_t)a.pos32[tok];
-        const double turn = a.freq[threadIdx.x] * 0.15915494309189533577;    // 1 / (2 pi)
+      for (int j = threadIdx.x; j < nt * np; j += kThreads) {
+        const int t = bs_div(j, a.pairs), i = j - t * np;
+        const int64_t p = a.pos64 ? a.pos64[tok0 + t] : (int64_t)a.pos32[tok0 + t];
+        const double turn = a.freq[i] * 0.15915494309189533577;              // 1 / (2 pi)
         const double frac = turn - floor(turn);
         // frac < 1; 2^64 itself (frac rounded up) saturates to 2^64 - 1
         const unsigned long long f = __double2ull_rn(frac * 18446744073709551616.0);
-        const long long t = (long long)((unsigned long long)p * f);
+        const long long v = (long long)((unsigned long long)p * f);
         float s, c;
-        sincospif((float)t * 1.0842021724855044e-19f, &s, &c);               // 2^-63: fraction of a turn x 2
-        cs[threadIdx.x] = make_float2(c * a.scale, (a.inverse ? -s : s) * a.scale);
+        sincospif((float)v * 1.0842021724855044e-19f, &s, &c);               // 2^-63: fraction of a turn x 2
+        cs[j] = make_float2(c * a.scale, (a.inverse ? -s : s) * a.scale);
       }
       __syncthreads();
     }
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
+    for (int u = 0; u < U; ++u) {
       const int task = base + u * kThreads + threadIdx.x;
       if (task < tasks) {
-        int h, j, d;
-        where(task, h, j, d);
-        T* o = out + h * a.o_head + d;
-        if (j >= 0) {
+        T* o = out + to[u];
+        if (at[u] >= 0) {
           float f[E];
           unpack<T>(lo[u], f);
           if (HALF) {
@@ -109,17 +115,17 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(Args a) {
             unpack<T>(hi[u], g);
 #pragma unroll
             for (int i = 0; i < E; ++i) {
-              const float2 t = cs[j * E + i];
+              const float2 t = cs[at[u] + i];
               p[i] = f[i] * t.x - g[i] * t.y;
               q[i] = f[i] * t.y + g[i] * t.x;
             }
-            *reinterpret_cast<uint4*>(o + a.n / 2) = pack<T>(q);
+            *reinterpret_cast<uint4*>(o + np) = pack<T>(q);
             lo[u] = pack<T>(p);
           } else {
             float p[E];
 #pragma unroll
             for (int i = 0; i < E; i += 2) {
-              const float2 t = cs[(j * E + i) >> 1];
+              const float2 t = cs[at[u] + (i >> 1)];
               p[i] = f[i] * t.x - f[i + 1] * t.y;
               p[i + 1] = f[i] * t.y + f[i + 1] * t.x;
             }
@@ -137,14 +143,28 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(Args a) {
 
 cudaError_t bs_launch_rope(rope::Args a, int dtype, int half, cudaStream_t st) {
   if (a.tokens == 0) return cudaSuccess;
-  const int esz = dtype == BS_DT_F32 ? 4 : 2;
-  // enough heads for about 16 KB of loads in each CTA
-  const int64_t head_bytes = (int64_t)(a.copy ? a.D : a.n) * esz;
-  int64_t hpc = 16384 / head_bytes;
-  hpc = hpc < 1 ? 1 : (hpc > a.H ? a.H : hpc);
+  const int esz = dtype == BS_DT_F32 ? 4 : 2, E = 16 / esz;
+  const int per_head = (half ? a.n / (2 * E) : a.n / E) + (a.copy ? (a.D - a.n) / E : 0);
+  // About 24 KB of loads per CTA, of as many whole tokens as that is (their cos/sin pairs have to fit), or of part of a
+  // token's heads; fewer when the CTAs would not fill the GPU twice.
+  const int want = half ? 768 : 1536;
+  const int64_t per_token = (int64_t)per_head * a.H;
+  int64_t tpc = want / per_token, hpc = a.H;
+  tpc = tpc < rope::kCs / (a.n / 2) ? tpc : rope::kCs / (a.n / 2);
+  const int64_t even = a.tokens / (4 * 148);
+  tpc = tpc < even ? tpc : even;
+  if (tpc <= 1) {
+    tpc = 1;
+    const int64_t most = a.tokens < 4 * 148 ? rope::kThreads : want;   // few tokens: more, smaller CTAs
+    if (per_token > most) hpc = most / per_head > 1 ? most / per_head : 1;
+  }
+  a.tokens_per_cta = (int)tpc;
   a.heads_per_cta = (int)hpc;
+  a.per_head = bs_make_div(per_head);
+  a.per_token = bs_make_div((uint32_t)(tpc > 1 ? per_token : 1));
+  a.pairs = bs_make_div(a.n / 2);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)a.tokens, (unsigned)((a.H + hpc - 1) / hpc));
+  cfg.gridDim = dim3((unsigned)((a.tokens + tpc - 1) / tpc), (unsigned)((a.H + hpc - 1) / hpc));
   cfg.blockDim = dim3(rope::kThreads);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -154,8 +174,8 @@ cudaError_t bs_launch_rope(rope::Args a, int dtype, int half, cudaStream_t st) {
   cfg.numAttrs = 1;
   auto go = [&](auto t) {
     using T = decltype(t);
-    return half ? cudaLaunchKernelEx(&cfg, rope::rope_kernel<T, true>, a)
-                : cudaLaunchKernelEx(&cfg, rope::rope_kernel<T, false>, a);
+    return half ? cudaLaunchKernelEx(&cfg, rope::rope_kernel<T, true, 3>, a)
+                : cudaLaunchKernelEx(&cfg, rope::rope_kernel<T, false, 6>, a);
   };
   if (dtype == BS_DT_BF16) return go(__nv_bfloat16());
   if (dtype == BS_DT_F16) return go(__half());

@@ -44,7 +44,8 @@ def no_device_error(pkg):
 
 NORM = [(1, 4096, "bf16", True), (3, 128, "bf16", False), (7, 7168, "bf16", True), (130, 5120, "f16", False),
         (5, 16384, "bf16", True), (33, 640, "f32", True), (2, 16384, "f32", False), (1000, 2304, "f16", True),
-        (4, 10368, "bf16", False), (1, 8192, "f16", True)]
+        (4, 10368, "bf16", False), (1, 8192, "f16", True), (2500, 4096, "bf16", True), (3001, 640, "f16", False),
+        (2400, 8192, "f32", False), (2369, 128, "bf16", True), (4800, 1024, "f32", True)]
 
 
 def _norm_inputs(rows, H, dt, res, seed=0):
