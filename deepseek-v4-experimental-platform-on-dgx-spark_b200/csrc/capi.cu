@@ -881,7 +881,7 @@ int bs_cache_attn(const void* q, int dtype, int64_t B, int64_t S, int H, int Hkv
   cudaError_t cerr;
   st = bs_launch_cache_attn(a, k_cache, v_cache, dtype == BS_DT_F16, workspace, (cudaStream_t)stream, &cerr);
   if (st == BS_ERR_CUDA) return cuda_status(cerr, "cache_attn");
-  if (st) return fail(st, "cache_attn: no TMA descriptor for this cache");
+  if (st) return fail(st, "cache_attn: more than 2^31 tiles or rows, or no TMA descriptor for this cache");
   return BS_OK;
 }
 

@@ -58,7 +58,7 @@ struct Args {
   const int* new_lens;             // or null: S for every sequence
   const float* sink;               // [H] or null
   void* out;                       // [B, S, H, D]
-  int64_t* plan;                   // [1 + B * RT]: tiles per CTA, first tile of each (sequence, row tile)
+  int* plan;                       // [1 + B * RT]: tiles per CTA, first tile of each (sequence, row tile)
   float* part_ml;                  // [2 * grid][R][2]
   float* part_o;                   // [2 * grid][R][NC * 128]
   int B, S, H, Hkv, G, D, RT, page_log2, max_pages, n_pages;
@@ -95,10 +95,10 @@ BS_DEVINL int tiles_of(int limit) { return (limit + kTok - 1) / kTok; }
 // A CTA's walk over its share: units (b, rt) in order, within a unit all kv heads, within a head its tiles.
 struct Walk {
   int unit, h, t, nt;
-  int64_t left;
   int b, rt, limit;
-  bool fresh;                       // nothing of this segment has been taken yet
   Seq s;
+  int left;
+  bool fresh;                       // nothing of this segment has been taken yet
   BS_DEVINL void enter(const Args& a, int R) {
     b = unit / a.RT;
     rt = unit - b * a.RT;
@@ -106,18 +106,7 @@ struct Walk {
     limit = tile_limit(a, s, rt, R);
     nt = tiles_of(limit);
   }
-  BS_DEVINL void start(const Args& a, int R, int unit0, int64_t off, int64_t n) {
-    unit = unit0;
-    left = n;
-    h = t = nt = 0;
-    fresh = true;
-    if (left > 0) {
-      enter(a, R);
-      h = (int)(off / nt);
-      t = (int)(off - (int64_t)h * nt);
-    }
-  }
-  BS_DEVINL int seg_end() const { return (int)min((int64_t)nt, (int64_t)t + left); }
+  BS_DEVINL int seg_end() const { return min(nt, t + left); }
   BS_DEVINL void next(const Args& a, int R) {
     left -= seg_end() - t;
     t = 0;
@@ -148,7 +137,7 @@ struct Info {                       // one tile, from the producer
 template <int R, int PP, int NC>
 struct Cfg {
   static constexpr int N = R * PP % 16 ? R * PP + 8 : R * PP;      // columns of one MMA
-  static constexpr int WG = R >= 32 ? 2 : 1;                       // softmax warpgroups
+  static constexpr int WG = R >= 32 ? R / 16 : 1;                  // softmax warpgroups
   static constexpr int RW = R / WG;                                // rows of each
   static constexpr int kThreads = 128 * (2 + WG);
   static constexpr int kQBytes = NC * N * 128;
@@ -172,9 +161,8 @@ struct Cfg {
     uint64_t s_full[2], s_empty[2], p_full[2], p_empty[2], o_full[2], o_empty[2], q_full[2], l_full[kSegRing], v_ready;
     uint32_t tmem;
     int abort;
-    int64_t scan[16];
-    int64_t start_off;
-    int start_unit;
+    int scan[24];
+    Walk start;                     // where this CTA's share begins
   };
   static constexpr int kFixed = 1024 + QB * kQBytes + 2 * kPBytes + (int)sizeof(Tail);
   // Two CTAs an SM for the small row tiles of a decode step: a tile's chain of waits (keys, S, maximum, P, O) is longer
@@ -344,48 +332,36 @@ BS_DEVINL void tmem_ld16x256(uint32_t taddr, uint32_t* v) {
   }
 }
 
-// R values of one TMEM lane out of their PP terms: columns term * R + row.
-template <int R, int PP>
+// B of the R values of one TMEM lane out of their PP terms: columns term * R + row.
+template <int R, int PP, int B>
 BS_DEVINL void load_rows(uint32_t taddr, float* s) {
-  if constexpr (R == 8 && PP == 2) {
-    uint32_t v[16];
-    BS_TMEM_LD16(taddr, v);
+  if constexpr (R == 8) {
+    uint32_t v[PP == 2 ? 16 : 32];             // all terms lie side by side
+    if constexpr (PP == 2) BS_TMEM_LD16(taddr, v);
+    else BS_TMEM_LD32(taddr, v);
     tmem_ld_wait();
 #pragma unroll
-    for (int r = 0; r < 8; ++r) s[r] = fmaf(__uint_as_float(v[8 + r]), 0.0625f, __uint_as_float(v[r]));
-  } else if constexpr (R == 8) {
-    uint32_t v[32];
-    BS_TMEM_LD32(taddr, v);
+    for (int r = 0; r < 8; ++r) {
+      float x = __uint_as_float(v[(PP - 1) * 8 + r]);
+#pragma unroll
+      for (int p = PP - 2; p >= 0; --p) x = fmaf(x, 0.0625f, __uint_as_float(v[p * 8 + r]));
+      s[r] = x;
+    }
+  } else {
+    static_assert(B == 16 || B == 32, "rows of a load");
+    uint32_t v[PP][B];
+#pragma unroll
+    for (int p = 0; p < PP; ++p) {
+      if constexpr (B == 16) BS_TMEM_LD16(taddr + p * R, v[p]);
+      else BS_TMEM_LD32(taddr + p * R, v[p]);
+    }
     tmem_ld_wait();
 #pragma unroll
-    for (int r = 0; r < 8; ++r)
-      s[r] = fmaf(fmaf(__uint_as_float(v[16 + r]), 0.0625f, __uint_as_float(v[8 + r])), 0.0625f, __uint_as_float(v[r]));
-  } else if constexpr (R == 16) {
-    uint32_t v[PP][16];
-#pragma unroll
-    for (int p = 0; p < PP; ++p) BS_TMEM_LD16(taddr + p * R, v[p]);
-    tmem_ld_wait();
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
+    for (int r = 0; r < B; ++r) {
       float x = __uint_as_float(v[PP - 1][r]);
 #pragma unroll
       for (int p = PP - 2; p >= 0; --p) x = fmaf(x, 0.0625f, __uint_as_float(v[p][r]));
       s[r] = x;
-    }
-  } else {
-#pragma unroll
-    for (int r0 = 0; r0 < R; r0 += 32) {
-      uint32_t v[PP][32];
-#pragma unroll
-      for (int p = 0; p < PP; ++p) BS_TMEM_LD32(taddr + p * R + r0, v[p]);
-      tmem_ld_wait();
-#pragma unroll
-      for (int r = 0; r < 32; ++r) {
-        float x = __uint_as_float(v[PP - 1][r]);
-#pragma unroll
-        for (int p = PP - 2; p >= 0; --p) x = fmaf(x, 0.0625f, __uint_as_float(v[p][r]));
-        s[r0 + r] = x;
-      }
     }
   }
 }
@@ -424,8 +400,6 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
     for (int i = 0; i < kSegRing; ++i) mbar_init(&T.l_full[i], 4 * C::WG);
     mbar_init(&T.v_ready, 1);
     T.abort = 0;
-    T.start_unit = 0;
-    T.start_off = 0;
     fence_barrier_init();
     tma_prefetch_desc(&tm_k);
     if (!a.shared) tma_prefetch_desc(&tm_v);
@@ -439,75 +413,94 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
     for (int i = tid; i < C::QB * C::kQBytes / 16; i += kThreads) reinterpret_cast<uint4*>(qbuf)[i] = make_uint4(0, 0, 0, 0);
     for (int i = tid; i < 2 * C::kPBytes / 16; i += kThreads) reinterpret_cast<uint4*>(pbuf)[i] = make_uint4(0, 0, 0, 0);
   }
-  for (int i = tid; i < kSegRing * NC * 128; i += kThreads) (&T.nanmin[0][0])[i] = 0x7FFFFFFF;
-  if (tid < kSegRing) T.nanseen[tid] = 0;
   pdl_launch_dependents();
   pdl_wait();
 
   // ---- the share of this CTA: tiles [start, start + count) of all
   const int units = a.B * a.RT;
-  auto unit_tiles = [&](int u, bool report) -> int64_t {
+  Walk mine;
+  auto unit_tiles = [&](int u, bool report) -> int {
     if (u >= units) return 0;
-    const int b = u / a.RT;
-    const Seq s = load_seq(a, b, report);
-    return (int64_t)a.Hkv * tiles_of(tile_limit(a, s, u - b * a.RT, R));
+    mine.unit = u;
+    mine.enter(a, R);
+    if (report && mine.rt == 0) load_seq(a, mine.b, true);
+    return a.Hkv * mine.nt;
   };
-  int64_t mine = 0;
-  for (int u = tid; u < units; u += kThreads) mine += unit_tiles(u, blockIdx.x == 0 && u % a.RT == 0);
+  auto warp_sum = [&](int x) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-  if (lane == 0) T.scan[warp] = mine;
-  fence_proxy_async_smem();
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  int64_t total = 0;
-#pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) total += T.scan[w];
-  __syncthreads();
-  const int64_t per = (total + gridDim.x - 1) / gridDim.x;
-  const int64_t start = min(per * blockIdx.x, total);
-  const int count = (int)min(per, total - start);
-  if (blockIdx.x == 0 && tid == 0) a.plan[0] = per;
-  if (count > 0 || blockIdx.x == 0) {
-    int64_t before = 0;
-    for (int u0 = 0; u0 < units; u0 += kThreads) {
-      const int64_t w = unit_tiles(u0 + tid, false);
-      int64_t inc = w;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t x = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += x;
-      }
-      if (lane == 31) T.scan[warp] = inc;
-      __syncthreads();
-      int64_t base = before;
-      for (int i = 0; i < warp; ++i) base += T.scan[i];
-      for (int i = 0; i < kThreads / 32; ++i) before += T.scan[i];
-      const int64_t ex = base + inc - w;
-      if (count > 0 && w > 0 && start >= ex && start < ex + w) {
-        T.start_unit = u0 + tid;
-        T.start_off = start - ex;
-      }
-      if (blockIdx.x == 0 && u0 + tid < units) a.plan[1 + u0 + tid] = ex;
-      __syncthreads();
-      if (blockIdx.x != 0 && before > start) break;
-    }
+    for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    return x;
+  };
+  int total = 0;
+  if (units > kThreads) {            // else one pass below sees them all
+    int x = 0;
+    for (int u = tid; u < units; u += kThreads) x += unit_tiles(u, false);
+    x = warp_sum(x);
+    if (lane == 0) T.scan[warp] = x;
+    __syncthreads();
+    for (int i = 0; i < kThreads / 32; ++i) total += T.scan[i];
+    __syncthreads();
   }
-  __syncthreads();
+  int per = 0, start = 0, count = 0, before = 0;
+  for (int u0 = 0; u0 == 0 || u0 < units; u0 += kThreads) {
+    const int x = unit_tiles(u0 + tid, blockIdx.x == 0);
+    int inc = x;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += y;
+    }
+    if (lane == 31) T.scan[warp] = inc;
+    if (u0 == 0) {
+      // the rest of the start-up, while the lengths are on their way
+      for (int i = tid; i < kSegRing * NC * 128; i += kThreads) (&T.nanmin[0][0])[i] = 0x7FFFFFFF;
+      if (tid < kSegRing) T.nanseen[tid] = 0;
+      fence_proxy_async_smem();
+      tc_fence_before();
+    }
+    __syncthreads();
+    if (u0 == 0) tc_fence_after();
+    int base = before, sum = 0;
+#pragma unroll
+    for (int i = 0; i < kThreads / 32; ++i) {
+      const int y = T.scan[i];
+      if (i < warp) base += y;
+      sum += y;
+    }
+    if (units <= kThreads) total = sum;
+    if (u0 == 0) {
+      per = (total + (int)gridDim.x - 1) / (int)gridDim.x;
+      start = min(per * (int)blockIdx.x, total);
+      count = min(per, total - start);
+      if (blockIdx.x == 0 && tid == 0) a.plan[0] = per;
+    }
+    const int first = base + inc - x;
+    if (start >= first && start < first + x) {
+      const int off = start - first;
+      mine.h = off / mine.nt;
+      mine.t = off - mine.h * mine.nt;
+      mine.left = count;
+      mine.fresh = true;
+      T.start = mine;
+    }
+    if (blockIdx.x == 0 && u0 + tid < units) a.plan[1 + u0 + tid] = first;
+    before += sum;
+    __syncthreads();
+    if (blockIdx.x != 0 && before > start) break;
+  }
   const uint32_t tmem = T.tmem;
-  const int unit0 = T.start_unit;
-  const int64_t off0 = T.start_off;
   // Slot of a running chunk number (tile x NC + c) and the parity of its phase.
   constexpr uint32_t KS = C::kKSlots, VS = C::kVSlots;
   auto k_slot = [&](uint32_t n) -> uint32_t { return a.shared ? n % SLOTS : n % KS; };
   auto k_par = [&](uint32_t n) -> uint32_t { return (a.shared ? n / SLOTS : n / KS) & 1; };
   auto v_slot = [&](uint32_t n) -> uint32_t { return a.shared ? n % SLOTS : KS + n % VS; };
   auto v_par = [&](uint32_t n) -> uint32_t { return (a.shared ? n / SLOTS : n / VS) & 1; };
-  // Registers move from the issuing warpgroup to the accumulators; the four shares add up to the launch's 4 x 128.
-  constexpr bool kSplitRegs = C::WG == 2;
-  constexpr int kIssueRegs = NC * R > 64 ? 72 : 120, kSoftRegs = NC * R > 64 ? 112 : 120, kAccRegs = NC * R > 64 ? 216 : 152;
-  static_assert(kIssueRegs + 2 * kSoftRegs + kAccRegs == 512, "registers");
+  // Registers move from the issuing and softmax warpgroups to the accumulators; the shares add up to the launch's
+  // 4 x 128 or 6 x 80.
+  constexpr bool kSplitRegs = C::WG >= 2;
+  constexpr int kIssueRegs = C::WG == 4 ? 64 : NC * R > 64 ? 72 : 120, kSoftRegs = C::WG == 4 ? 72 : NC * R > 64 ? 112 : 120,
+                kAccRegs = C::WG == 4 ? 128 : NC * R > 64 ? 216 : 152;
+  static_assert(!kSplitRegs || kIssueRegs + C::WG * kSoftRegs + kAccRegs == (C::WG == 4 ? 6 * 80 : 4 * 128), "registers");
 
   if (warp < 4) {
     if constexpr (kSplitRegs) reg_dec<kIssueRegs>();
@@ -522,8 +515,8 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
         uint32_t there;
         float ks, vs;
       };
-      Walk w;
-      w.start(a, R, unit0, off0, count);
+      Walk w = T.start;
+      if (count == 0) w.left = 0;
       auto load = [&](Batch& o) {
         o.n = 0;
         if (w.left <= 0) return;
@@ -646,28 +639,31 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
       int seg = -1;
       for (uint32_t i = 0; i < (uint32_t)count; ++i) {
         const uint32_t sb = i % C::SB;
-        const uint32_t at = i * NC + min(lane, NC - 1);
-        if (!warp_wait(lane < NC ? &T.full[k_slot(at)] : &T.s_empty[sb], lane < NC ? k_par(at) : ((i / C::SB) & 1) ^ 1,
-                       lane <= NC, abort_flag))
+        if (!warp_wait(lane ? &T.s_empty[sb] : &T.full[k_slot(i * NC)], lane ? ((i / C::SB) & 1) ^ 1 : k_par(i * NC), lane < 2,
+                       abort_flag))
           break;
         if (T.info[i % kInfo].first) {
           ++seg;
           if (!warp_wait(&T.q_full[seg % C::QB], (seg / C::QB) & 1, true, abort_flag)) break;
         }
-        tc_fence_after();
-        if (elect_one()) {
+        bool ok = true;
 #pragma unroll
-          for (int c = 0; c < NC; ++c) {
-            const uint32_t slot = k_slot(i * NC + c);
+        for (int c = 0; c < NC; ++c) {         // each chunk as it comes in
+          const uint32_t slot = k_slot(i * NC + c);
+          if (c > 0) ok = ok && warp_wait(&T.full[slot], k_par(i * NC + c), true, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_one()) {
             const uint64_t da = dk + (uint64_t)(slot * kChunk >> 4);
             const uint64_t db = dq + (uint64_t)(((seg % C::QB) * C::kQBytes + c * N * 128) >> 4);
 #pragma unroll
             for (int k = 0; k < 4; ++k) tc_mma_f8f6f4(tmem + sb * N, da + 2 * k, db + 2 * k, idesc, (c | k) != 0);
             if (!a.shared) tc_commit(&T.empty[slot]);
+            if (c == NC - 1) tc_commit(&T.s_full[sb]);
           }
-          tc_commit(&T.s_full[sb]);
+          __syncwarp();
         }
-        __syncwarp();
+        if (!ok) break;
       }
     } else if (warp == 2) {
       // ---------------------------------------------------------- O = V^T P^T
@@ -967,8 +963,8 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
       __syncwarp();
       if (lane == 0) mbar_arrive(&T.q_full[seg % C::QB]);
     };
-    Walk w;
-    w.start(a, R, unit0, off0, count);
+    Walk w = T.start;
+    if (count == 0) w.left = 0;
     if (w.left > 0) stage(w, 0);
     int i = 0;
     bool ok = true;
@@ -991,14 +987,18 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
         const float* al = T.alpha[i & 3];
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-          float o[R];
-          load_rows<R, PP>(tmem + lane_base + C::SB * N + (ob * NC + c) * N, o);
+          constexpr int B = R == 64 ? 16 : R;   // rows at a time: the registers of 64 would not fit
 #pragma unroll
-          for (int r = 0; r < R; r += 2) {
-            const float2 x = fma2(make_float2(acc[c][r], acc[c][r + 1]), *reinterpret_cast<const float2*>(al + r),
-                                  mul2(make_float2(o[r], o[r + 1]), both(unit)));
-            acc[c][r] = x.x;
-            acc[c][r + 1] = x.y;
+          for (int b = 0; b < R; b += B) {
+            float o[B];
+            load_rows<R, PP, B>(tmem + lane_base + C::SB * N + (ob * NC + c) * N + b, o);
+#pragma unroll
+            for (int r = 0; r < B; r += 2) {
+              const float2 x = fma2(make_float2(acc[c][b + r], acc[c][b + r + 1]), *reinterpret_cast<const float2*>(al + b + r),
+                                    mul2(make_float2(o[r], o[r + 1]), both(unit)));
+              acc[c][b + r] = x.x;
+              acc[c][b + r + 1] = x.y;
+            }
           }
         }
         tc_fence_before();
@@ -1031,7 +1031,7 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
         }
         T.fin[buf][row] = f;
       }
-      if (!group_all(3, ok)) break;
+      if (!group_all(8, ok)) break;
       if (T.nanseen[sr]) {
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
@@ -1079,17 +1079,16 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
 }
 
 // One warp per row: joins the partial results of heads that several CTAs share, and writes zeros for rows that see
-// nothing (empty sequences, padded query tokens).
-template <typename T>
-__global__ void __launch_bounds__(256) merge_kernel(const Args a, int R, int DC, int64_t rows) {
+// nothing (empty sequences, padded query tokens).  A lane weighs one partial result and holds four dims of each chunk.
+template <typename T, int NC>
+__global__ void __launch_bounds__(256) merge_kernel(const Args a, int R, int rows) {
   pdl_wait();
   const int lane = threadIdx.x & 31;
-  const int64_t per = a.plan[0];
-  for (int64_t id = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 5; id < rows; id += (int64_t)gridDim.x * 8) {
-    const int r = (int)(id % R);
-    const int64_t item = id / R;
-    const int h = (int)(item % a.Hkv);
-    const int unit = (int)(item / a.Hkv);
+  const int per = a.plan[0];
+  for (int id = (blockIdx.x * 256 + threadIdx.x) >> 5; id < rows; id += gridDim.x * 8) {
+    const int item = id / R, r = id - item * R;
+    const int unit = item / a.Hkv, h = item - unit * a.Hkv;
+    const int start = a.plan[1 + unit];
     const int b = unit / a.RT, rt = unit - b * a.RT;
     const int rr = rt * R + r;
     if (rr >= a.S * a.G) continue;
@@ -1097,34 +1096,59 @@ __global__ void __launch_bounds__(256) merge_kernel(const Args a, int R, int DC,
     const Seq s = load_seq(a, b, false);
     const int nt = tiles_of(tile_limit(a, s, rt, R));
     T* out = reinterpret_cast<T*>(a.out) + (((int64_t)b * a.S + i) * a.H + h * a.G + g) * a.D;
-    if (row_limit(s, i) == 0) {
-      for (int d = lane; d < a.D; d += 32) out[d] = bs_from_f32<T>(0.0f);
-      continue;
-    }
-    const int64_t first = a.plan[1 + unit] + (int64_t)h * nt;
-    const int64_t c0 = first / per, c1 = (first + nt - 1) / per;
-    if (c0 == c1) continue;                    // one CTA had it all
-    float M = -INFINITY, sk = -INFINITY;
-    if (a.sink) M = sk = a.sink[h * a.G + g] * 1.4426950408889634f;
-    // a CTA's first segment is in its slot 0, its last one in slot 1
-    auto slot = [&](int64_t c) { return 2 * c + (c * per >= first ? 0 : 1); };
-    for (int64_t c = c0 + lane; c <= c1; c += 32) M = fmaxf(M, a.part_ml[(slot(c) * R + r) * 2]);
+    const bool empty = row_limit(s, i) == 0;
+    const int first = start + h * nt;
+    const int c0 = empty ? 0 : first / per, c1 = empty ? 0 : (first + nt - 1) / per;
+    if (!empty && c0 == c1) continue;            // one CTA had it all
+    float4 acc[NC];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    const float use = M == -INFINITY ? 0.0f : M;
-    float z = sk == -INFINITY ? 0.0f : exp2f(sk - use);
-    for (int64_t c = c0; c <= c1; ++c) {
-      const float* ml = a.part_ml + (slot(c) * R + r) * 2;
-      z += ml[1] * exp2f(ml[0] - use);
-    }
-    const float f = z == 0.0f ? 0.0f : 1.0f / z;
-    for (int d = lane; d < a.D; d += 32) {
-      float acc = 0.0f;
-      for (int64_t c = c0; c <= c1; ++c) {
-        const int64_t at = slot(c) * R + r;
-        acc = fmaf(a.part_o[at * DC + d], exp2f(a.part_ml[at * 2] - use), acc);
+    for (int c = 0; c < NC; ++c) acc[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (!empty) {
+      // a CTA's first segment is in its slot 0, its last one in slot 1
+      auto part = [&](int c) { return (int64_t)(2 * c + (c * per >= first ? 0 : 1)) * R + r; };
+      const float sk = a.sink ? a.sink[h * a.G + g] * 1.4426950408889634f : -INFINITY;
+      float M = sk, z = 0.0f;
+      for (int c = c0 + lane; c <= c1; c += 32) {   // this lane's running maximum and sum
+        const float2 ml = *reinterpret_cast<const float2*>(&a.part_ml[part(c) * 2]);
+        const float m = fmaxf(M, ml.x);
+        if (m != -INFINITY) z = z * exp2f(M - m) + ml.y * exp2f(ml.x - m);
+        M = m;
       }
-      out[d] = bs_from_f32<T>(acc * f);
+      float top = M;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const float use = top == -INFINITY ? 0.0f : top;
+      z *= exp2f(M - use);                       // no part: 0 x exp2(-inf) = 0
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+      if (sk != -INFINITY) z += exp2f(sk - use);
+      const float f = z == 0.0f ? 0.0f : 1.0f / z;
+      for (int cb = c0; cb <= c1; cb += 32) {
+        const int n = min(32, c1 - cb + 1);
+        float w = 0.0f;
+        if (lane < n) w = exp2f(a.part_ml[part(cb + lane) * 2] - use) * f;
+#pragma unroll 4
+        for (int j = 0; j < n; ++j) {
+          const float wj = __shfl_sync(0xffffffffu, w, j);
+          const float4* po = reinterpret_cast<const float4*>(a.part_o + part(cb + j) * (NC * 128)) + lane;
+#pragma unroll
+          for (int c = 0; c < NC; ++c) {
+            const float4 v = po[c * 32];
+            acc[c].x = fmaf(v.x, wj, acc[c].x);
+            acc[c].y = fmaf(v.y, wj, acc[c].y);
+            acc[c].z = fmaf(v.z, wj, acc[c].z);
+            acc[c].w = fmaf(v.w, wj, acc[c].w);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int d = c * 128 + lane * 4;
+      if (d < a.D) {
+        T v[4] = {bs_from_f32<T>(acc[c].x), bs_from_f32<T>(acc[c].y), bs_from_f32<T>(acc[c].z), bs_from_f32<T>(acc[c].w)};
+        *reinterpret_cast<uint2*>(out + d) = *reinterpret_cast<const uint2*>(v);
+      }
     }
   }
 }
@@ -1171,7 +1195,7 @@ Layout layout(int64_t B, int64_t S, int H, int Hkv, int D, int f16) {
   l.RT = (int)((rows + l.R - 1) / l.R);
   l.grid = sm_count() * (l.NC == 1 && l.R <= 16 ? 2 : 1);
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
-  l.plan = up((1 + (size_t)B * l.RT) * 8);
+  l.plan = up((1 + (size_t)B * l.RT) * 4);
   l.ml = up((size_t)2 * l.grid * l.R * 2 * 4);
   l.o = (size_t)2 * l.grid * l.R * l.NC * 128 * 4;
   l.total = l.plan + l.ml + l.o;
@@ -1222,8 +1246,11 @@ int bs_launch_cache_attn(cattn::Args a, const void* k_cache, const void* v_cache
                          cudaError_t* cerr) {
   *cerr = cudaSuccess;
   const cattn::Layout l = cattn::layout(a.B, a.S, a.H, a.Hkv, a.D, f16);
+  // tiles and rows are counted in 32 bits
+  const int64_t most = (((int64_t)a.max_pages << a.page_log2) + 127) / 128;
+  if ((int64_t)a.B * l.RT * a.Hkv > 0x7fffffff / (most > l.R ? most : l.R) - 1024) return BS_ERR_UNSUPPORTED;
   a.RT = l.RT;
-  a.plan = (int64_t*)ws;
+  a.plan = (int*)ws;
   a.part_ml = (float*)((char*)ws + l.plan);
   a.part_o = (float*)((char*)ws + l.plan + l.ml);
   const int64_t page = (int64_t)1 << a.page_log2;
@@ -1252,8 +1279,14 @@ int bs_launch_cache_attn(cattn::Args a, const void* k_cache, const void* v_cache
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  e = f16 ? cudaLaunchKernelEx(&cfg, cattn::merge_kernel<__half>, a, l.R, l.NC * 128, rows)
-          : cudaLaunchKernelEx(&cfg, cattn::merge_kernel<__nv_bfloat16>, a, l.R, l.NC * 128, rows);
+  auto merge = [&](auto t) {
+    using T = decltype(t);
+    return l.NC == 1   ? cudaLaunchKernelEx(&cfg, cattn::merge_kernel<T, 1>, a, l.R, (int)rows)
+           : l.NC == 2 ? cudaLaunchKernelEx(&cfg, cattn::merge_kernel<T, 2>, a, l.R, (int)rows)
+           : l.NC == 3 ? cudaLaunchKernelEx(&cfg, cattn::merge_kernel<T, 3>, a, l.R, (int)rows)
+                       : cudaLaunchKernelEx(&cfg, cattn::merge_kernel<T, 4>, a, l.R, (int)rows);
+  };
+  e = f16 ? merge(__half()) : merge(__nv_bfloat16());
   *cerr = e;
   return e == cudaSuccess ? 0 : BS_ERR_CUDA;
 }
