@@ -27,10 +27,11 @@
 //
 // One work unit is a tile: 128 tokens of one (sequence, row tile, kv head);
 // a row tile is R of the S * (H / Hkv) query rows of a kv head.  All tiles of
-// the call lie in one sequence, and each CTA (one per SM) takes an equal
-// contiguous share of it, whatever the lengths; where a share ends inside a
-// head's tokens, both sides leave partial results (unnormalised O, max, sum)
-// and a second kernel joins them.  Lengths are read on the device only.
+// the call lie in one line, every head's preceded by what its start and end
+// cost (in tiles), and each resident CTA takes an equal stretch of the line,
+// whatever the lengths; where a stretch ends inside a head's tokens, both
+// sides leave partial results (unnormalised O, max, sum) and a second kernel
+// joins them.  Lengths are read on the device only.
 //
 // Roles: one warpgroup with the TMA producer and an issuer for each of the two
 // products; one or (from
@@ -38,6 +39,8 @@
 // that stages Q and accumulates O, one head dim per thread and 128-dim chunk.
 // Shared memory: a ring of 16 KB chunks, Q (this segment's and, where it fits,
 // the next one's), two P buffers.
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace cattn {
@@ -58,7 +61,7 @@ struct Args {
   const int* new_lens;             // or null: S for every sequence
   const float* sink;               // [H] or null
   void* out;                       // [B, S, H, D]
-  int* plan;                       // [1 + B * RT]: tiles per CTA, first tile of each (sequence, row tile)
+  int* plan;                       // [1 + B * RT]: places per CTA, first place of each (sequence, row tile)
   float* part_ml;                  // [2 * grid][R][2]
   float* part_o;                   // [2 * grid][R][NC * 128]
   int B, S, H, Hkv, G, D, RT, page_log2, max_pages, n_pages;
@@ -134,12 +137,17 @@ struct Info {                       // one tile, from the producer
   int pad;
 };
 
+__host__ __device__ constexpr int seg_cost(int wg) { return wg > 1 ? 3 : 1; }
+__host__ __device__ constexpr int softmax_groups(int R) { return R >= 32 ? R / 16 : 1; }
+
 template <int R, int PP, int NC>
 struct Cfg {
   static constexpr int N = R * PP % 16 ? R * PP + 8 : R * PP;      // columns of one MMA
-  static constexpr int WG = R >= 32 ? R / 16 : 1;                  // softmax warpgroups
+  static constexpr int WG = softmax_groups(R);                     // softmax warpgroups
   static constexpr int RW = R / WG;                                // rows of each
   static constexpr int kThreads = 128 * (2 + WG);
+  // Places before a head's tiles on the line of work: staging its rows, draining the pipeline, writing its results.
+  static constexpr int kSegCost = seg_cost(WG);
   static constexpr int kQBytes = NC * N * 128;
   static constexpr int kPBytes = N * kTok;
   static constexpr int QB = kQBytes >= 32768 ? 1 : 2;              // Q buffers
@@ -161,7 +169,8 @@ struct Cfg {
     uint64_t s_full[2], s_empty[2], p_full[2], p_empty[2], o_full[2], o_empty[2], q_full[2], l_full[kSegRing], v_ready;
     uint32_t tmem;
     int abort;
-    int scan[24];
+    int2 scan[24];
+    int first_tile, end_tile;       // its tiles on the line
     Walk start;                     // where this CTA's share begins
   };
   static constexpr int kFixed = 1024 + QB * kQBytes + 2 * kPBytes + (int)sizeof(Tail);
@@ -213,11 +222,6 @@ BS_DEVINL bool warp_wait(uint64_t* bar, uint32_t parity, bool active, volatile i
   return __all_sync(0xffffffffu, ok);
 }
 
-BS_DEVINL float redux_max(float v) {
-  float r;
-  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
-  return r;
-}
 // Barrier of one warpgroup that also says whether all of it is still alive.
 BS_DEVINL bool group_all(int id, bool ok) {
   uint32_t r;
@@ -286,21 +290,9 @@ BS_DEVINL uint16_t h2_to_e4m3x2(__half2 v) {
   asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(c) : "r"(*reinterpret_cast<uint32_t*>(&v)));
   return c;
 }
-// The PP terms of two values, in fp32 (Q).
-template <int PP>
-BS_DEVINL void split2(float x, float y, uint16_t* c) {
-#pragma unroll
-  for (int p = 0; p < PP; ++p) {
-    c[p] = bs_cvt_e4m3x2(x, y);
-    if (p + 1 < PP) {
-      const float2 b = __half22float2(e4m3x2_to_h2(c[p]));
-      x = (x - b.x) * 16.0f;
-      y = (y - b.y) * 16.0f;
-    }
-  }
-}
-// The same from f16 (P): rounding to f16 first costs 2^-12 of the value at most, and three terms then hold its 11 bits;
-// differences of a value and its nearest e4m3 neighbour are exact.
+// The PP terms of two values, from f16.  A weight loses 2^-12 of its value at most by that (three terms then hold its 11
+// bits); a value of Q, 8 or 11 bits wide on a scale where its row's largest is in [128, 256), nothing above 2^-25.
+// Differences of a value and its nearest e4m3 neighbour are exact.
 template <int PP>
 BS_DEVINL void split2h(float x, float y, uint16_t* c) {
   __half2 v = __floats2half2_rn(x, y);
@@ -431,24 +423,38 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
     for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
     return x;
   };
-  int total = 0;
+  // Lengths of the line: in places (tiles and the costs before them), and in tiles.
+  int total = 0, tiles = 0;
   if (units > kThreads) {            // else one pass below sees them all
-    int x = 0;
-    for (int u = tid; u < units; u += kThreads) x += unit_tiles(u, false);
+    int x = 0, y = 0;
+    for (int u = tid; u < units; u += kThreads) {
+      const int n = unit_tiles(u, false);
+      y += n;
+      x += n ? n + a.Hkv * C::kSegCost : 0;
+    }
     x = warp_sum(x);
-    if (lane == 0) T.scan[warp] = x;
+    y = warp_sum(y);
+    if (lane == 0) T.scan[warp] = make_int2(x, y);
     __syncthreads();
-    for (int i = 0; i < kThreads / 32; ++i) total += T.scan[i];
+    for (int i = 0; i < kThreads / 32; ++i) {
+      total += T.scan[i].x;
+      tiles += T.scan[i].y;
+    }
     __syncthreads();
   }
-  int per = 0, start = 0, count = 0, before = 0;
+  int start = 0, end = 0;
+  int2 before = make_int2(0, 0);
   for (int u0 = 0; u0 == 0 || u0 < units; u0 += kThreads) {
-    const int x = unit_tiles(u0 + tid, blockIdx.x == 0);
-    int inc = x;
+    const int n = unit_tiles(u0 + tid, blockIdx.x == 0);
+    const int2 x = make_int2(n ? n + a.Hkv * C::kSegCost : 0, n);
+    int2 inc = x;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += y;
+      const int y = __shfl_up_sync(0xffffffffu, inc.x, o), z = __shfl_up_sync(0xffffffffu, inc.y, o);
+      if (lane >= o) {
+        inc.x += y;
+        inc.y += z;
+      }
     }
     if (lane == 31) T.scan[warp] = inc;
     if (u0 == 0) {
@@ -460,34 +466,53 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
     }
     __syncthreads();
     if (u0 == 0) tc_fence_after();
-    int base = before, sum = 0;
+    int2 base = before, sum = make_int2(0, 0);
 #pragma unroll
     for (int i = 0; i < kThreads / 32; ++i) {
-      const int y = T.scan[i];
-      if (i < warp) base += y;
-      sum += y;
+      const int2 y = T.scan[i];
+      if (i < warp) {
+        base.x += y.x;
+        base.y += y.y;
+      }
+      sum.x += y.x;
+      sum.y += y.y;
     }
-    if (units <= kThreads) total = sum;
+    if (units <= kThreads) {
+      total = sum.x;
+      tiles = sum.y;
+    }
     if (u0 == 0) {
-      per = (total + (int)gridDim.x - 1) / (int)gridDim.x;
+      const int per = (total + (int)gridDim.x - 1) / (int)gridDim.x;
       start = min(per * (int)blockIdx.x, total);
-      count = min(per, total - start);
+      end = min(start + per, total);
       if (blockIdx.x == 0 && tid == 0) a.plan[0] = per;
+      if (tid == 0 && start == total) T.first_tile = tiles;
+      if (tid == 0 && end == total) T.end_tile = tiles;
     }
-    const int first = base + inc - x;
-    if (start >= first && start < first + x) {
-      const int off = start - first;
-      mine.h = off / mine.nt;
-      mine.t = off - mine.h * mine.nt;
-      mine.left = count;
+    const int first = base.x + inc.x - x.x, first_tile = base.y + inc.y - x.y;
+    // tiles of the line before place p of this unit; h and t: the head and tile there
+    auto place = [&](int p, int& h, int& t) {
+      const int each = mine.nt + C::kSegCost;
+      h = (p - first) / each;
+      t = max(0, p - first - h * each - C::kSegCost);
+      return first_tile + h * mine.nt + t;
+    };
+    if (start >= first && start < first + x.x) {
+      T.first_tile = place(start, mine.h, mine.t);
       mine.fresh = true;
       T.start = mine;
     }
+    if (end >= first && end < first + x.x) {
+      int h, t;
+      T.end_tile = place(end, h, t);
+    }
     if (blockIdx.x == 0 && u0 + tid < units) a.plan[1 + u0 + tid] = first;
-    before += sum;
+    before.x += sum.x;
+    before.y += sum.y;
     __syncthreads();
-    if (blockIdx.x != 0 && before > start) break;
+    if (blockIdx.x != 0 && before.x > end) break;
   }
+  const int count = T.end_tile - T.first_tile;
   const uint32_t tmem = T.tmem;
   // Slot of a running chunk number (tile x NC + c) and the parity of its phase.
   constexpr uint32_t KS = C::kKSlots, VS = C::kVSlots;
@@ -516,7 +541,7 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
         float ks, vs;
       };
       Walk w = T.start;
-      if (count == 0) w.left = 0;
+      w.left = count;
       auto load = [&](Batch& o) {
         o.n = 0;
         if (w.left <= 0) return;
@@ -887,76 +912,75 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
     if constexpr (kSplitRegs) reg_inc<kAccRegs>();
     const int quad = warp & 3;
     const uint32_t lane_base = (uint32_t)(quad * 32) << 16;
-    // One warp per row: amax, power-of-two scale, terms, swizzled store.  The loads of RB rows go out together.
-    constexpr int RB = R / 4 < 4 ? R / 4 : NC > 2 ? 2 : 4;
+    // One warp per row: amax, power-of-two scale, terms, swizzled store.  Lane k works out where the warp's k-th row
+    // lies; the loads of RB rows go out together.
+    constexpr int RB = R / 4 < 4 ? R / 4 : 4;
     auto stage = [&](const Walk& w, int seg) {
       uint8_t* qb = qbuf + (seg % C::QB) * C::kQBytes;
       const int buf = seg & 1;
-      for (int r0 = quad; r0 < R; r0 += 4 * RB) {
+      int64_t from = -1;
+      if (lane < R / 4) {
+        const int r = quad + 4 * lane, rr = w.rt * R + r;
+        int lim = 0;
+        int64_t off = -1;
+        if (rr < a.S * a.G) {
+          const int i = rr / a.G, head = w.h * a.G + rr - i * a.G;
+          lim = row_limit(w.s, i);
+          from = (int64_t)w.b * a.q_sb + (int64_t)i * a.q_ss + (int64_t)head * a.q_sh;
+          if (i < w.s.nl) off = (((int64_t)w.b * a.S + i) * a.H + head) * a.D;
+        }
+        T.lim[buf][r] = lim;
+        T.off[buf][r] = off;
+      }
+#pragma unroll 1
+      for (int k0 = 0; k0 < R / 4; k0 += RB) {
         uint2 raw[RB][NC];
-        int64_t off[RB];
-        int lim[RB];
 #pragma unroll
         for (int k = 0; k < RB; ++k) {
-          const int rr = w.rt * R + r0 + 4 * k;
-          const int i = rr / a.G, head = w.h * a.G + rr - i * a.G;
-          const bool in = rr < a.S * a.G;
-          lim[k] = in ? row_limit(w.s, i) : 0;
-          off[k] = in && i < w.s.nl ? (((int64_t)w.b * a.S + i) * a.H + head) * a.D : -1;
-          const uint16_t* q = reinterpret_cast<const uint16_t*>(a.q) + (int64_t)w.b * a.q_sb + (int64_t)i * a.q_ss +
-                              (int64_t)head * a.q_sh + lane * 4;
+          const int64_t at = __shfl_sync(0xffffffffu, from, k0 + k);
+          const uint16_t* q = reinterpret_cast<const uint16_t*>(a.q) + at + lane * 4;
 #pragma unroll
           for (int c = 0; c < NC; ++c)
-            raw[k][c] = in && c * 128 + lane * 4 < a.D ? *reinterpret_cast<const uint2*>(q + c * 128) : make_uint2(0, 0);
+            raw[k][c] = at >= 0 && c * 128 + lane * 4 < a.D ? *reinterpret_cast<const uint2*>(q + c * 128) : make_uint2(0, 0);
         }
 #pragma unroll
         for (int k = 0; k < RB; ++k) {
-          const int r = r0 + 4 * k;
-          float f[NC][4];
-          float amax = 0.0f;
+          const int r = quad + 4 * (k0 + k);
+          // amax of 16-bit numbers without their sign, two at a time: integer order is float order, NaN on top
+          uint32_t top = 0;
 #pragma unroll
-          for (int c = 0; c < NC; ++c) {
-            const uint32_t u[2] = {raw[k][c].x, raw[k][c].y};
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              if (PP == 3) {
-                const float2 z = __half22float2(*reinterpret_cast<const __half2*>(&u[e]));
-                f[c][2 * e] = z.x;
-                f[c][2 * e + 1] = z.y;
-              } else {
-                f[c][2 * e] = __uint_as_float(u[e] << 16);
-                f[c][2 * e + 1] = __uint_as_float(u[e] & 0xFFFF0000u);
-              }
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) amax = fmaxf(amax, fabsf(f[c][e]));
-          }
-          amax = redux_max(amax);
-          // 2^e with amax * 2^e in [128, 256); zero rows, tiny ones and infinities keep to the exponents that exist
+          for (int c = 0; c < NC; ++c) top = max_u16x2(top, max_u16x2(raw[k][c].x & 0x7FFF7FFFu, raw[k][c].y & 0x7FFF7FFFu));
+          const uint32_t bits = __reduce_max_sync(0xffffffffu, max(top & 0xFFFFu, top >> 16));
+          const float amax = PP == 3 ? __half2float(__ushort_as_half((uint16_t)bits)) : __uint_as_float(bits << 16);
+          // 2^e with amax * 2^e in [128, 256); zero rows and tiny ones keep to the exponents that exist; a row with
+          // infinities or NaN becomes NaN (e4m3 would saturate it)
           int e = 134 - (int)(__float_as_uint(amax) >> 23);
           e = amax == 0.0f ? 0 : min(max(e, -120), 120);
           float up = __uint_as_float((uint32_t)(127 + e) << 23);
           const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-          if (amax == __uint_as_float(0x7F800000u)) up = __uint_as_float(0x7FC00000u);   // e4m3 would saturate it
+          if (!(amax < __uint_as_float(0x7F800000u))) up = __uint_as_float(0x7FC00000u);
           if (a.scale_log2 < 0.0f) up = -up;
 #pragma unroll
           for (int c = 0; c < NC; ++c) {
-            uint16_t lo[PP], hi[PP];
-            split2<PP>(f[c][0] * up, f[c][1] * up, lo);
-            split2<PP>(f[c][2] * up, f[c][3] * up, hi);
+            uint16_t t[2][PP];
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              const uint32_t u = y ? raw[k][c].y : raw[k][c].x;
+              float2 x;
+              if (PP == 3) x = __half22float2(*reinterpret_cast<const __half2*>(&u));
+              else x = make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u));
+              x = mul2(x, both(up));
+              split2h<PP>(x.x, x.y, t[y]);
+            }
 #pragma unroll
             for (int p = 0; p < PP; ++p) {
               const int n = p * R + r;
               *reinterpret_cast<uint32_t*>(qb + c * N * 128 + n * 128 + ((lane * 4) ^ ((n & 7) << 4))) =
-                  (uint32_t)lo[p] | ((uint32_t)hi[p] << 16);
+                  (uint32_t)t[0][p] | ((uint32_t)t[1][p] << 16);
             }
           }
-          if (lane == 0) {
-            // not zero: a hidden token's -inf times it has to stay -inf
-            T.qf[buf][r] = fmaxf(down * fabsf(a.scale_log2), 1e-35f);
-            T.lim[buf][r] = lim[k];
-            T.off[buf][r] = off[k];
-          }
+          // not zero: a hidden token's -inf times it has to stay -inf
+          if (lane == 0) T.qf[buf][r] = fmaxf(down * fabsf(a.scale_log2), 1e-35f);
         }
       }
       fence_proxy_async_smem();
@@ -964,7 +988,7 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
       if (lane == 0) mbar_arrive(&T.q_full[seg % C::QB]);
     };
     Walk w = T.start;
-    if (count == 0) w.left = 0;
+    w.left = count;
     if (w.left > 0) stage(w, 0);
     int i = 0;
     bool ok = true;
@@ -1078,14 +1102,16 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
   }
 }
 
-// One warp per row: joins the partial results of heads that several CTAs share, and writes zeros for rows that see
-// nothing (empty sequences, padded query tokens).  A lane weighs one partial result and holds four dims of each chunk.
-template <typename T, int NC>
+// Joins the partial results of heads that several CTAs share, and writes zeros for rows that see nothing (empty
+// sequences, padded query tokens).  A row is one warp's, or with SPLIT (few rows) a CTA's, whose warps then share the
+// partial results.  A lane weighs one partial result and holds four dims of each chunk.
+template <typename T, int NC, bool SPLIT>
 __global__ void __launch_bounds__(256) merge_kernel(const Args a, int R, int rows) {
+  __shared__ float4 part_acc[SPLIT ? 8 : 1][SPLIT ? NC * 32 : 1];
   pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const int per = a.plan[0];
-  for (int id = (blockIdx.x * 256 + threadIdx.x) >> 5; id < rows; id += gridDim.x * 8) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int per = a.plan[0], cost = seg_cost(softmax_groups(R));
+  for (int id = SPLIT ? blockIdx.x : blockIdx.x * 8 + warp; id < rows; id += gridDim.x * (SPLIT ? 1 : 8)) {
     const int item = id / R, r = id - item * R;
     const int unit = item / a.Hkv, h = item - unit * a.Hkv;
     const int start = a.plan[1 + unit];
@@ -1097,7 +1123,7 @@ __global__ void __launch_bounds__(256) merge_kernel(const Args a, int R, int row
     const int nt = tiles_of(tile_limit(a, s, rt, R));
     T* out = reinterpret_cast<T*>(a.out) + (((int64_t)b * a.S + i) * a.H + h * a.G + g) * a.D;
     const bool empty = row_limit(s, i) == 0;
-    const int first = start + h * nt;
+    const int place = start + h * (nt + cost), first = place + cost;
     const int c0 = empty ? 0 : first / per, c1 = empty ? 0 : (first + nt - 1) / per;
     if (!empty && c0 == c1) continue;            // one CTA had it all
     float4 acc[NC];
@@ -1105,7 +1131,7 @@ __global__ void __launch_bounds__(256) merge_kernel(const Args a, int R, int row
     for (int c = 0; c < NC; ++c) acc[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if (!empty) {
       // a CTA's first segment is in its slot 0, its last one in slot 1
-      auto part = [&](int c) { return (int64_t)(2 * c + (c * per >= first ? 0 : 1)) * R + r; };
+      auto part = [&](int c) { return (int64_t)(2 * c + (c * per >= place ? 0 : 1)) * R + r; };
       const float sk = a.sink ? a.sink[h * a.G + g] * 1.4426950408889634f : -INFINITY;
       float M = sk, z = 0.0f;
       for (int c = c0 + lane; c <= c1; c += 32) {   // this lane's running maximum and sum
@@ -1123,14 +1149,15 @@ __global__ void __launch_bounds__(256) merge_kernel(const Args a, int R, int row
       for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
       if (sk != -INFINITY) z += exp2f(sk - use);
       const float f = z == 0.0f ? 0.0f : 1.0f / z;
-      for (int cb = c0; cb <= c1; cb += 32) {
-        const int n = min(32, c1 - cb + 1);
+      constexpr int step = SPLIT ? 8 : 1;
+      for (int cb = c0 + (SPLIT ? warp : 0); cb <= c1; cb += 32 * step) {
+        const int n = min(32, (c1 - cb) / step + 1);
         float w = 0.0f;
-        if (lane < n) w = exp2f(a.part_ml[part(cb + lane) * 2] - use) * f;
+        if (lane < n) w = exp2f(a.part_ml[part(cb + lane * step) * 2] - use) * f;
 #pragma unroll 4
         for (int j = 0; j < n; ++j) {
           const float wj = __shfl_sync(0xffffffffu, w, j);
-          const float4* po = reinterpret_cast<const float4*>(a.part_o + part(cb + j) * (NC * 128)) + lane;
+          const float4* po = reinterpret_cast<const float4*>(a.part_o + part(cb + j * step) * (NC * 128)) + lane;
 #pragma unroll
           for (int c = 0; c < NC; ++c) {
             const float4 v = po[c * 32];
@@ -1142,13 +1169,32 @@ __global__ void __launch_bounds__(256) merge_kernel(const Args a, int R, int row
         }
       }
     }
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      const int d = c * 128 + lane * 4;
+    auto put = [&](int d, float4 x) {
       if (d < a.D) {
-        T v[4] = {bs_from_f32<T>(acc[c].x), bs_from_f32<T>(acc[c].y), bs_from_f32<T>(acc[c].z), bs_from_f32<T>(acc[c].w)};
+        T v[4] = {bs_from_f32<T>(x.x), bs_from_f32<T>(x.y), bs_from_f32<T>(x.z), bs_from_f32<T>(x.w)};
         *reinterpret_cast<uint2*>(out + d) = *reinterpret_cast<const uint2*>(v);
       }
+    };
+    if constexpr (SPLIT) {
+#pragma unroll
+      for (int c = 0; c < NC; ++c) part_acc[warp][c * 32 + lane] = acc[c];
+      __syncthreads();                           // a row's course is the same for all threads
+      if ((int)threadIdx.x < NC * 32) {
+        float4 x = part_acc[0][threadIdx.x];
+#pragma unroll
+        for (int k = 1; k < 8; ++k) {
+          const float4 y = part_acc[k][threadIdx.x];
+          x.x += y.x;
+          x.y += y.y;
+          x.z += y.z;
+          x.w += y.w;
+        }
+        put(threadIdx.x * 4, x);
+      }
+      __syncthreads();
+    } else {
+#pragma unroll
+      for (int c = 0; c < NC; ++c) put(c * 128 + lane * 4, acc[c]);
     }
   }
 }
@@ -1247,7 +1293,7 @@ int bs_launch_cache_attn(cattn::Args a, const void* k_cache, const void* v_cache
   *cerr = cudaSuccess;
   const cattn::Layout l = cattn::layout(a.B, a.S, a.H, a.Hkv, a.D, f16);
   // tiles and rows are counted in 32 bits
-  const int64_t most = (((int64_t)a.max_pages << a.page_log2) + 127) / 128;
+  const int64_t most = (((int64_t)a.max_pages << a.page_log2) + 127) / 128 + 8;
   if ((int64_t)a.B * l.RT * a.Hkv > 0x7fffffff / (most > l.R ? most : l.R) - 1024) return BS_ERR_UNSUPPORTED;
   a.RT = l.RT;
   a.plan = (int*)ws;
@@ -1270,7 +1316,8 @@ int bs_launch_cache_attn(cattn::Args a, const void* k_cache, const void* v_cache
   }
   const int64_t rows = (int64_t)a.B * a.RT * a.Hkv * l.R;
   cudaLaunchConfig_t cfg = {};
-  const int64_t want = (rows + 7) / 8;
+  const bool split = rows <= 4 * 148;        // few rows: a CTA each
+  const int64_t want = split ? rows : (rows + 7) / 8;
   cfg.gridDim = dim3((unsigned)(want < 148 * 8 ? want : 148 * 8));
   cfg.blockDim = dim3(256);
   cfg.stream = st;
@@ -1279,12 +1326,17 @@ int bs_launch_cache_attn(cattn::Args a, const void* k_cache, const void* v_cache
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  auto merge = [&](auto t) {
+  auto merge_n = [&](auto t, auto nc) {
     using T = decltype(t);
-    return l.NC == 1   ? cudaLaunchKernelEx(&cfg, cattn::merge_kernel<T, 1>, a, l.R, (int)rows)
-           : l.NC == 2 ? cudaLaunchKernelEx(&cfg, cattn::merge_kernel<T, 2>, a, l.R, (int)rows)
-           : l.NC == 3 ? cudaLaunchKernelEx(&cfg, cattn::merge_kernel<T, 3>, a, l.R, (int)rows)
-                       : cudaLaunchKernelEx(&cfg, cattn::merge_kernel<T, 4>, a, l.R, (int)rows);
+    constexpr int NC = decltype(nc)::value;
+    return split ? cudaLaunchKernelEx(&cfg, cattn::merge_kernel<T, NC, true>, a, l.R, (int)rows)
+                 : cudaLaunchKernelEx(&cfg, cattn::merge_kernel<T, NC, false>, a, l.R, (int)rows);
+  };
+  auto merge = [&](auto t) {
+    return l.NC == 1   ? merge_n(t, std::integral_constant<int, 1>())
+           : l.NC == 2 ? merge_n(t, std::integral_constant<int, 2>())
+           : l.NC == 3 ? merge_n(t, std::integral_constant<int, 3>())
+                       : merge_n(t, std::integral_constant<int, 4>());
   };
   e = f16 ? merge(__half()) : merge(__nv_bfloat16());
   *cerr = e;
