@@ -66,6 +66,7 @@ struct Args {
   float* part_o;                   // [2 * grid][R][NC * 128]
   int B, S, H, Hkv, G, D, RT, page_log2, max_pages, n_pages;
   float scale_log2;                // softmax scale x log2(e)
+  int seg_cost;                    // Cfg::kSegCost, for the joining kernel
   int shared;                      // values are the keys' codes
 };
 
@@ -137,7 +138,6 @@ struct Info {                       // one tile, from the producer
   int pad;
 };
 
-__host__ __device__ constexpr int seg_cost(int wg) { return wg > 1 ? 3 : 1; }
 __host__ __device__ constexpr int softmax_groups(int R) { return R >= 32 ? R / 16 : 1; }
 
 template <int R, int PP, int NC>
@@ -146,11 +146,13 @@ struct Cfg {
   static constexpr int WG = softmax_groups(R);                     // softmax warpgroups
   static constexpr int RW = R / WG;                                // rows of each
   static constexpr int kThreads = 128 * (2 + WG);
-  // Places before a head's tiles on the line of work: staging its rows, draining the pipeline, writing its results.
-  static constexpr int kSegCost = seg_cost(WG);
   static constexpr int kQBytes = NC * N * 128;
   static constexpr int kPBytes = N * kTok;
   static constexpr int QB = kQBytes >= 32768 ? 1 : 2;              // Q buffers
+  // Places before a head's tiles on the line of work, for staging its rows, draining the pipeline and writing its
+  // results.  Measured with 0 to 8: 1 is best for 64 ragged sequences of 8 rows a head (182 us; 0: 184, 2: 183), 4 to 6
+  // for a chunk of 512 tokens (301 us; 2: 333, 8: 305), 6 to 8 with one Q buffer (latent: 89 us; 2: 97).
+  static constexpr int kSegCost = QB == 1 ? 7 : WG > 1 ? 5 : 1;
   static constexpr int OB = 2 * N + 2 * NC * N <= 512 ? 2 : 1;     // O buffers
   static constexpr int SB = 2 * N + OB * NC * N <= 512 ? 2 : 1;    // S buffers
   static constexpr int kCols = SB * N + OB * NC * N;
@@ -1110,7 +1112,7 @@ __global__ void __launch_bounds__(256) merge_kernel(const Args a, int R, int row
   __shared__ float4 part_acc[SPLIT ? 8 : 1][SPLIT ? NC * 32 : 1];
   pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int per = a.plan[0], cost = seg_cost(softmax_groups(R));
+  const int per = a.plan[0], cost = a.seg_cost;
   for (int id = SPLIT ? blockIdx.x : blockIdx.x * 8 + warp; id < rows; id += gridDim.x * (SPLIT ? 1 : 8)) {
     const int item = id / R, r = id - item * R;
     const int unit = item / a.Hkv, h = item - unit * a.Hkv;
@@ -1249,8 +1251,9 @@ Layout layout(int64_t B, int64_t S, int H, int Hkv, int D, int f16) {
 }
 
 template <int R, int PP, int NC>
-cudaError_t launch(const CUtensorMap& mk, const CUtensorMap& mv, const Args& a, int grid, cudaStream_t st) {
+cudaError_t launch(const CUtensorMap& mk, const CUtensorMap& mv, Args& a, int grid, cudaStream_t st) {
   using C = Cfg<R, PP, NC>;
+  a.seg_cost = C::kSegCost;
   auto kern = cache_attn_kernel<R, PP, NC>;
   static int done[hostcache::kMaxDevices];
   cudaError_t e = (cudaError_t)hostcache::get(done, [&] {
@@ -1271,7 +1274,7 @@ cudaError_t launch(const CUtensorMap& mk, const CUtensorMap& mv, const Args& a, 
 }
 
 template <int PP, int NC>
-cudaError_t launch_r(int R, const CUtensorMap& mk, const CUtensorMap& mv, const Args& a, int grid, cudaStream_t st) {
+cudaError_t launch_r(int R, const CUtensorMap& mk, const CUtensorMap& mv, Args& a, int grid, cudaStream_t st) {
   if (R == 8) return launch<8, PP, NC>(mk, mv, a, grid, st);
   if (R == 16) return launch<16, PP, NC>(mk, mv, a, grid, st);
   if constexpr (most_rows(PP, NC) >= 32)

@@ -17,69 +17,40 @@ reports it.
 from __future__ import annotations
 
 import ctypes
-import functools
+import importlib
 import math
+import threading
 import time as _time
 from typing import Optional
 
 import torch
 
 from . import _lib
-from .kernel import _X_DT, _tally
+from .kernel import _tally
 
 __all__ = ["rms_norm", "rms_norm_quant", "rope", "rope_freqs", "cache_append", "cache_attn"]
 
-_I64x3 = ctypes.c_int64 * 3
+_lock = threading.Lock()
+_mod = None
+_ENTRY_POINTS = ("bs_rms_norm", "bs_rms_norm_quant", "bs_rope", "bs_cache_append", "bs_cache_attn",
+                 "bs_cache_attn_workspace_size")
 
 
-# Host time counts where a decode step is not captured into a graph: these two are what
-# torch.cuda.current_stream(...).cuda_stream and torch.cuda.current_device() end in, without 2 us of wrapping.
-_raw_stream = torch._C._cuda_getCurrentRawStream
-_current_device = torch._C._cuda_getDevice
-
-
-def _device_of(*ts: Optional[torch.Tensor]) -> int:
-    """The index of the CUDA device that all the tensors are on."""
-    index = ts[0].get_device()
-    if index < 0:
-        raise RuntimeError("bsgemm ops run on CUDA tensors only (no CPU fallback)")
-    for t in ts:
-        if t is not None and t.get_device() != index:
-            raise ValueError(f"tensors on {ts[0].device} and {t.device}")
-    return index
-
-
-def _call(index: int, fn, *args) -> None:
-    """The library call on the current stream of device ``index``, with that device current."""
-    if index == _current_device():
-        status = fn(*args, _raw_stream(index))
-        if status:
-            _lib.check(status)
-    else:
-        with torch.cuda.device(index):
-            _lib.check(fn(*args, _raw_stream(index)))
-
-
-def _ptr(t: Optional[torch.Tensor]):
-    return None if t is None else t.data_ptr()
-
-
-def _norm_args(x, weight, residual):
-    dev = _device_of(x, weight, residual)
-    dt = x.dtype
-    if dt not in _X_DT:
-        raise TypeError(f"rms_norm: x is {dt}, expected bf16, f16 or fp32")
-    if weight.dtype != dt or (residual is not None and residual.dtype != dt):
-        raise TypeError("rms_norm: x, weight and residual must have one type")
-    shape = x.shape
-    if not shape or weight.shape != shape[-1:]:
-        raise ValueError(f"rms_norm: weight {tuple(weight.shape)} does not match x {tuple(shape)}")
-    if residual is not None and residual.shape != shape:
-        raise ValueError(f"rms_norm: residual {tuple(residual.shape)} does not match x {tuple(shape)}")
-    xc = x.contiguous()
-    H = shape[-1]
-    return (dev, _X_DT[dt], H, xc.numel() // H if H else 0, xc, weight.contiguous(),
-            None if residual is None else residual.contiguous(), None if residual is None else torch.empty_like(xc))
+def _native():
+    """The C++ host path (csrc/bind.cpp), calling the library that _lib loaded."""
+    global _mod
+    if _mod is None:
+        with _lock:
+            if _mod is None:
+                lib = _lib.load()
+                try:
+                    mod = importlib.import_module("._native", __package__)
+                except ImportError as e:
+                    raise RuntimeError(f"the serving operators' host path (_native.so) cannot be loaded ({e}): build it "
+                                       "with the package's build.py") from e
+                mod.bind({n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in _ENTRY_POINTS})
+                _mod = mod
+    return _mod
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: Optional[torch.Tensor] = None):
@@ -92,11 +63,11 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual:
     with a residual.
     """
     t0 = _time.perf_counter()
-    dev, dt, H, rows, xc, wc, rc, h = _norm_args(x, weight, residual)
-    y = torch.empty_like(xc)
-    _call(dev, _lib.load().bs_rms_norm, xc.data_ptr(), _ptr(rc), wc.data_ptr(), dt, rows, H, eps, _ptr(h), y.data_ptr())
+    got = (_mod or _native()).rms(x, weight, eps, residual, False, False, False)
+    if got[0]:
+        _lib.check(got[0])
     _tally("rms_norm", t0)
-    return y if h is None else (y, h)
+    return got[1] if residual is None else got[1:]
 
 
 def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: Optional[torch.Tensor] = None,
@@ -109,18 +80,14 @@ def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, res
     with a residual; codes and scales go to fp8_gemm / fp4_gemm.
     """
     t0 = _time.perf_counter()
-    if scale_dtype not in (torch.float32, torch.float8_e8m0fnu):
+    e8m0 = scale_dtype == torch.float8_e8m0fnu
+    if not e8m0 and scale_dtype != torch.float32:
         raise NotImplementedError(f"rms_norm_quant: scale_dtype {scale_dtype} not supported")
-    dev, dt, H, rows, xc, wc, rc, h = _norm_args(x, weight, residual)
-    if H % 128 != 0:
-        raise NotImplementedError(f"rms_norm_quant: H={H} is not a multiple of 128")
-    y = torch.empty_like(xc, dtype=torch.float8_e4m3fn)
-    s = xc.new_empty((*x.shape[:-1], H // 128), dtype=scale_dtype)
-    _call(dev, _lib.load().bs_rms_norm_quant, xc.data_ptr(), _ptr(rc), wc.data_ptr(), dt, rows, H, eps,
-          0 if scale_fmt is None else 1, _ptr(h), y.data_ptr(), s.data_ptr(),
-          _lib.DT_F32 if scale_dtype == torch.float32 else _lib.DT_E8M0)
+    got = (_mod or _native()).rms(x, weight, eps, residual, True, scale_fmt is not None, e8m0)
+    if got[0]:
+        _lib.check(got[0])
     _tally("rms_norm_quant", t0)
-    return (y, s) if h is None else (y, s, h)
+    return got[1:]
 
 
 def rope_freqs(rope_dim: int, base: float = 10000.0, scaling: Optional[str] = None, factor: float = 1.0,
@@ -168,76 +135,13 @@ def rope(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, layout: 
     D multiples of 8.
     """
     t0 = _time.perf_counter()
-    dev = _device_of(x, positions, freqs)
-    dt = _X_DT.get(x.dtype)
-    if dt is None:
-        raise TypeError(f"rope: x is {x.dtype}, expected bf16, f16 or fp32")
-    if positions.dtype != torch.int64 and positions.dtype != torch.int32:
-        raise TypeError(f"rope: positions are {positions.dtype}, expected int64 or int32")
-    if freqs.dtype != torch.float64 or freqs.dim() != 1:
-        raise TypeError("rope: freqs must be a float64 vector")
     if layout not in ("interleaved", "half"):
         raise ValueError(f"rope: layout {layout!r}: expected 'interleaved' or 'half'")
-    shape = x.shape
-    if len(shape) < 2 or positions.shape != shape[:-2]:
-        raise ValueError(f"rope: positions {tuple(positions.shape)} do not match x {tuple(shape)}")
-    H, D = shape[-2:]
-    xt, tok, head = x, H * D, D
-    if not x.is_contiguous() or x.data_ptr() % 16:
-        e = 16 // x.element_size()
-        # one token stride: the leading dims collapse into one, heads and dims stay
-        tok, head = _token_stride(x), x.stride(-2)
-        if tok is None or x.stride(-1) != 1 or head % e or tok % e or x.data_ptr() % 16:
-            if inplace:
-                raise ValueError("rope: an in-place x needs contiguous 16-byte aligned dims and one stride over its tokens")
-            xt, tok, head = x.clone(memory_format=torch.contiguous_format), H * D, D
-    out = xt if inplace else torch.empty_like(x, memory_format=torch.contiguous_format)
-    pc, fc = positions.contiguous(), freqs.contiguous()
-    _call(dev, _lib.load().bs_rope, xt.data_ptr(), dt, pc.numel(), H, D, tok, head, pc.data_ptr(),
-          1 if pc.dtype == torch.int64 else 0, fc.data_ptr(), 2 * fc.numel(), offset, 1 if layout == "half" else 0,
-          1 if inverse else 0, scale, out.data_ptr(), tok if inplace else H * D, head if inplace else D)
+    status, out = (_mod or _native()).rope(x, positions, freqs, layout == "half", offset, inverse, scale, inplace)
+    if status:
+        _lib.check(status)
     _tally("rope", t0)
-    return out
-
-
-def _token_stride(x: torch.Tensor) -> Optional[int]:
-    """The stride of dims 0..-3 taken as one, or None where they are not one."""
-    stride, want = x.size(-1) * x.size(-2), None
-    for i in range(x.dim() - 3, -1, -1):
-        if x.size(i) == 1:
-            continue
-        if want is None:
-            stride = x.stride(i)
-        elif x.stride(i) != want:
-            return None
-        want = x.stride(i) * x.size(i)
-    return stride
-
-
-def _check_cache(name, cache, scale, D, Hkv):
-    if cache.dtype != torch.float8_e4m3fn or scale.dtype != torch.float32:
-        raise TypeError(f"{name}: a cache is float8_e4m3fn with fp32 scales")
-    if cache.dim() != 4 or cache.size(1) != Hkv or cache.size(3) != D or scale.shape != cache.shape[:2]:
-        raise ValueError(f"{name}: cache {tuple(cache.shape)} and scales {tuple(scale.shape)} do not match "
-                         f"[n_pages, {Hkv}, page, {D}]")
-    if not (cache.is_contiguous() and scale.is_contiguous()):
-        raise ValueError(f"{name}: cache and scales must be contiguous")
-
-
-def _check_index(name, what, t, shape):
-    if t.dtype != torch.int32:
-        raise TypeError(f"{name}: {what} is {t.dtype}, expected int32")
-    if t.shape != shape:
-        raise ValueError(f"{name}: {what} {tuple(t.shape)}, expected {tuple(shape)}")
-    return t if t.is_contiguous() else t.contiguous()
-
-
-def _strided(x: torch.Tensor, unit: int, align: int) -> torch.Tensor:
-    """x, or a contiguous copy where its strides do not keep vectors of ``unit`` elements whole."""
-    s = x.stride()
-    if s[3] == 1 and not (s[0] % unit or s[1] % unit or s[2] % unit or x.data_ptr() % align):
-        return x
-    return x.clone(memory_format=torch.contiguous_format)
+    return x if inplace else out
 
 
 def cache_append(k: torch.Tensor, v: Optional[torch.Tensor], k_cache: torch.Tensor, v_cache: Optional[torch.Tensor],
@@ -259,41 +163,10 @@ def cache_append(k: torch.Tensor, v: Optional[torch.Tensor], k_cache: torch.Tens
     they were.  Sequences of one call must not write to the same page.
     """
     t0 = _time.perf_counter()
-    dev = _device_of(k, v, k_cache, v_cache, k_scale, v_scale, block_table, start, new_lens)
-    if k.dim() != 4:
-        raise ValueError(f"cache_append: k {tuple(k.shape)}, expected [B, S, Hkv, D]")
-    B, S, Hkv, D = k.shape
-    if (v is None) != (v_cache is None) or (v is None) != (v_scale is None):
-        raise ValueError("cache_append: v, v_cache and v_scale go together")
-    if k.dtype not in _X_DT or (v is not None and v.dtype != k.dtype):
-        raise TypeError("cache_append: k and v must have one type of bf16, f16 or fp32")
-    _check_cache("cache_append", k_cache, k_scale, D, Hkv)
-    if v is not None:
-        if v.shape != k.shape or v_cache.shape != k_cache.shape:
-            raise ValueError("cache_append: v does not match k")
-        _check_cache("cache_append", v_cache, v_scale, D, Hkv)
-    if block_table.dim() != 2:
-        raise ValueError("cache_append: block_table must be [B, max_pages]")
-    bt = _check_index("cache_append", "block_table", block_table, (B, block_table.size(1)))
-    st = _check_index("cache_append", "start", start, (B,))
-    nl = None if new_lens is None else _check_index("cache_append", "new_lens", new_lens, (B,))
-    if S == 0 or B == 0:
-        return
-    e = 16 // k.element_size()
-    kc = _strided(k, e, 16)
-    vc = None if v is None else _strided(v, e, 16)
-    _call(dev, _lib.load().bs_cache_append, kc.data_ptr(), _ptr(vc), _X_DT[k.dtype], B, S, Hkv, D,
-          _I64x3(*kc.stride()[:3]), None if vc is None else _I64x3(*vc.stride()[:3]), k_cache.data_ptr(), _ptr(v_cache),
-          k_scale.data_ptr(), _ptr(v_scale), k_cache.size(0), k_cache.size(2), bt.data_ptr(), bt.size(1), st.data_ptr(),
-          _ptr(nl))
+    status = (_mod or _native()).append(k, v, k_cache, v_cache, k_scale, v_scale, block_table, start, new_lens)
+    if status:
+        _lib.check(status)
     _tally("cache_append", t0)
-
-
-@functools.lru_cache(maxsize=4096)
-def _attn_workspace(index: int, B: int, S: int, H: int, Hkv: int, D: int, dt: int) -> int:
-    with torch.cuda.device(index):
-        n = _lib.load().bs_cache_attn_workspace_size(B, S, H, Hkv, D, dt)
-    return (max(n, 256) + 3) // 4 * 4
 
 
 def cache_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: Optional[torch.Tensor], k_scale: torch.Tensor,
@@ -313,43 +186,9 @@ def cache_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: Optional[torch.T
     it.
     """
     t0 = _time.perf_counter()
-    dev = _device_of(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, attn_sink, new_lens)
-    if q.dim() != 4:
-        raise ValueError(f"cache_attn: q {tuple(q.shape)}, expected [B, S, H, D]")
-    B, S, H, D = q.shape
-    if q.dtype not in (torch.bfloat16, torch.float16):
-        raise TypeError(f"cache_attn: q is {q.dtype}, expected bf16 or f16")
-    if (v_cache is None) != (v_scale is None):
-        raise ValueError("cache_attn: v_cache and v_scale go together")
-    if k_cache.dim() != 4:
-        raise ValueError(f"cache_attn: k_cache {tuple(k_cache.shape)}, expected [n_pages, Hkv, page, D]")
-    Hkv = k_cache.size(1)
-    _check_cache("cache_attn", k_cache, k_scale, D, Hkv)
-    if v_cache is not None:
-        _check_cache("cache_attn", v_cache, v_scale, D, Hkv)
-        if v_cache.shape != k_cache.shape:
-            raise ValueError("cache_attn: v_cache does not match k_cache")
-    if Hkv == 0 or H % Hkv:
-        raise ValueError(f"cache_attn: {H} query heads over {Hkv} kv heads")
-    if block_table.dim() != 2:
-        raise ValueError("cache_attn: block_table must be [B, max_pages]")
-    bt = _check_index("cache_attn", "block_table", block_table, (B, block_table.size(1)))
-    sl = _check_index("cache_attn", "seq_lens", seq_lens, (B,))
-    nl = None if new_lens is None else _check_index("cache_attn", "new_lens", new_lens, (B,))
-    sink = None
-    if attn_sink is not None:
-        if attn_sink.shape != (H,):
-            raise ValueError(f"cache_attn: attn_sink {tuple(attn_sink.shape)}, expected ({H},)")
-        sink = attn_sink.float().contiguous()
-    out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    if out.numel() == 0:
-        return out
-    qc = _strided(q, 4, 8)
-    dt = _X_DT[q.dtype]
-    ws = bt.new_empty(_attn_workspace(dev, B, S, H, Hkv, D, dt) // 4)
-    _call(dev, _lib.load().bs_cache_attn, qc.data_ptr(), dt, B, S, H, Hkv, D, _I64x3(*qc.stride()[:3]),
-          k_cache.data_ptr(), _ptr(v_cache), k_scale.data_ptr(), _ptr(v_scale), k_cache.size(0), k_cache.size(2),
-          bt.data_ptr(), bt.size(1), sl.data_ptr(), _ptr(nl), _ptr(sink), softmax_scale, out.data_ptr(), ws.data_ptr(),
-          4 * ws.numel())
+    status, out = (_mod or _native()).attn(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, softmax_scale,
+                                           attn_sink, new_lens)
+    if status:
+        _lib.check(status)
     _tally("cache_attn", t0)
     return out
