@@ -14,7 +14,7 @@
 #include <torch/types.h>
 
 #include <optional>
-#include <sstream>
+#include <string>
 
 #include "../../include/bsgemm.h"
 
@@ -42,11 +42,20 @@ void bind(const py::dict& address) {
   get("bs_cache_attn_workspace_size", p_cache_attn_ws);
 }
 
+// Messages are put together without iostreams: formatting a number through one crashed here (facets of another copy of
+// the C++ library in the process).
+std::string str(const char* s) { return s; }
+std::string str(int64_t v) { return std::to_string(v); }
+std::string str(at::ScalarType t) { return c10::toString(t); }
+std::string str(const c10::Device& d) { return d.str(); }
+std::string str(at::IntArrayRef v) {
+  std::string s = "[";
+  for (size_t i = 0; i < v.size(); ++i) s += (i ? ", " : "") + std::to_string(v[i]);
+  return s + "]";
+}
 template <class... A>
 std::string text(const A&... a) {
-  std::ostringstream s;
-  (s << ... << a);
-  return s.str();
+  return (std::string() + ... + str(a));
 }
 template <class... A>
 [[noreturn]] void bad_type(const A&... a) { throw py::type_error(text(a...)); }

@@ -341,3 +341,335 @@ ATTN_LONG = [
 @pytest.mark.parametrize("case", ATTN + ATTN_LONG, ids=lambda c: "-".join(str(x) for x in c).replace(" ", ""))
 def test_cache_attn(pkg, case):
     run_attn(pkg, *case)
+
+
+# ------------------------------------------------------------------ cache attention: what goes wrong at the edges
+
+def check(pkg, q, cache, table, lens, scale=None, sink=None, new_lens=None):
+    D = q.shape[-1]
+    scale = D ** -0.5 if scale is None else scale
+    sl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    nl = None if new_lens is None else torch.tensor(new_lens, dtype=torch.int32, device="cuda")
+    got = pkg.cache_attn(q, *cache, table, sl, scale, attn_sink=sink, new_lens=nl)
+    want, bound = ref.attn(q, *cache, table, sl, scale, sink=sink, new_lens=nl)
+    tol = ref.attn_tolerance(q.dtype, D, want, bound)
+    assert ((got.double() - want).abs() <= tol).all()
+    return got
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("S", [1, 5])
+def test_cache_attn_empty_rows(pkg, dt, S):
+    """Sequences without tokens, shorter than their new tokens, padded queries: zero rows, the others right."""
+    g = gen(21 + S)
+    lens = [0, 300, 2, 129, 0, 1]
+    table, n = make_table(g, lens, 32)
+    cache = make_cache(g, n, 2, 32, 64)
+    q = randn(g, 6, S, 8, 64, dtype=DT[dt])
+    got = check(pkg, q, cache, table, lens)
+    assert (got[0] == 0).all() and (got[4] == 0).all()
+    if S > 2:
+        assert (got[2, :S - 2] == 0).all() and (got[2, S - 2:] != 0).any()
+    new = [min(S, x) for x in (3, 1, 2, 0, 5, 1)]
+    got = check(pkg, q, cache, table, lens, new_lens=new)
+    for b, m in enumerate(new):
+        assert (got[b, m:] == 0).all()
+    sink = randn(g, 8)
+    got = check(pkg, q, cache, table, lens, sink=sink)
+    assert (got[0] == 0).all()
+
+
+@pytest.mark.parametrize("page,H,Hkv,D,shared", [(16, 8, 2, 64, False), (64, 64, 1, 512, True), (128, 64, 2, 128, False),
+                                                 (32, 12, 1, 256, False), (64, 20, 1, 320, True)])
+@pytest.mark.parametrize("S", [1, 9])
+def test_cache_attn_nan_in_hidden_slots(pkg, page, H, Hkv, D, shared, S):
+    """What lies behind a sequence's tokens (unwritten slots of its last page, here NaN codes) reaches no row; a NaN in
+    a new token reaches the rows that see it, in its dims (values) or wholly (keys), and no other."""
+    g = gen(page + H + S)
+    lens = [page * 3 + 7, 140, page]
+    table, n = make_table(g, lens, page)
+    cache = make_cache(g, n, Hkv, page, D, shared)
+    q = randn(g, 3, S, H, D, dtype=torch.bfloat16)
+    clean = check(pkg, q, cache, table, lens)
+    dirty = [None if t is None else t.clone() for t in cache]
+    for codes in dirty[:2]:
+        if codes is not None:
+            raw = codes.view(torch.uint8)
+            for b, m in enumerate(lens):
+                if m % page:
+                    raw[table[b, m // page].long(), :, m % page:] = 0x7F
+    sl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    got = pkg.cache_attn(q, *dirty, table, sl, D ** -0.5)
+    assert torch.equal(got, clean)
+    if S == 1:
+        return
+    # the fourth new token of sequence 1, kv head 0: dims 3 and D - 1 of its value
+    at = lens[1] - S + 3
+    i = table[1, at // page].long()
+    codes = dirty[0] if shared else dirty[1]
+    codes.view(torch.uint8)[i, 0, at % page, 3] = 0xFF
+    codes.view(torch.uint8)[i, 0, at % page, D - 1] = 0x7F
+    got = pkg.cache_attn(q, *dirty, table, sl, D ** -0.5)
+    G = H // Hkv
+    bad = torch.zeros_like(got, dtype=torch.bool)
+    if shared:
+        bad[1, 3:, :G] = True                     # a NaN key is a NaN score
+    else:
+        bad[1, 3:, :G, 3] = True
+        bad[1, 3:, :G, D - 1] = True
+    assert torch.equal(got.isnan(), bad)
+    assert torch.equal(got[~bad], clean[~bad])
+
+
+def test_cache_attn_odd_queries(pkg):
+    """Rows of zeros, infinities and NaN stay their own; huge and tiny rows; scales of either sign and zero; sinks of
+    any size; queries inside a wider projection and at an odd offset."""
+    g = gen(31)
+    lens = [500, 77]
+    table, n = make_table(g, lens, 64)
+    cache = make_cache(g, n, 2, 64, 128)
+    q = randn(g, 2, 3, 8, 128, dtype=torch.bfloat16)
+    q[0, 0, 0] = 0
+    q[0, 0, 1] *= 1e-30
+    q[0, 1, 2] *= 100
+    check(pkg, q, cache, table, lens)
+    check(pkg, q, cache, table, lens, scale=-0.05)
+    got = check(pkg, q, cache, table, lens, scale=0.0)
+    sink = torch.tensor([-float("inf"), -100.0, 0.0, 5.0, 30.0, 80.0, -3e38, 3.0], device="cuda")
+    check(pkg, q, cache, table, lens, sink=sink)
+    clean = pkg.cache_attn(q, *cache, table, torch.tensor(lens, dtype=torch.int32, device="cuda"), 0.1)
+    q2 = q.clone()
+    q2[0, 1, 4, 7], q2[1, 2, 0, 127] = float("inf"), float("nan")
+    got = pkg.cache_attn(q2, *cache, table, torch.tensor(lens, dtype=torch.int32, device="cuda"), 0.1)
+    bad = torch.zeros(2, 3, 8, dtype=torch.bool, device="cuda")
+    bad[0, 1, 4] = bad[1, 2, 0] = True
+    assert got[bad].isnan().all() and torch.equal(got[~bad], clean[~bad])
+    wide = torch.zeros(2, 3, 3 * 8 * 128 + 8, dtype=torch.bfloat16, device="cuda")
+    for off in (1024, 1028, 1025):               # aligned, 8-byte aligned, neither (copied)
+        view = wide[..., off:off + 1024].view(2, 3, 8, 128) if off % 4 == 0 else wide[..., off:off + 1024].unflatten(-1, (8, 128))
+        view.copy_(q)
+        assert torch.equal(pkg.cache_attn(view, *cache, table, torch.tensor(lens, dtype=torch.int32, device="cuda"), 0.1), clean)
+
+
+def test_cache_attn_scales(pkg):
+    """Page scales of any size, not only powers of two; a page of zeros; a value scale of zero and of very different pages."""
+    g = gen(41)
+    lens = [700]
+    table, n = make_table(g, lens, 16)
+    k, v, ks, vs = make_cache(g, n, 4, 16, 64)
+    ks.mul_(torch.rand(ks.shape, generator=g, device="cuda") + 0.5)
+    vs.copy_(torch.exp2(torch.randint(-30, 10, vs.shape, generator=g, device="cuda").float()) * 1.7)
+    vs[table[0, 3].long()] = 0
+    k.view(torch.uint8)[table[0, 5].long()] = 0
+    check(pkg, randn(g, 1, 1, 16, 64, dtype=torch.float16), (k, v, ks, vs), table, lens)
+
+
+def test_cache_attn_many_sequences(pkg):
+    """More (sequence, row tile) pairs than threads of a CTA, and many empty sequences among them."""
+    g = gen(51)
+    lens = [int(x) for x in torch.randint(-200, 300, (1500,), generator=g, device="cuda").clamp(min=0).tolist()]
+    table, n = make_table(g, lens, 16)
+    cache = make_cache(g, n, 1, 16, 32)
+    check(pkg, randn(g, 1500, 1, 4, 32, dtype=torch.bfloat16), cache, table, lens)
+
+
+def test_cache_beyond_32_bits(pkg):
+    """Pages whose bytes lie beyond 2^32 in the cache: append and attention."""
+    page, D, n = 128, 512, 66000                  # 4.3 GB
+    k_cache = torch.zeros(n, 1, page, D, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+    ks = torch.ones(n, 1, device="cuda")
+    g = gen(61)
+    table = torch.tensor([[65999, 3, 65537], [32768, 65536, 1]], dtype=torch.int32, device="cuda")
+    k = randn(g, 2, 300, 1, D, dtype=torch.bfloat16)
+    start = torch.tensor([0, 0], dtype=torch.int32, device="cuda")
+    pkg.cache_append(k, None, k_cache, None, ks, None, table, start)
+    small = [65999, 3, 65537, 32768, 65536, 1]
+    t2 = torch.tensor([[0, 1, 2], [3, 4, 5]], device="cuda")
+    want, ws = ref.append(k, torch.zeros(6, 1, page, D, device="cuda"), torch.ones(6, 1, device="cuda"), t2, start)
+    assert same_codes(k_cache[small], want) and torch.equal(ks[small].double(), ws)
+    q = randn(g, 2, 1, 16, D, dtype=torch.bfloat16)
+    lens = torch.tensor([300, 300], dtype=torch.int32, device="cuda")
+    got = pkg.cache_attn(q, k_cache, None, ks, None, table, lens, D ** -0.5)
+    near = pkg.cache_attn(q, k_cache[small], None, ks[small], None, t2.to(torch.int32), lens, D ** -0.5)
+    assert torch.equal(got, near)
+
+
+def test_cache_attn_bad_index(pkg):
+    """Page indices and lengths out of range read as absent and are reported."""
+    g = gen(71)
+    lens = [200, 150]
+    table, n = make_table(g, lens, 64)
+    cache = make_cache(g, n, 2, 64, 64)
+    q = randn(g, 2, 1, 4, 64, dtype=torch.bfloat16)
+    bad = table.clone()
+    bad[0, 1] = n
+    bad[1, 2] = -7
+    sl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    got = pkg.cache_attn(q, *cache, bad, sl, 0.125)
+    with pytest.raises(pkg._lib.BsError, match="out of range"):
+        pkg._lib.device_error_check()
+    # the same with those pages' tokens taken out
+    t2 = torch.full((2, 3), -1, dtype=torch.int32, device="cuda")
+    t2[0] = table[0, [0, 2, 3]]
+    t2[1, :2] = table[1, :2]
+    check(pkg, q, cache, t2, [136, 128])
+    want, bound = ref.attn(q, *cache, t2, torch.tensor([136, 128]), 0.125)
+    assert ((got.double() - want).abs() <= ref.attn_tolerance(q.dtype, 64, want, bound)).all()
+    got = pkg.cache_attn(q, *cache, table, torch.tensor([-1, 100000], dtype=torch.int32, device="cuda"), 0.125)
+    with pytest.raises(pkg._lib.BsError, match="out of range"):
+        pkg._lib.device_error_check()
+    assert (got == 0).all()
+
+
+def test_refusals(pkg):
+    """Python-level refusals that need CUDA tensors."""
+    g = gen(81)
+    table, n = make_table(g, [40], 16)
+    k, v, ks, vs = make_cache(g, n, 2, 16, 64)
+    q = randn(g, 1, 1, 4, 64, dtype=torch.bfloat16)
+    sl = torch.tensor([40], dtype=torch.int32, device="cuda")
+    x, w = randn(g, 2, 256, dtype=torch.bfloat16), torch.ones(256, dtype=torch.bfloat16, device="cuda")
+    pos, f = torch.zeros(1, 1, dtype=torch.int64, device="cuda"), pkg.rope_freqs(64)
+    for err, call in [
+            (TypeError, lambda: pkg.rms_norm(x, w.float())), (TypeError, lambda: pkg.rms_norm(x.double(), w.double())),
+            (ValueError, lambda: pkg.rms_norm(x, w[:128])), (ValueError, lambda: pkg.rms_norm(x, w, residual=x[:1])),
+            (ValueError, lambda: pkg.rms_norm(x, w.cpu())), (NotImplementedError, lambda: pkg.rms_norm_quant(x[:, :200], w[:200])),
+            (TypeError, lambda: pkg.rope(q, pos.float(), f)), (TypeError, lambda: pkg.rope(q, pos, f.float())),
+            (ValueError, lambda: pkg.rope(q, pos[0], f)), (ValueError, lambda: pkg.rope(q, pos, f, offset=8)),
+            (NotImplementedError, lambda: pkg.rope(q, pos, f[:5])),
+            (ValueError, lambda: pkg.rope(q.transpose(2, 3), pos, f, inplace=True)),
+            (TypeError, lambda: pkg.cache_attn(q.float(), k, v, ks, vs, table, sl, 1.0)),
+            (TypeError, lambda: pkg.cache_attn(q, k, v, ks, vs, table.long(), sl, 1.0)),
+            (TypeError, lambda: pkg.cache_attn(q, k.view(torch.uint8), v, ks, vs, table, sl, 1.0)),
+            (ValueError, lambda: pkg.cache_attn(q, k, v, ks, None, table, sl, 1.0)),
+            (ValueError, lambda: pkg.cache_attn(q[:, :, :3], k, v, ks, vs, table, sl, 1.0)),
+            (ValueError, lambda: pkg.cache_attn(q, k, v, ks, vs, table, sl, 1.0, attn_sink=ks[0])),
+            (ValueError, lambda: pkg.cache_attn(q, k[:, :, :, :32], v, ks, vs, table, sl, 1.0)),
+            (ValueError, lambda: pkg.cache_attn(q, k, v, ks, vs, table, torch.cat((sl, sl)), 1.0)),
+            (NotImplementedError, lambda: pkg.cache_attn(q, k[:, :, :8].contiguous(), v[:, :, :8].contiguous(), ks, vs, table, sl, 1.0)),
+            (TypeError, lambda: pkg.cache_append(q, q.half(), k, v, ks, vs, table, sl)),
+            (ValueError, lambda: pkg.cache_append(q, None, k, v, ks, vs, table, sl)),
+            (ValueError, lambda: pkg.cache_append(q, q, k, v, ks, vs, table, sl)),
+            (ValueError, lambda: pkg.cache_append(q[:, :, :2], q[:, :, :2], k, v, ks, vs[:1], table, sl))]:
+        with pytest.raises(err):
+            call()
+
+
+# ------------------------------------------------------------------ streams, graphs, the same bits again
+
+def serving_inputs(g, lens, page=64, Hkv=2, D=128, H=16, S=1):
+    table, n = make_table(g, [x + S for x in lens], page)
+    cache = make_cache(g, n, Hkv, page, D)
+    return (randn(g, len(lens), S, H, D, dtype=torch.bfloat16), randn(g, len(lens), S, Hkv, D, dtype=torch.bfloat16),
+            randn(g, len(lens), S, Hkv, D, dtype=torch.bfloat16), cache, table)
+
+
+def test_same_bits_again(pkg):
+    g = gen(91)
+    lens = [5000, 1, 700, 12345]
+    q, k, v, cache, table = serving_inputs(g, lens)
+    sl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    first = pkg.cache_attn(q, *cache, table, sl, 0.1)
+    for _ in range(20):
+        assert torch.equal(pkg.cache_attn(q, *cache, table, sl, 0.1), first)
+
+
+def test_graphs_and_streams(pkg):
+    """One decode step captured twice (two graphs with memory of their own), replayed with new inputs and lengths, at once
+    on two streams, against eager calls on a third."""
+    P = pkg
+    f = P.rope_freqs(128)
+
+    class Step:
+        def __init__(self, seed):
+            g = gen(seed)
+            self.lens = [900, 17, 300]
+            self.q, self.k, self.v, (kc, vc, ks, vs), self.table = serving_inputs(g, [x + 30 for x in self.lens])
+            self.cache = (kc, vc, ks, vs)
+            self.start = torch.tensor(self.lens, dtype=torch.int32, device="cuda")
+            self.x, self.w = randn(g, 3, 1024, dtype=torch.bfloat16), torch.ones(1024, dtype=torch.bfloat16, device="cuda")
+
+        def run(self, cache):
+            y, s = P.rms_norm_quant(self.x, self.w)
+            pos = self.start.view(3, 1)
+            q = P.rope(self.q, pos, f)
+            P.cache_append(P.rope(self.k, pos, f), self.v, cache[0], cache[1], cache[2], cache[3], self.table, self.start)
+            return y, s, P.cache_attn(q, *cache, self.table, self.start + 1, 0.1)
+
+    steps = [Step(1), Step(2)]
+    graphs = []
+    for st in steps:
+        st.eager = [t.clone() for t in st.cache]
+        st.run([t.clone() for t in st.cache])
+        torch.cuda.synchronize()
+        gr = torch.cuda.CUDAGraph()
+        keep = [t.clone() for t in st.cache]
+        with torch.cuda.graph(gr):
+            st.out = st.run(st.cache)
+        for a, b in zip(st.cache, keep):
+            a.copy_(b)
+        graphs.append(gr)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    side = torch.cuda.Stream()
+    for it in range(6):
+        g = gen(100 + it)
+        for st in steps:
+            for t in (st.q, st.k, st.v, st.x):
+                t.copy_(randn(g, *t.shape, dtype=t.dtype))
+        torch.cuda.synchronize()
+        for gr, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                gr.replay()
+        want = []
+        with torch.cuda.stream(side):
+            for st in steps:
+                want.append(st.run(st.eager))
+        torch.cuda.synchronize()
+        for st, w in zip(steps, want):
+            for a, b in zip(st.out, w):
+                assert torch.equal(a.view(torch.uint8) if a.dtype == torch.float8_e4m3fn else a,
+                                   b.view(torch.uint8) if b.dtype == torch.float8_e4m3fn else b)
+            for a, b in zip(st.cache, st.eager):
+                assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+            st.start.add_(1)
+
+
+def test_layer_step(pkg):
+    """A decoder layer's attention half as it is used: norm into e4m3, the projection, rotary positions in place on its
+    query and key heads, append, attention, for a prompt and then single tokens; against 64-bit operations on the stored
+    codes at every step."""
+    g = gen(7)
+    B, Hd, H, Hkv, D, page = 2, 512, 8, 2, 64, 16
+    qkv_rows = (H + 2 * Hkv) * D
+    w = (1 + 0.1 * randn(g, Hd)).bfloat16()
+    ws = torch.rand(qkv_rows // 128, Hd // 128, generator=g, device="cuda") * 1e-3 + 1e-4
+    wq = (randn(g, qkv_rows, Hd) * 60).clamp(-448, 448).to(torch.float8_e4m3fn)
+    freqs = pkg.rope_freqs(32)
+    lens = [0, 0]
+    table, n = make_table(g, [60, 90], page)
+    kc, vc, ks, vs = make_cache(g, n, Hkv, page, D)
+    h = None
+    for new in ([37, 50], [1, 1], [1, 1], [3, 2]):
+        S = max(new)
+        x = randn(g, B, S, Hd, dtype=torch.bfloat16)
+        res = randn(g, B, S, Hd, dtype=torch.bfloat16) if h is None or h.shape[1] != S else h
+        y, s, h = pkg.rms_norm_quant(x, w, residual=res)
+        want = ref.rms((x.float() + res.float()).bfloat16(), w, 1e-6)
+        deq = y.to(torch.float32).double().unflatten(-1, (-1, 128)) * s.double()[..., None]
+        assert ((deq.flatten(-2) - want).abs() <= torch.maximum(want.abs() * 2.0 ** -4, s.double().repeat_interleave(128, -1) * 2.0 ** -10) * 1.01).all()
+        qkv = pkg.fp8_gemm(y, s, wq, ws)
+        exact = deq.flatten(-2) @ (wq.to(torch.float32).double() * ws.double().repeat_interleave(128, 0).repeat_interleave(128, 1)).T
+        assert ((qkv.double() - exact).norm() / exact.norm()) < 1e-2
+        heads = qkv.view(B, S, H + 2 * Hkv, D)
+        start = torch.tensor(lens, dtype=torch.int32, device="cuda")
+        pos = start.long()[:, None] + torch.arange(S, device="cuda")
+        turned = ref.rope(heads[:, :, :H + Hkv], pos, freqs, "half", 0)
+        pkg.rope(heads[:, :, :H + Hkv], pos, freqs, layout="half", inplace=True)
+        assert ((heads[:, :, :H + Hkv].double() - turned).abs() <= turned.abs() * 2.0 ** -8 + heads.double().abs().amax() * 2.0 ** -19).all()
+        q, k, v = heads[:, :, :H], heads[:, :, H:H + Hkv], heads[:, :, H + Hkv:]
+        nl = torch.tensor(new, dtype=torch.int32, device="cuda")
+        wk, wv = ref.append(k, kc.float(), ks, table, start, nl), ref.append(v, vc.float(), vs, table, start, nl)
+        pkg.cache_append(k, v, kc, vc, ks, vs, table, start, nl)
+        assert same_codes(kc, wk[0]) and torch.equal(ks.double(), wk[1]) and same_codes(vc, wv[0]) and torch.equal(vs.double(), wv[1])
+        lens = [a + b for a, b in zip(lens, new)]
+        check(pkg, q, (kc, vc, ks, vs), table, lens, scale=D ** -0.5 / 4, new_lens=new)
