@@ -14,13 +14,15 @@
 //
 //   x = c1 + c2/16 + c3/256,  c1 = e4m3(x), c2 = e4m3(16 (x - c1)), ...
 //
-// Each e4m3 term takes 4 significant bits.  Two terms hold a bf16 value
-// exactly (8 bits); three hold an f16 value (11 bits).  Rows of Q are first
+// Rounding to e4m3 leaves at most 2^-4 of the value's power of two, after the
+// second term 2^-9 and after the third 2^-14, so two terms hold a bf16 value
+// (8 bits) exactly and three an f16 value (11 bits).  Rows of Q are first
 // scaled by a power of two so that their amax lies in [128, 256): what the
 // terms cannot hold is below 2^-22 of the row's amax for two terms and 2^-26
 // for three.  P = exp2(s - max) * (page's value scale / largest of the tile) *
-// 256 is rounded to the same number of terms: 2^-8 of the value at most with
-// bf16 outputs (half a step of bf16 itself is 2^-8), 2^-12 with f16.
+// 256 is rounded to the same number of terms: with bf16 outputs to 2^-8 of the
+// value at most (2^-9, and f16 on the way; half a step of bf16 itself is
+// 2^-8), with f16 outputs to 2^-14.
 // Accumulation is fp32 in TMEM; O is taken out after every tile and added, in
 // fp32, to accumulators in registers, where the running maximum's factor and
 // the tile's value scale are applied.
@@ -292,9 +294,9 @@ BS_DEVINL uint16_t h2_to_e4m3x2(__half2 v) {
   asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(c) : "r"(*reinterpret_cast<uint32_t*>(&v)));
   return c;
 }
-// The PP terms of two values, from f16.  A weight loses 2^-12 of its value at most by that (three terms then hold its 11
-// bits); a value of Q, 8 or 11 bits wide on a scale where its row's largest is in [128, 256), nothing above 2^-25.
-// Differences of a value and its nearest e4m3 neighbour are exact.
+// The PP terms of two values of Q: they are f16 numbers here (8 or 11 bits on a scale where the row's largest is in
+// [128, 256); what f16 loses is below 2^-25 on that scale).  Differences of a value and its nearest e4m3 neighbour are
+// exact.
 template <int PP>
 BS_DEVINL void split2h(float x, float y, uint16_t* c) {
   __half2 v = __floats2half2_rn(x, y);
@@ -302,6 +304,25 @@ BS_DEVINL void split2h(float x, float y, uint16_t* c) {
   for (int p = 0; p < PP; ++p) {
     c[p] = h2_to_e4m3x2(v);
     if (p + 1 < PP) v = __hmul2(__hsub2(v, e4m3x2_to_h2(c[p])), __float2half2_rn(16.0f));
+  }
+}
+// The same for two weights: with two terms (2^-9 of the value is left) through f16, whose 2^-11 is below that; with three
+// (2^-14) in fp32.
+template <int PP>
+BS_DEVINL void split2p(float x, float y, uint16_t* c) {
+  if constexpr (PP == 2) {
+    split2h<PP>(x, y, c);
+  } else {
+#pragma unroll
+    for (int p = 0; p < PP; ++p) {
+      c[p] = bs_cvt_e4m3x2(x, y);
+      if (p + 1 < PP) {
+        const float2 b = __half22float2(e4m3x2_to_h2(c[p]));
+        const float2 r = mul2(add2(make_float2(x, y), make_float2(-b.x, -b.y)), both(16.0f));
+        x = r.x;
+        y = r.y;
+      }
+    }
   }
 }
 
@@ -849,7 +870,7 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
         for (int g = 0; g < K; ++g) {
           uint16_t c[PP];
           const float2 w = mul2(s[g][k], ratio);
-          split2h<PP>(w.x, w.y, c);
+          split2p<PP>(w.x, w.y, c);
 #pragma unroll
           for (int t = 0; t < PP; ++t) {
             const int n = t * R + row0 + 8 * g;

@@ -11,11 +11,12 @@
 //   code = e4m3_rn(y / s)      2^ceil(log2 s) for s in the power-of-two form
 //
 // The codes come from the fp32 y: act_quant(rms_norm(x)) would round y to 16
-// bits first.  y is the fp32 number nearest to its exact value: squares are
-// summed in fp64 (a 16-bit value's is exact in fp32, but rounding errors of an
-// fp32 sum move a whole row by up to 2^-22, and every value that near to the
-// border of two codes with it), and the root is kept as a sum of two fp32.
-// y / s is y * (1/s): exact for powers of two, else within 2 ulp.
+// bits first.  y is the fp32 number nearest to its exact value: per-thread sums
+// of 8 squares are added up in fp64 (for few rows every square is), the root is
+// kept as a sum of two fp32.  s and y / s are rounded to nearest as well.  It
+// costs a few instructions under the loads, and values next to the border of
+// two codes (with 16-bit inputs y / s often lies on one) fall as the formula
+// in exact fp32 steps says.
 //
 // HBM-bound: every value is read and written once.  A block of 128 values is
 // half a warp x 8 values, so its amax is four shuffles.  Two forms:
@@ -66,8 +67,6 @@ struct Args {
   int s_e8m0, pow2;
 };
 
-// What follows the loads, for a thread's vectors f (h, as loaded and added up) of one row: y, out or codes.
-// `put(c, v)` hands over vector c of y; sum of squares in, through `part`, one barrier.
 // max that propagates NaN, as torch.amax
 BS_DEVINL float max_nan(float a, float b) {
   float r;
@@ -107,32 +106,32 @@ BS_DEVINL float2 inv_sqrt(double v) {
   return make_float2(hi, fabsf(hi) < __uint_as_float(0x7F800000u) ? (float)(x - (double)hi) : 0.0f);
 }
 
-// y of one vector, in place.
+// y of one vector, in place; returns what put_codes takes as its largest.
 template <typename T>
-BS_DEVINL void scale_row(float* f, const float* g, float2 r) {
+BS_DEVINL float scale_row(float* f, const float* g, float2 r) {
+  float m = 0.0f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float p = f[i] * g[i];                                   // exact for 16-bit values
     float e = p * r.y;
     if (sizeof(T) == 4) e = fmaf(fmaf(f[i], g[i], -p), r.x, e);
     f[i] = fmaf(p, r.x, e);
+    m = max_nan(m, fabsf(sizeof(T) == 4 ? f[i] : p));
   }
+  return m;
 }
 
 // Codes and scales of a thread's V vectors of y (vector v is number v blockDim + threadIdx of the row; H is a multiple
 // of 128, so the 16 lanes of a block are all in the row or all out).  The V maxima over 16 lanes go through one
 // butterfly, which leaves each group of lanes with one vector's: 5 shuffles for four vectors instead of 16, and one
 // scale to compute per lane instead of four.
+//
+// `pmax`: the V vectors' largest |h w|, exact for 16-bit types, whose product with the row's factor r gives the block's
+// amax unrounded; for fp32 the rounded y's largest magnitude, r = 1.
 template <int V>
-BS_DEVINL void put_codes(const Args& a, int64_t row, int nvec, const float (*f)[8]) {
+BS_DEVINL void put_codes(const Args& a, int64_t row, int nvec, const float (*f)[8], const float* pmax, float2 r) {
   const int lane = threadIdx.x & 31;
-  float m[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    m[v] = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m[v] = max_nan(m[v], fabsf(f[v][i]));
-  }
+  const float* m = pmax;
   int own = 0;                       // the vector whose maximum this lane ends up with
   float amax;
   if constexpr (V == 4) {
@@ -152,16 +151,16 @@ BS_DEVINL void put_codes(const Args& a, int64_t row, int nvec, const float (*f)[
   }
   amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
   amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-  amax = max_nan(amax, 1e-4f);
-  // amax / 448 rounded to nearest, for a finite amax; an infinite or NaN one is its own quotient
-  float s = amax < __uint_as_float(0x7F800000u) ? div_markstein(amax, 448.0f, 1.0f / 448.0f) : amax;
-  float z;
-  if (a.pow2) {
-    s = bs_round_pow2(s);
-    z = s < __uint_as_float(0x7F800000u) ? bs_inv_pow2(s) : __fdividef(1.0f, s);
-  } else {
-    asm("rcp.approx.f32 %0, %1;" : "=f"(z) : "f"(s));               // 1 ulp
+  // amax / 448: the exact products' tail corrects the rounded quotient (an infinite or NaN amax is its own quotient)
+  const float top = max_nan(amax * r.x, 1e-4f);
+  float s = top;
+  if (top < __uint_as_float(0x7F800000u)) {
+    const float tail = top == 1e-4f ? 0.0f : fmaf(amax, r.y, fmaf(amax, r.x, -top));
+    const float q = div_markstein(top, 448.0f, 1.0f / 448.0f);
+    s = fmaf(fmaf(-448.0f, q, top) + tail, 1.0f / 448.0f, q);
   }
+  if (a.pow2) s = bs_round_pow2(s);
+  const float z = a.pow2 && s < __uint_as_float(0x7F800000u) ? bs_inv_pow2(s) : __frcp_rn(s);
   const int c_own = own * blockDim.x + threadIdx.x;
   if ((lane & (V == 4 ? 3 : V == 2 ? 7 : 15)) == 0 && c_own < nvec) {
     const int64_t at = row * (a.H >> 7) + (c_own >> 4);
@@ -171,10 +170,24 @@ BS_DEVINL void put_codes(const Args& a, int64_t row, int nvec, const float (*f)[
   uint8_t* y = reinterpret_cast<uint8_t*>(a.y) + row * a.H + threadIdx.x * 8;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    const float k = V == 1 ? z : __shfl_sync(0xffffffffu, z, (lane & 16) + (v & 1) * 8 + (v >> 1) * 4);
+    const int from = (lane & 16) + (v & 1) * 8 + (v >> 1) * 4;
+    const float k = V == 1 ? z : __shfl_sync(0xffffffffu, z, from);
+    float g[8];
+    if (a.pow2) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) g[i] = f[v][i] * k;
+    } else {
+      // one correction of y * RN(1/s): the remainder is exact, so the sum rounds to the nearest of y / s
+      const float d = V == 1 ? s : __shfl_sync(0xffffffffu, s, from);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        g[i] = f[v][i] * k;
+        g[i] = fmaf(fmaf(-d, g[i], f[v][i]), k, g[i]);
+      }
+    }
     uint2 q;
-    q.x = bs_cvt_e4m3x2(f[v][0] * k, f[v][1] * k) | ((uint32_t)bs_cvt_e4m3x2(f[v][2] * k, f[v][3] * k) << 16);
-    q.y = bs_cvt_e4m3x2(f[v][4] * k, f[v][5] * k) | ((uint32_t)bs_cvt_e4m3x2(f[v][6] * k, f[v][7] * k) << 16);
+    q.x = bs_cvt_e4m3x2(g[0], g[1]) | ((uint32_t)bs_cvt_e4m3x2(g[2], g[3]) << 16);
+    q.y = bs_cvt_e4m3x2(g[4], g[5]) | ((uint32_t)bs_cvt_e4m3x2(g[6], g[7]) << 16);
     if ((int)(v * blockDim.x + threadIdx.x) < nvec) *reinterpret_cast<uint2*>(y + v * blockDim.x * 8) = q;
   }
 }
@@ -220,20 +233,29 @@ __global__ void __launch_bounds__(kMaxThreads) rms_rows_kernel(const Args a) {
   pdl_launch_dependents();
   double sum = 0.0;
 #pragma unroll
-  for (int v = 0; v < V; ++v) sum += (double)squares(f[v]);
+  for (int v = 0; v < V; ++v) {
+    if constexpr (V == 1) {          // few rows: every square exactly
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum = fma((double)f[v][i], (double)f[v][i], sum);
+    } else {
+      sum += (double)squares(f[v]);
+    }
+  }
   const float2 r = inv_sqrt(fma(row_sum(sum, part), a.inv_h, (double)a.eps));
   const T* w = reinterpret_cast<const T*>(a.w);
+  float m[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     const int c = v * blockDim.x + threadIdx.x;
+    m[v] = 0.0f;
     if (c < nvec) {
       float g[8];
       load8<T>(w + c * 8, g);
-      scale_row<T>(f[v], g, r);
+      m[v] = scale_row<T>(f[v], g, r);
       if (MODE == kOut) store8<T>(reinterpret_cast<T*>(a.y) + row * a.H + c * 8, f[v]);
     }
   }
-  if (MODE == kCodes) put_codes<V>(a, row, nvec, f);
+  if (MODE == kCodes) put_codes<V>(a, row, nvec, f, m, sizeof(T) == 4 ? make_float2(1.0f, 0.0f) : r);
 }
 
 constexpr int kMaxStages = 8;
@@ -312,15 +334,16 @@ __global__ void __launch_bounds__(kMaxThreads) rms_ring_kernel(const Args a, int
     const float2 r = inv_sqrt(fma(row_sum(sum, t.part[n & 1]), a.inv_h, (double)a.eps));
     if (t.abort) break;                  // uniform: set before the barrier or seen by the next one's wait
     if (threadIdx.x == 0 && row + stages * step < a.rows) issue(row + stages * step, s);
+    float m[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const int c = v * blockDim.x + threadIdx.x;
       float g[8];
       load8<T>(reinterpret_cast<const T*>(w[v]), g);
-      scale_row<T>(f[v], g, r);
+      m[v] = scale_row<T>(f[v], g, r);
       if (MODE == kOut && c < nvec) store8<T>(reinterpret_cast<T*>(a.y) + row * a.H + c * 8, f[v]);
     }
-    if (MODE == kCodes) put_codes<V>(a, row, nvec, f);
+    if (MODE == kCodes) put_codes<V>(a, row, nvec, f, m, sizeof(T) == 4 ? make_float2(1.0f, 0.0f) : r);
     if (++s == stages) {
       s = 0;
       phase ^= 1;
