@@ -143,12 +143,6 @@ __global__ void __launch_bounds__(512, 2) append_kernel(const Args a) {
     const int i = threadIdx.x + k * nthr;
     if (i < nvec) raw[k] = vec(i);
   }
-  if (id < 0 || id >= a.n_pages) {
-    if (threadIdx.x == 0) bs_set_error(BS_ERR_BAD_INDEX);
-    return;
-  }
-  const int64_t sat = (int64_t)id * a.Hkv + h;
-  const float old = a.scale[w][sat];
   uint32_t top = 0;
 #pragma unroll
   for (int k = 0; k < kU; ++k)
@@ -163,7 +157,7 @@ __global__ void __launch_bounds__(512, 2) append_kernel(const Args a) {
     for (int k = 0; k < (nthr >> 5); ++k) x = nan_max(x, red[k]);
     return x;
   };
-  float amax = over_cta(top_value<T>(top));   // its barrier: every thread has read the old scale
+  float amax = over_cta(top_value<T>(top));
   const bool odd = !(amax < __uint_as_float(0x7F800000u));
   if (odd) {                                  // the same for the whole CTA
     amax = 0.0f;
@@ -174,10 +168,17 @@ __global__ void __launch_bounds__(512, 2) append_kernel(const Args a) {
     __syncthreads();
     amax = over_cta(amax);
   }
+  if (id < 0 || id >= a.n_pages) {            // looked at this late, its load is behind the rows'
+    if (threadIdx.x == 0) bs_set_error(BS_ERR_BAD_INDEX);
+    return;
+  }
+  const int64_t sat = (int64_t)id * a.Hkv + h;
   float s = pow2_scale(amax);
   uint8_t* dst = a.cache[w] + sat * ((int64_t)a.D << a.page_log2);
   if (before > 0) {
+    const float old = a.scale[w][sat];
     s = fmaxf(s, old);
+    __syncthreads();                          // every thread has read the old scale
     if (s > old) {
       const float f = __fdiv_rn(old, s);
       const int n16 = before * a.D / 16;

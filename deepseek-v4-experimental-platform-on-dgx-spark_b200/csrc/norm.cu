@@ -271,7 +271,7 @@ struct RingTail {
 };
 
 template <typename T, int MODE, bool RES, int V>
-__global__ void __launch_bounds__(kMaxThreads) rms_ring_kernel(const Args a, int stages) {
+__global__ void __maxnreg__(96) rms_ring_kernel(const Args a, int stages) {
   extern __shared__ __align__(128) uint8_t smem[];
   const int nvec = a.H >> 3;
   const uint32_t row_bytes = (uint32_t)a.H * sizeof(T);

@@ -45,7 +45,10 @@ struct Args {
 template <typename T, bool HALF, int U>
 __global__ void __launch_bounds__(kThreads) rope_kernel(const Args a) {
   constexpr int E = 16 / (int)sizeof(T);               // elements per vector
-  __shared__ float2 cs[kCs];
+  constexpr int PV = HALF ? E : E / 2;                 // pairs of a task
+  // Two pairs (cos, sin, cos, sin) in 16 bytes, a task's PV / 2 of them nrot apart: lanes next to each other read next
+  // to each other.
+  __shared__ float4 cs[kCs / 2];
   pdl_wait();
   const int64_t tok0 = (int64_t)blockIdx.x * a.tokens_per_cta;
   const int nt = (int)min((int64_t)a.tokens_per_cta, a.tokens - tok0);
@@ -61,7 +64,7 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const Args a) {
   for (int base = 0; base < tasks; base += kThreads * U) {
     uint4 lo[U], hi[HALF ? U : 1];
     int64_t to[U];
-    int at[U];                       // first cos/sin pair, or -1: copy
+    int at[U];                       // first cos/sin pairs, or -1: copy
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int task = base + u * kThreads + threadIdx.x;
@@ -74,7 +77,7 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const Args a) {
         int d;
         if (k < nrot) {
           d = a.offset + k * E;
-          at[u] = t * np + (HALF ? k * E : k * E / 2);
+          at[u] = t * (np / 2) + k;
         } else {
           const int e = (k - nrot) * E;
           d = e < a.offset ? e : e + a.n;
@@ -98,7 +101,9 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const Args a) {
         const long long v = (long long)((unsigned long long)p * f);
         float s, c;
         sincospif((float)v * 1.0842021724855044e-19f, &s, &c);               // 2^-63: fraction of a turn x 2
-        cs[j] = make_float2(c * a.scale, (a.inverse ? -s : s) * a.scale);
+        const int k = i / PV, in = i - k * PV;
+        reinterpret_cast<float2*>(cs)[(t * (np / 2) + (in / 2) * nrot + k) * 2 + (in & 1)] =
+            make_float2(c * a.scale, (a.inverse ? -s : s) * a.scale);
       }
       __syncthreads();
     }
@@ -114,20 +119,24 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const Args a) {
             float g[E], p[E], q[E];
             unpack<T>(hi[u], g);
 #pragma unroll
-            for (int i = 0; i < E; ++i) {
-              const float2 t = cs[at[u] + i];
+            for (int i = 0; i < E; i += 2) {
+              const float4 t = cs[at[u] + (i / 2) * nrot];
               p[i] = f[i] * t.x - g[i] * t.y;
               q[i] = f[i] * t.y + g[i] * t.x;
+              p[i + 1] = f[i + 1] * t.z - g[i + 1] * t.w;
+              q[i + 1] = f[i + 1] * t.w + g[i + 1] * t.z;
             }
             *reinterpret_cast<uint4*>(o + np) = pack<T>(q);
             lo[u] = pack<T>(p);
           } else {
             float p[E];
 #pragma unroll
-            for (int i = 0; i < E; i += 2) {
-              const float2 t = cs[at[u] + (i >> 1)];
+            for (int i = 0; i < E; i += 4) {
+              const float4 t = cs[at[u] + (i / 4) * nrot];
               p[i] = f[i] * t.x - f[i + 1] * t.y;
               p[i + 1] = f[i] * t.y + f[i + 1] * t.x;
+              p[i + 2] = f[i + 2] * t.z - f[i + 3] * t.w;
+              p[i + 3] = f[i + 2] * t.w + f[i + 3] * t.z;
             }
             lo[u] = pack<T>(p);
           }
@@ -145,9 +154,12 @@ cudaError_t bs_launch_rope(rope::Args a, int dtype, int half, cudaStream_t st) {
   if (a.tokens == 0) return cudaSuccess;
   const int esz = dtype == BS_DT_F32 ? 4 : 2, E = 16 / esz;
   const int per_head = (half ? a.n / (2 * E) : a.n / E) + (a.copy ? (a.D - a.n) / E : 0);
-  // About 24 KB of loads per CTA, of as many whole tokens as that is (their cos/sin pairs have to fit), or of part of a
-  // token's heads; fewer when the CTAs would not fill the GPU twice.
-  const int want = half ? 768 : 1536;
+  // Tasks of a CTA: two per thread in the half layout (two vectors each), one in the interleaved one, of as many whole
+  // tokens as that is (their cos/sin pairs have to fit) or of part of a token's heads; fewer when the CTAs would not
+  // fill the GPU a few times.  More per thread costs registers, and with them loads in flight: 8192 tokens x 40 heads x
+  // 128 bf16 take 30 us half (1: 41, 3: 42) and 43 us interleaved (2: 52, 4: 63); 64 tokens x 64 heads x 512 with 64
+  // dims turned 2.9 us (2: 3.4, 4: 4.7).
+  const int want = half ? 2 * rope::kThreads : rope::kThreads;
   const int64_t per_token = (int64_t)per_head * a.H;
   int64_t tpc = want / per_token, hpc = a.H;
   tpc = tpc < rope::kCs / (a.n / 2) ? tpc : rope::kCs / (a.n / 2);
@@ -174,8 +186,8 @@ cudaError_t bs_launch_rope(rope::Args a, int dtype, int half, cudaStream_t st) {
   cfg.numAttrs = 1;
   auto go = [&](auto t) {
     using T = decltype(t);
-    return half ? cudaLaunchKernelEx(&cfg, rope::rope_kernel<T, true, 3>, a)
-                : cudaLaunchKernelEx(&cfg, rope::rope_kernel<T, false, 6>, a);
+    return half ? cudaLaunchKernelEx(&cfg, rope::rope_kernel<T, true, 2>, a)
+                : cudaLaunchKernelEx(&cfg, rope::rope_kernel<T, false, 1>, a);
   };
   if (dtype == BS_DT_BF16) return go(__nv_bfloat16());
   if (dtype == BS_DT_F16) return go(__half());
