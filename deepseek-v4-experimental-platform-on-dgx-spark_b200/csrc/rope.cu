@@ -13,7 +13,8 @@
 // and only that fraction, in [-1/2, 1/2) turns, is rounded to fp32 for
 // sincospif.  What is left of the error is freq's own 2^-53.
 //
-// HBM-bound: a CTA takes a few tokens (or, when there are few, a range of one
+// HBM-bound (8192 tokens x 40 heads x 128 bf16: 30 us, 0.85 of the copy
+// bandwidth): a CTA takes a few tokens (or, when there are few, a range of one
 // token's heads), loads its 16-byte vectors first, computes the tokens' cos/sin
 // pairs into shared memory while they are in flight, rotates and stores.
 #include "common.cuh"
