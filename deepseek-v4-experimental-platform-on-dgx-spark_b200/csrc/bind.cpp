@@ -7,6 +7,7 @@
 // the C entry points (include/bsgemm.h) do the work and check what they are
 // given again.  Their addresses come from the library that _lib.py loaded, so
 // there is one copy of it.
+#include <ATen/MemoryOverlap.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -98,6 +99,13 @@ at::Tensor empty(const at::Tensor& like, at::IntArrayRef shape, at::ScalarType d
   return at::empty(shape, like.options().dtype(dtype).memory_format(at::MemoryFormat::Contiguous));
 }
 
+bool misaligned(const at::Tensor& t, uintptr_t a) { return reinterpret_cast<uintptr_t>(t.const_data_ptr()) % a != 0; }
+
+// t, or a copy where it is not contiguous or does not start on 16 bytes.
+at::Tensor dense(const at::Tensor& t) {
+  return t.is_contiguous() && !misaligned(t, 16) ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
 // Status and outputs; the caller turns a status into its exception.
 py::tuple rms(const at::Tensor& x, const at::Tensor& weight, double eps, const Opt& residual, bool codes, bool pow2, bool e8m0) {
   const On on(x, weight, residual);
@@ -109,15 +117,14 @@ py::tuple rms(const at::Tensor& x, const at::Tensor& weight, double eps, const O
     bad_value("rms_norm: weight ", weight.sizes(), " does not match x ", x.sizes());
   if (residual && residual->sizes() != x.sizes()) bad_value("rms_norm: residual ", residual->sizes(), " does not match x ", x.sizes());
   const int64_t H = x.size(-1);
-  const auto xc = x.expect_contiguous(), wc = weight.expect_contiguous();
-  const at::Tensor rc = residual ? residual->contiguous() : at::Tensor();
+  const at::Tensor xc = dense(x), wc = dense(weight), rc = residual ? dense(*residual) : at::Tensor();
   at::Tensor h = residual ? empty(x, x.sizes(), dt) : at::Tensor();
   const int64_t rows = H ? x.numel() / H : 0;
   const void* r = residual ? rc.const_data_ptr() : nullptr;
   void* hp = residual ? h.mutable_data_ptr() : nullptr;
   if (!codes) {
     at::Tensor y = empty(x, x.sizes(), dt);
-    const int st = p_rms_norm(xc->const_data_ptr(), r, wc->const_data_ptr(), tag(dt), rows, H, (float)eps, hp,
+    const int st = p_rms_norm(xc.const_data_ptr(), r, wc.const_data_ptr(), tag(dt), rows, H, (float)eps, hp,
                               y.mutable_data_ptr(), on.stream);
     return residual ? py::make_tuple(st, y, h) : py::make_tuple(st, y);
   }
@@ -125,12 +132,10 @@ py::tuple rms(const at::Tensor& x, const at::Tensor& weight, double eps, const O
   c10::SmallVector<int64_t, 8> shape(x.sizes().begin(), x.sizes().end());
   shape.back() = H / 128;
   at::Tensor s = empty(x, shape, e8m0 ? at::ScalarType::Float8_e8m0fnu : at::kFloat);
-  const int st = p_rms_norm_quant(xc->const_data_ptr(), r, wc->const_data_ptr(), tag(dt), rows, H, (float)eps, pow2, hp,
+  const int st = p_rms_norm_quant(xc.const_data_ptr(), r, wc.const_data_ptr(), tag(dt), rows, H, (float)eps, pow2, hp,
                                   y.mutable_data_ptr(), s.mutable_data_ptr(), e8m0 ? BS_DT_E8M0 : BS_DT_F32, on.stream);
   return residual ? py::make_tuple(st, y, s, h) : py::make_tuple(st, y, s);
 }
-
-bool misaligned(const at::Tensor& t, uintptr_t a) { return reinterpret_cast<uintptr_t>(t.const_data_ptr()) % a != 0; }
 
 // The stride of dims 0..-3 taken as one, or -1 where they are not one.
 int64_t token_stride(const at::Tensor& x) {
@@ -155,6 +160,7 @@ py::tuple rope(const at::Tensor& x, const at::Tensor& positions, const at::Tenso
     bad_value("rope: positions ", positions.sizes(), " do not match x ", x.sizes());
   const int64_t H = x.size(-2), D = x.size(-1);
   if (H > INT_MAX || D > INT_MAX) bad_value("rope: x ", x.sizes());
+  if (inplace && at::has_internal_overlap(x) == at::MemOverlap::Yes) bad_value("rope: an in-place x overlaps itself");
   at::Tensor xt = x;
   int64_t tok = H * D, head = D;
   if (!x.is_contiguous() || misaligned(x, 16)) {

@@ -859,6 +859,7 @@ int bs_cache_attn(const void* q, int dtype, int64_t B, int64_t S, int H, int Hkv
   if (st) return st;
   st = cache_check("cache_attn", B, S, Hkv, D, page, n_pages, max_pages);
   if (st) return st;
+  if (!(softmax_scale - softmax_scale == 0.0f)) return fail(BS_ERR_INVALID_ARG, "cache_attn: softmax_scale is not finite");
   if (B == 0) return BS_OK;
   if (!q || !q_strides || !k_cache || !k_scale || !block_table || !seq_lens || !out || (!v_cache != !v_scale))
     return fail(BS_ERR_INVALID_ARG, "cache_attn: null pointer");

@@ -129,9 +129,12 @@ struct Walk {
     if (++h == a.Hkv) {
       h = 0;
       do {
-        ++unit;
+        if (++unit >= a.B * a.RT) {   // left > 0 means a later unit has tiles, unless the lengths changed under the call
+          left = 0;
+          return;
+        }
         enter(a, R);
-      } while (nt == 0);            // left > 0: a later unit has tiles
+      } while (nt == 0);
     }
   }
 };
@@ -341,17 +344,11 @@ BS_DEVINL void tmem_ld16x256(uint32_t taddr, uint32_t* v) {
     asm volatile("tcgen05.ld.sync.aligned.16x256b.x1.b32 {%0,%1,%2,%3}, [%4];"
                  : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
                  : "r"(taddr));
-  } else if constexpr (K == 2) {
+  } else {
+    static_assert(K == 2, "16x256b.x2");
     asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                  : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
                  : "r"(taddr));
-  } else {
-    static_assert(K == 4, "16x256b.x4");
-    asm volatile(
-        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
-          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-        : "r"(taddr));
   }
 }
 

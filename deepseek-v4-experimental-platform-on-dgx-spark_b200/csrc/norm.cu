@@ -375,7 +375,7 @@ cudaError_t launch_v(const Args& a, int threads, cudaStream_t st) {
   cfg.numAttrs = 1;
   // The ring where three rows fit each CTA's buffers and each CTA gets kRingRows rows at least (its start is a serial
   // load).
-  {
+  if constexpr (V > 1) {             // one vector a thread is for few rows
     auto kern = rms_ring_kernel<T, MODE, RES, V>;
     static int regs_of[hostcache::kMaxDevices];
     const int regs = hostcache::get(regs_of, [&] {

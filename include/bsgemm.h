@@ -409,7 +409,8 @@ int bs_cache_append(const void* k, const void* v, int dtype, int64_t B, int64_t 
  * seq_lens int32 [B] counts all cached tokens, the S (or new_lens[b]) newest
  * included; query token i sees the first seq_lens[b] - new_lens[b] + i + 1.
  * Query heads h*H/Hkv .. share kv head h.  v_cache NULL: the values are the
- * keys.  Any finite or NaN scales are taken (fp32 [n_pages, Hkv]).
+ * keys.  Any finite or NaN page scales are taken (fp32 [n_pages, Hkv]);
+ * softmax_scale has to be finite.
  * attn_sink fp32 [H] or NULL: a logit per head that takes softmax weight and
  * adds no value.  A row that sees nothing is zero, padded query tokens too.
  * Softmax statistics and sums in fp32; weights and queries enter the tensor

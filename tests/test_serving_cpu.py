@@ -92,9 +92,9 @@ def test_append_refusals(lib):
 
 
 def attn(lib, dtype=1, B=1, S=1, H=8, Hkv=1, D=128, page=64, n_pages=4, max_pages=4, q=FAKE, v=None, v_scale=None,
-         strides=(1024, 1024, 128), ws=FAKE, ws_bytes=1 << 40):
+         strides=(1024, 1024, 128), ws=FAKE, ws_bytes=1 << 40, scale=0.1):
     return lib.bs_cache_attn(q, dtype, B, S, H, Hkv, D, S3(*strides), FAKE, v, FAKE, v_scale, n_pages, page, FAKE, max_pages, FAKE,
-                             None, None, 0.1, FAKE, ws, ws_bytes, None)
+                             None, None, scale, FAKE, ws, ws_bytes, None)
 
 
 def test_attn_refusals(lib):
@@ -111,6 +111,7 @@ def test_attn_refusals(lib):
     assert attn(lib, ws_bytes=64) == L.BS_ERR_INVALID_ARG and b"needed" in lib.bs_last_error()
     assert attn(lib, ws=None) == L.BS_ERR_INVALID_ARG
     assert attn(lib, q=None) == L.BS_ERR_INVALID_ARG
+    assert attn(lib, scale=float("inf")) == L.BS_ERR_INVALID_ARG and attn(lib, scale=float("nan")) == L.BS_ERR_INVALID_ARG
     assert attn(lib, B=2 ** 31) == L.BS_ERR_UNSUPPORTED
     assert attn(lib, B=2 ** 20, H=8 * 2 ** 12, Hkv=2 ** 12, max_pages=2 ** 20) == L.BS_ERR_UNSUPPORTED   # over 2^31 tiles
     assert attn(lib, B=0, q=None) == L.BS_OK

@@ -124,6 +124,25 @@ def test_rms_norm_empty_and_strided(pkg):
     assert ((pkg.rms_norm(x, w).double() - want).abs() <= want.abs() * (2.0 ** -11 + 2.0 ** -18) + 2.0 ** -25).all()
 
 
+def test_rms_norm_unaligned_and_in_place(pkg):
+    """Inputs that start off a 16-byte boundary are copied; the C entry point may write h over x or the residual."""
+    g = gen(9)
+    flat = randn(g, 4 * 256 + 3, dtype=torch.bfloat16)
+    x, w = flat[3:].view(4, 256), torch.ones(257, dtype=torch.bfloat16, device="cuda")[1:]
+    assert torch.equal(pkg.rms_norm(x, w, residual=x)[0], pkg.rms_norm(x.clone(), w.clone(), residual=x.clone())[0])
+    L, st = pkg._lib, torch.cuda.current_stream().cuda_stream
+    for rows in (5, 3000):                       # both forms of the kernel
+        x, r = randn(g, rows, 1024, dtype=torch.bfloat16), randn(g, rows, 1024, dtype=torch.bfloat16)
+        w = torch.ones(1024, dtype=torch.bfloat16, device="cuda")
+        y, h = pkg.rms_norm(x, w, residual=r)
+        for into in (0, 1):
+            a, b = x.clone(), r.clone()
+            got = torch.empty_like(y)
+            L.check(L.load().bs_rms_norm(a.data_ptr(), b.data_ptr(), w.data_ptr(), L.DT_BF16, rows, 1024, 1e-6,
+                                         (b if into else a).data_ptr(), got.data_ptr(), st))
+            assert torch.equal(got, y) and torch.equal(b if into else a, h)
+
+
 # ------------------------------------------------------------------ rope
 
 @pytest.mark.parametrize("shape,n,offset,layout,dt", [
@@ -538,6 +557,8 @@ def test_refusals(pkg):
             (ValueError, lambda: pkg.rope(q, pos[0], f)), (ValueError, lambda: pkg.rope(q, pos, f, offset=8)),
             (NotImplementedError, lambda: pkg.rope(q, pos, f[:5])),
             (ValueError, lambda: pkg.rope(q.transpose(2, 3), pos, f, inplace=True)),
+            (ValueError, lambda: pkg.rope(q.expand(1, 3, 4, 64), pos.expand(1, 3), f, inplace=True)),
+            (ValueError, lambda: pkg.cache_attn(q, k, v, ks, vs, table, sl, float("nan"))),
             (TypeError, lambda: pkg.cache_attn(q.float(), k, v, ks, vs, table, sl, 1.0)),
             (TypeError, lambda: pkg.cache_attn(q, k, v, ks, vs, table.long(), sl, 1.0)),
             (TypeError, lambda: pkg.cache_attn(q, k.view(torch.uint8), v, ks, vs, table, sl, 1.0)),
