@@ -377,13 +377,22 @@ BS_DEVINL void load_rows(uint32_t taddr, float* s) {
     }
     tmem_ld_wait();
 #pragma unroll
-    for (int r = 0; r < B; ++r) {
-      float x = __uint_as_float(v[PP - 1][r]);
+    for (int r = 0; r < B; r += 2) {
+      float2 x = make_float2(__uint_as_float(v[PP - 1][r]), __uint_as_float(v[PP - 1][r + 1]));
 #pragma unroll
-      for (int p = PP - 2; p >= 0; --p) x = fmaf(x, 0.0625f, __uint_as_float(v[p][r]));
-      s[r] = x;
+      for (int p = PP - 2; p >= 0; --p)
+        x = fma2(x, both(0.0625f), make_float2(__uint_as_float(v[p][r]), __uint_as_float(v[p][r + 1])));
+      s[r] = x.x;
+      s[r + 1] = x.y;
     }
   }
+}
+
+// Row of column r of P and O.  From 16 rows on, the columns of 16 rows are in the order in which the softmax threads hold
+// them: rows 2i, 2i + 1, 2i + 8, 2i + 9 of thread i of 4 lie side by side, one 4-byte store.
+template <int R>
+__host__ __device__ constexpr int row_of(int r) {
+  return R < 16 ? r : (r & ~15) + 8 * ((r >> 1) & 1) + 2 * ((r >> 2) & 3) + (r & 1);
 }
 
 // e4m3 NaN (0x7F or 0xFF) among four codes: bytes whose low seven bits are all set.
@@ -871,15 +880,21 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
         const int tok = tok0 + 8 * k;
         const float2 ratio = both(in.vr[tok >> a.page_log2]);
         uint8_t* p = pbuf + pb * C::kPBytes + tok * 16;
+        uint16_t c[K][PP];
 #pragma unroll
         for (int g = 0; g < K; ++g) {
-          uint16_t c[PP];
           const float2 w = mul2(s[g][k], ratio);
-          split2p<PP>(w.x, w.y, c);
+          split2p<PP>(w.x, w.y, c[g]);
+        }
 #pragma unroll
-          for (int t = 0; t < PP; ++t) {
-            const int n = t * R + row0 + 8 * g;
-            *reinterpret_cast<uint16_t*>(p + (n >> 4) * 2048 + (n & 15)) = c[t];
+        for (int t = 0; t < PP; ++t) {
+          if constexpr (K == 1) {
+            const int n = t * R + row0;
+            *reinterpret_cast<uint16_t*>(p + (n >> 4) * 2048 + (n & 15)) = c[0][t];
+          } else {
+            // the thread's four rows next to each other (row_of)
+            *reinterpret_cast<uint32_t*>(p + (t * (R / 16) + wg) * 2048 + 4 * (lane & 3)) =
+                (uint32_t)c[0][t] | ((uint32_t)c[1][t] << 16);
           }
         }
       }
@@ -1046,7 +1061,7 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
             load_rows<R, PP, B>(tmem + lane_base + C::SB * N + (ob * NC + c) * N + b, o);
 #pragma unroll
             for (int r = 0; r < B; r += 2) {
-              const float2 x = fma2(make_float2(acc[c][b + r], acc[c][b + r + 1]), *reinterpret_cast<const float2*>(al + b + r),
+              const float2 x = fma2(make_float2(acc[c][b + r], acc[c][b + r + 1]), *reinterpret_cast<const float2*>(al + row_of<R>(b + r)),
                                     mul2(make_float2(o[r], o[r + 1]), both(unit)));
               acc[c][b + r] = x.x;
               acc[c][b + r + 1] = x.y;
@@ -1090,7 +1105,7 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
           const int first_nan = T.nanmin[sr][c * 128 + quad * 32 + lane];
 #pragma unroll
           for (int r = 0; r < R; ++r)
-            if (first_nan < T.lim[buf][r]) acc[c][r] = __uint_as_float(0x7FC00000u);
+            if (first_nan < T.lim[buf][row_of<R>(r)]) acc[c][r] = __uint_as_float(0x7FC00000u);
           T.nanmin[sr][c * 128 + quad * 32 + lane] = 0x7FFFFFFF;
         }
       }
@@ -1102,8 +1117,8 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
         uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + d0;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-          const int64_t at = lds_s64(off + 8 * r);
-          const float f = lds_f32(fin + 4 * r);
+          const int64_t at = lds_s64(off + 8 * row_of<R>(r));
+          const float f = lds_f32(fin + 4 * row_of<R>(r));
           if (at < 0) continue;
 #pragma unroll
           for (int c = 0; c < NC; ++c) {
@@ -1118,7 +1133,7 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
 #pragma unroll
         for (int r = 0; r < R; ++r)
 #pragma unroll
-          for (int c = 0; c < NC; ++c) po[r * (NC * 128) + c * 128] = acc[c][r];
+          for (int c = 0; c < NC; ++c) po[row_of<R>(r) * (NC * 128) + c * 128] = acc[c][r];
       }
     }
   }

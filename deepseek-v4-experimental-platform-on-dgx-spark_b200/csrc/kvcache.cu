@@ -13,19 +13,20 @@
 // before does not count), and slots behind the new tokens are left alone.
 // Infinities and NaN are stored as NaN and take no part in the scale.
 //
-// One CTA per (sequence, page it touches, head, key or value): it owns that
+// One CTA per (sequence, page it touches, head), for its keys and values: it owns that
 // page and head, so there are no atomics and the result does not depend on any
 // order.  Its new rows are read once into registers, the loads going out
 // before the page's index and old scale are known; rows that do not fit there
 // (long pages of wide heads) are read twice, the second time out of L2.
-// 4 x 4001 tokens x 8 heads x 128 bf16 take 24 us (0.61 of the copy bandwidth:
+// 4 x 4001 tokens x 8 heads x 128 bf16 take 22 us (0.68 of the copy bandwidth;
+// keys and values in CTAs of their own 24, with 8 vectors a thread 27 to 31):
 // a CTA is a chain of dependent loads, its start, its rows and page index, with
-// 128 KB of rows in flight per SM); one token for each of 128 sequences 4.7 us.
+// 128 KB of rows in flight per SM.  One token for each of 128 sequences: 3.9 us.
 #include "common.cuh"
 
 namespace kvc {
 
-constexpr int kU = 8;             // 16-byte vectors of new rows in registers
+constexpr int kU = 4;             // 16-byte vectors of new rows in registers, for keys and for values
 
 struct Args {
   const void* src[2];           // k, v: [B, S, Hkv, D], last dim contiguous
@@ -106,18 +107,18 @@ BS_DEVINL float finite_top(const uint4& raw, float amax) {
   return amax;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(512, 2) append_kernel(const Args a) {
+// W = 2: keys and values, whose loads go out together.
+template <typename T, int W>
+__global__ void __maxnreg__(64) append_kernel(const Args a) {
   constexpr int E = 16 / (int)sizeof(T);
-  __shared__ float red[16];
+  __shared__ float red[W][16];
   pdl_wait();
-  const int nthr = blockDim.x;
+  const int nthr = blockDim.x, warps = nthr >> 5;
   unsigned u = blockIdx.x;
   const int h = (int)(u % (unsigned)a.Hkv);
   u /= (unsigned)a.Hkv;
   const int j = (int)(u % (unsigned)a.span);
   const int b = (int)(u / (unsigned)a.span);
-  const int w = blockIdx.y;
   const int page = 1 << a.page_log2;
   const int start = a.start[b];
   const int nl = a.new_lens ? a.new_lens[b] : a.S;
@@ -132,83 +133,112 @@ __global__ void __launch_bounds__(512, 2) append_kernel(const Args a) {
   const int id = pg < a.max_pages ? a.table[(int64_t)b * a.max_pages + pg] : -1;
   const int m = (int)(hi - lo), before = (int)(lo - first);
   const int vrow = (int)a.vrow.d, nvec = m * vrow;   // 16-byte vectors
-  const T* src = reinterpret_cast<const T*>(a.src[w]) + b * a.sb[w] + (lo - start) * a.ss[w] + h * a.sh[w];
-  const int64_t ss = a.ss[w];
-  auto vec = [&](int i) {
+  const T* src[W];
+#pragma unroll
+  for (int w = 0; w < W; ++w)
+    src[w] = reinterpret_cast<const T*>(a.src[w]) + b * a.sb[w] + (lo - start) * a.ss[w] + h * a.sh[w];
+  auto vec = [&](int w, int i) {
     const int r = (int)bs_div(i, a.vrow);
-    return *reinterpret_cast<const uint4*>(src + r * ss + (i - r * vrow) * E);
+    return *reinterpret_cast<const uint4*>(src[w] + r * a.ss[w] + (i - r * vrow) * E);
   };
   // a thread's vectors are threadIdx.x + k nthr; the first kU stay in registers
-  uint4 raw[kU];
+  uint4 raw[W][kU];
 #pragma unroll
-  for (int k = 0; k < kU; ++k) {
-    const int i = threadIdx.x + k * nthr;
-    if (i < nvec) raw[k] = vec(i);
-  }
-  uint32_t top = 0;
+  for (int w = 0; w < W; ++w)
 #pragma unroll
-  for (int k = 0; k < kU; ++k)
-    if ((int)threadIdx.x + k * nthr < nvec) top = top_of<T>(raw[k], top);
-#pragma unroll 4
-  for (int i = threadIdx.x + kU * nthr; i < nvec; i += nthr) top = top_of<T>(vec(i), top);
-  auto over_cta = [&](float x) {
+    for (int k = 0; k < kU; ++k) {
+      const int i = threadIdx.x + k * nthr;
+      if (i < nvec) raw[w][k] = vec(w, i);
+    }
+  float amax[W];
+  auto over_cta = [&]() {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) x = nan_max(x, __shfl_xor_sync(0xffffffffu, x, o));
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = x;
+    for (int w = 0; w < W; ++w) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) amax[w] = nan_max(amax[w], __shfl_xor_sync(0xffffffffu, amax[w], o));
+      if ((threadIdx.x & 31) == 0) red[w][threadIdx.x >> 5] = amax[w];
+    }
     __syncthreads();
-    for (int k = 0; k < (nthr >> 5); ++k) x = nan_max(x, red[k]);
-    return x;
+#pragma unroll
+    for (int w = 0; w < W; ++w)
+      for (int k = 0; k < warps; ++k) amax[w] = nan_max(amax[w], red[w][k]);
   };
-  float amax = over_cta(top_value<T>(top));
-  const bool odd = !(amax < __uint_as_float(0x7F800000u));
-  if (odd) {                                  // the same for the whole CTA
-    amax = 0.0f;
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    uint32_t top = 0;
 #pragma unroll
     for (int k = 0; k < kU; ++k)
-      if ((int)threadIdx.x + k * nthr < nvec) amax = finite_top<T>(raw[k], amax);
-    for (int i = threadIdx.x + kU * nthr; i < nvec; i += nthr) amax = finite_top<T>(vec(i), amax);
+      if ((int)threadIdx.x + k * nthr < nvec) top = top_of<T>(raw[w][k], top);
+#pragma unroll 4
+    for (int i = threadIdx.x + kU * nthr; i < nvec; i += nthr) top = top_of<T>(vec(w, i), top);
+    amax[w] = top_value<T>(top);
+  }
+  over_cta();
+  bool odd = false;
+#pragma unroll
+  for (int w = 0; w < W; ++w) odd |= !(amax[w] < __uint_as_float(0x7F800000u));
+  if (odd) {                                  // infinities or NaN: the same for the whole CTA
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      amax[w] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < kU; ++k)
+        if ((int)threadIdx.x + k * nthr < nvec) amax[w] = finite_top<T>(raw[w][k], amax[w]);
+      for (int i = threadIdx.x + kU * nthr; i < nvec; i += nthr) amax[w] = finite_top<T>(vec(w, i), amax[w]);
+    }
     __syncthreads();
-    amax = over_cta(amax);
+    over_cta();
   }
   if (id < 0 || id >= a.n_pages) {            // looked at this late, its load is behind the rows'
     if (threadIdx.x == 0) bs_set_error(BS_ERR_BAD_INDEX);
     return;
   }
   const int64_t sat = (int64_t)id * a.Hkv + h;
-  float s = pow2_scale(amax);
-  uint8_t* dst = a.cache[w] + sat * ((int64_t)a.D << a.page_log2);
-  if (before > 0) {
-    const float old = a.scale[w][sat];
-    s = fmaxf(s, old);
-    __syncthreads();                          // every thread has read the old scale
-    if (s > old) {
-      const float f = __fdiv_rn(old, s);
-      const int n16 = before * a.D / 16;
-#pragma unroll 4
-      for (int i = threadIdx.x; i < n16; i += nthr) {
-        uint4 c = reinterpret_cast<uint4*>(dst)[i];
-        uint32_t* p = reinterpret_cast<uint32_t*>(&c);
+  float s[W];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint32_t v = p[k];
-          p[k] = bs_cvt_e4m3x2(bs_e4m3_to_f32(v & 0xFF) * f, bs_e4m3_to_f32((v >> 8) & 0xFF) * f) |
-                 ((uint32_t)bs_cvt_e4m3x2(bs_e4m3_to_f32((v >> 16) & 0xFF) * f, bs_e4m3_to_f32(v >> 24) * f) << 16);
+  for (int w = 0; w < W; ++w) s[w] = pow2_scale(amax[w]);
+  if (before > 0) {
+    float old[W];
+#pragma unroll
+    for (int w = 0; w < W; ++w) old[w] = a.scale[w][sat];
+    __syncthreads();                          // every thread has read the old scales
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      s[w] = fmaxf(s[w], old[w]);
+      if (s[w] > old[w]) {
+        const float f = __fdiv_rn(old[w], s[w]);
+        const int n16 = before * a.D / 16;
+        uint4* dst = reinterpret_cast<uint4*>(a.cache[w] + sat * ((int64_t)a.D << a.page_log2));
+#pragma unroll 4
+        for (int i = threadIdx.x; i < n16; i += nthr) {
+          uint4 c = dst[i];
+          uint32_t* p = reinterpret_cast<uint32_t*>(&c);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t v = p[k];
+            p[k] = bs_cvt_e4m3x2(bs_e4m3_to_f32(v & 0xFF) * f, bs_e4m3_to_f32((v >> 8) & 0xFF) * f) |
+                   ((uint32_t)bs_cvt_e4m3x2(bs_e4m3_to_f32((v >> 16) & 0xFF) * f, bs_e4m3_to_f32(v >> 24) * f) << 16);
+          }
+          dst[i] = c;
         }
-        reinterpret_cast<uint4*>(dst)[i] = c;
       }
     }
   }
-  if (threadIdx.x == 0) a.scale[w][sat] = s;
-  dst += (int64_t)before * a.D;               // the new rows lie one behind the other there
-  const bool pow2 = (__float_as_uint(s) & 0x7FFFFFu) == 0 && s >= 1.1754944e-38f && s < 1.7e38f;
-  const float inv = pow2 ? bs_inv_pow2(s) : 0.0f;
 #pragma unroll
-  for (int k = 0; k < kU; ++k) {
-    const int i = threadIdx.x + k * nthr;
-    if (i < nvec) put_codes<T>(dst + i * E, raw[k], s, inv, pow2, odd);
-  }
+  for (int w = 0; w < W; ++w) {
+    if (threadIdx.x == 0) a.scale[w][sat] = s[w];
+    // the new rows lie one behind the other there
+    uint8_t* dst = a.cache[w] + sat * ((int64_t)a.D << a.page_log2) + (int64_t)before * a.D;
+    const bool pow2 = (__float_as_uint(s[w]) & 0x7FFFFFu) == 0 && s[w] >= 1.1754944e-38f && s[w] < 1.7e38f;
+    const float inv = pow2 ? bs_inv_pow2(s[w]) : 0.0f;
+#pragma unroll
+    for (int k = 0; k < kU; ++k) {
+      const int i = threadIdx.x + k * nthr;
+      if (i < nvec) put_codes<T>(dst + i * E, raw[w][k], s[w], inv, pow2, odd);
+    }
 #pragma unroll 4
-  for (int i = threadIdx.x + kU * nthr; i < nvec; i += nthr) put_codes<T>(dst + i * E, vec(i), s, inv, pow2, odd);
+    for (int i = threadIdx.x + kU * nthr; i < nvec; i += nthr) put_codes<T>(dst + i * E, vec(w, i), s[w], inv, pow2, odd);
+  }
   pdl_launch_dependents();
 }
 
@@ -222,7 +252,7 @@ cudaError_t bs_launch_cache_append(kvc::Args a, int dtype, int both, cudaStream_
   int threads = 32;
   while (threads < 512 && (int64_t)threads * kvc::kU < vecs) threads *= 2;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((int64_t)a.B * a.span * a.Hkv), both ? 2 : 1);
+  cfg.gridDim = dim3((unsigned)((int64_t)a.B * a.span * a.Hkv));
   cfg.blockDim = dim3(threads);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -230,7 +260,11 @@ cudaError_t bs_launch_cache_append(kvc::Args a, int dtype, int both, cudaStream_
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (dtype == BS_DT_BF16) return cudaLaunchKernelEx(&cfg, kvc::append_kernel<__nv_bfloat16>, a);
-  if (dtype == BS_DT_F16) return cudaLaunchKernelEx(&cfg, kvc::append_kernel<__half>, a);
-  return cudaLaunchKernelEx(&cfg, kvc::append_kernel<float>, a);
+  auto go = [&](auto t) {
+    using T = decltype(t);
+    return both ? cudaLaunchKernelEx(&cfg, kvc::append_kernel<T, 2>, a) : cudaLaunchKernelEx(&cfg, kvc::append_kernel<T, 1>, a);
+  };
+  if (dtype == BS_DT_BF16) return go(__nv_bfloat16());
+  if (dtype == BS_DT_F16) return go(__half());
+  return go(float());
 }
