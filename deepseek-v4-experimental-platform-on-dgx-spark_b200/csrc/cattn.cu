@@ -44,11 +44,10 @@
 // (48 sequences of up to 8192: 82 us, 314 TFLOP/s).
 //
 // Roles: one warpgroup with the TMA producer and an issuer for each of the two
-// products; one or (from
-// 32 rows on) two softmax warpgroups, each with its share of the rows; one
-// that stages Q and accumulates O, one head dim per thread and 128-dim chunk.
-// Shared memory: a ring of 16 KB chunks, Q (this segment's and, where it fits,
-// the next one's), two P buffers.
+// products; one softmax warpgroup, or from 32 rows on one for every 16 of them;
+// one that stages Q and accumulates O, one head dim per thread and 128-dim
+// chunk.  Shared memory: rings of 16 KB chunks, Q (this segment's and, where it
+// fits, the next one's), two P buffers.
 #include <type_traits>
 
 #include "common.cuh"
