@@ -141,7 +141,7 @@ struct Walk {
 struct Info {                       // one tile, from the producer
   float ks[8];                      // per page of the tile
   float vr[8];                      // 256 x value scale / unit
-  float unit;                       // largest |value scale|
+  float unit;                       // largest |value scale| that is a number
   int valid;                        // bits of the pages that are there
   int t0;                           // first token
   int limit;                        // tokens that any row sees
@@ -646,7 +646,7 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
           const int prow = __shfl_sync(0xffffffffu, cur.prow, src);
           const float ks = __shfl_sync(0xffffffffu, cur.ks, src), vs = __shfl_sync(0xffffffffu, cur.vs, src);
           const uint32_t valid = (cur.there >> (k * ppt)) & ((1u << ppt) - 1u);
-          float unit = fabsf(vs);
+          float unit = vs == vs ? fabsf(vs) : 0.0f;   // a NaN scale stays with its page
 #pragma unroll
           for (int o = 4; o > 0; o >>= 1) unit = fmaxf(unit, __shfl_xor_sync(0xffffffffu, unit, o));
           // the first slot of the tile free: the entry's last reader is far behind
@@ -655,7 +655,7 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
           Info& in = T.info[tile % kInfo];
           if (lane < 8) {
             in.ks[lane] = ks;
-            in.vr[lane] = unit > 0.0f ? 256.0f * (vs / unit) : 0.0f;
+            in.vr[lane] = vs != vs ? vs : unit > 0.0f ? 256.0f * (vs / unit) : 0.0f;
           }
           if (lane == 0) {
             const int t = cur.t + k;
@@ -878,11 +878,17 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
       for (int k = 0; k < 4; ++k) {
         const int tok = tok0 + 8 * k;
         const float2 ratio = both(in.vr[tok >> a.page_log2]);
+        const bool nan_scale = in.mask && ratio.x != ratio.x;
         uint8_t* p = pbuf + pb * C::kPBytes + tok * 16;
         uint16_t c[K][PP];
 #pragma unroll
         for (int g = 0; g < K; ++g) {
-          const float2 w = mul2(s[g][k], ratio);
+          float2 w = mul2(s[g][k], ratio);
+          if (nan_scale) {                      // 0 x NaN for the rows that do not see it
+            const int2 lim = *reinterpret_cast<const int2*>(&T.lim[seg & 1][row0 + 8 * g]);
+            if (in.t0 + tok >= lim.x) w.x = 0.0f;
+            if (in.t0 + tok >= lim.y) w.y = 0.0f;
+          }
           split2p<PP>(w.x, w.y, c[g]);
         }
 #pragma unroll

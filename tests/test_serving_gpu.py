@@ -483,6 +483,29 @@ def test_cache_attn_scales(pkg):
     check(pkg, randn(g, 1, 1, 16, 64, dtype=torch.float16), (k, v, ks, vs), table, lens)
 
 
+@pytest.mark.parametrize("page", [16, 64, 128])
+@pytest.mark.parametrize("H,Hkv,D,dt,which", [(8, 2, 64, "bf16", "v"), (8, 2, 128, "f16", "v"), (64, 2, 128, "bf16", "k"),
+                                              (16, 1, 512, "bf16", "shared"), (32, 2, 128, "bf16", "v")])
+@pytest.mark.parametrize("n,S,i", [(134, 9, 128), (150, 25, 144), (134, 1, 128)])
+def test_cache_attn_nan_scale(pkg, page, H, Hkv, D, dt, which, n, S, i):
+    """A page whose scale is NaN (here the one that holds token i, kv head 0) reaches the rows that see a token of it,
+    whether or not its tile has other pages, and no row that does not."""
+    g = gen(page + H + n)
+    table, n_pages = make_table(g, [n], page)
+    cache = make_cache(g, n_pages, Hkv, page, D, which == "shared")
+    q = randn(g, 1, S, H, D, dtype=DT[dt])
+    sl = torch.tensor([n], dtype=torch.int32, device="cuda")
+    want, bound = ref.attn(q, *cache, table, sl, D ** -0.5)
+    tol = ref.attn_tolerance(DT[dt], D, want, bound)
+    (cache[3] if which == "v" else cache[2])[table[0, i // page].long(), 0] = float("nan")
+    got = pkg.cache_attn(q, *cache, table, sl, D ** -0.5)
+    sees = n - S + 1 + torch.arange(S, device="cuda") > i // page * page
+    bad = torch.zeros_like(got, dtype=torch.bool)
+    bad[0, sees, :H // Hkv] = True
+    assert torch.equal(got.isnan(), bad)
+    assert ((got.double() - want).abs() <= tol)[~bad].all()
+
+
 def test_cache_attn_many_sequences(pkg):
     """More (sequence, row tile) pairs than threads of a CTA, and many empty sequences among them."""
     g = gen(51)
