@@ -794,7 +794,8 @@ static int cache_check(const char* name, int64_t B, int64_t S, int Hkv, int D, i
   if (!(page == 16 || page == 32 || page == 64 || page == 128))
     return fail(BS_ERR_UNSUPPORTED, "%s: pages of %lld tokens (16, 32, 64 or 128)", name, (long long)page);
   if (D % 16 != 0 || D > 512) return fail(BS_ERR_UNSUPPORTED, "%s: head dim %d (a multiple of 16 up to 512)", name, D);
-  if (n_pages * Hkv > 0x7ffffffe || max_pages * page > 0x7fffffff || n_pages > 0x7fffffff)
+  // positions are 32-bit numbers, and the kernels look up to a few tiles of 128 past the last one
+  if (n_pages > 0x7ffffffe / Hkv || max_pages > (0x7fffffff - 1023) / page)
     return fail(BS_ERR_UNSUPPORTED, "%s: %lld pages of %d heads, %lld pages per sequence", name, (long long)n_pages, Hkv,
                 (long long)max_pages);
   return BS_OK;

@@ -387,7 +387,8 @@ int bs_rope(const void* x, int dtype, int64_t tokens, int H, int D, int64_t x_to
  *   k_cache, v_cache  [n_pages, Hkv, page, D] e4m3; k_scale, v_scale
  *              [n_pages, Hkv] fp32; page 16, 32, 64 or 128; D a multiple of
  *              16 up to 512
- *   block_table  int32 [B, max_pages]; start  int32 [B], tokens already
+ *   block_table  int32 [B, max_pages], max_pages * page below 2^31 - 1023;
+ *              start  int32 [B], tokens already
  *              cached; new_lens  int32 [B] or NULL: how many of the S are real
  * Token i of sequence b goes to position start[b] + i.  A page's scale is the
  * smallest power of two that holds its values' amax (at least 1e-4) in 448;

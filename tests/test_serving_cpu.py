@@ -119,6 +119,15 @@ def test_attn_refusals(lib):
     assert lib.bs_cache_attn_workspace_size(4, 1, 8, 1, 128, 1) > 148 * 8 * 128 * 4
 
 
+def test_cache_lengths_refused(lib):
+    """Positions within a tile's reach of 2^31, where a tile's end would not be a 32-bit number; products past 64 bits."""
+    for most in (2 ** 27 - 1, 2 ** 27 - 63, 2 ** 62):              # pages of 16: 2^31 - 16, 2^31 - 1008 tokens
+        assert attn(lib, page=16, max_pages=most) == L.BS_ERR_UNSUPPORTED and b"pages per sequence" in lib.bs_last_error()
+        assert append(lib, page=16, max_pages=most) == L.BS_ERR_UNSUPPORTED
+    assert attn(lib, page=16, max_pages=2 ** 27 - 64, q=None) == L.BS_ERR_INVALID_ARG         # accepted up to the pointers
+    assert append(lib, n_pages=2 ** 62, Hkv=4) == L.BS_ERR_UNSUPPORTED
+
+
 def test_cpu_tensors_rejected(lib):
     pkg = import_pkg()
     x, w = torch.zeros(2, 256, dtype=torch.bfloat16), torch.ones(256, dtype=torch.bfloat16)
