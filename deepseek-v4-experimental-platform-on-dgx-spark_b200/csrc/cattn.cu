@@ -147,7 +147,7 @@ struct Info {                       // one tile, from the producer
   int limit;                        // tokens that any row sees
   int first, last;                  // of its segment
   int mask;                         // some row does not see all of the tile
-  int pad;
+  int nan;                          // bits of the pages whose value scale is NaN
 };
 
 __host__ __device__ constexpr int softmax_groups(int R) { return R >= 32 ? R / 16 : 1; }
@@ -653,9 +653,13 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
           ok = __all_sync(0xffffffffu, wait_quick(&T.empty[k_slot(k_sent)], k_par(k_sent) ^ 1, abort_flag));
           if (!ok) break;
           Info& in = T.info[tile % kInfo];
+          // a NaN scale makes its page's weights NaN where every row sees the tile; else they are 0, and the softmax
+          // warps note the page's tokens as NaN values
+          const bool mask = (cur.t + k + 1) * kTok > cur.low || valid != (1u << ppt) - 1u;
+          const uint32_t nan = __ballot_sync(0xffffffffu, vs != vs) & ((1u << ppt) - 1u);
           if (lane < 8) {
             in.ks[lane] = ks;
-            in.vr[lane] = vs != vs ? vs : unit > 0.0f ? 256.0f * (vs / unit) : 0.0f;
+            in.vr[lane] = vs != vs ? (mask ? 0.0f : vs) : unit > 0.0f ? 256.0f * (vs / unit) : 0.0f;
           }
           if (lane == 0) {
             const int t = cur.t + k;
@@ -665,7 +669,8 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
             in.limit = cur.limit;
             in.first = cur.first && k == 0;
             in.last = cur.last && k + 1 == cur.n;
-            in.mask = (t + 1) * kTok > cur.low || valid != (1u << ppt) - 1u;
+            in.mask = mask;
+            in.nan = (int)nan;
           }
           __syncwarp();
           k_chunks(prow);
@@ -878,17 +883,11 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
       for (int k = 0; k < 4; ++k) {
         const int tok = tok0 + 8 * k;
         const float2 ratio = both(in.vr[tok >> a.page_log2]);
-        const bool nan_scale = in.mask && ratio.x != ratio.x;
         uint8_t* p = pbuf + pb * C::kPBytes + tok * 16;
         uint16_t c[K][PP];
 #pragma unroll
         for (int g = 0; g < K; ++g) {
-          float2 w = mul2(s[g][k], ratio);
-          if (nan_scale) {                      // 0 x NaN for the rows that do not see it
-            const int2 lim = *reinterpret_cast<const int2*>(&T.lim[seg & 1][row0 + 8 * g]);
-            if (in.t0 + tok >= lim.x) w.x = 0.0f;
-            if (in.t0 + tok >= lim.y) w.y = 0.0f;
-          }
+          const float2 w = mul2(s[g][k], ratio);
           split2p<PP>(w.x, w.y, c[g]);
         }
 #pragma unroll
@@ -908,6 +907,10 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
         // in a row that only some see becomes zero too, and is put back for those when the segment ends.
         const int tok = quad * 32 + lane, t = in.t0 + tok;
         dead = !__all_sync(0xffffffffu, wait_quick(&T.v_ready, masked++ & 1, abort_flag));
+        if (in.nan && ((in.nan >> (tok >> a.page_log2)) & 1) && t < in.limit) {
+          T.nanseen[seg % kSegRing] = 1;
+          for (int d = 0; d < NC * 128; ++d) atomicMin(&T.nanmin[seg % kSegRing][d], t);
+        }
         for (int c = 0; c < NC && !dead; ++c) {
           uint4* row16 = reinterpret_cast<uint4*>(smem + v_slot(i * NC + c) * kChunk + tok * 128);
           for (int k = 0; k < 8; ++k) {
