@@ -1046,6 +1046,8 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
     for (int seg = 0; w.left > 0 && ok; ++seg) {
       const int t0 = w.t, t1 = w.seg_end(), nt = w.nt;
       w.next(a, R);
+      // The next rows' places go where those of the segment before this one were: all four warps are done with them.
+      if (seg > 0) group_all(8, true);
       // the other Q buffer: its last products are behind the O tiles taken out before
       if (C::QB == 2 && w.left > 0) stage(w, seg + 1);
       float acc[NC][R];
