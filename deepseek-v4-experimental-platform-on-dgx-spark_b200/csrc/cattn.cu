@@ -19,13 +19,20 @@
 // (8 bits) exactly and three an f16 value (11 bits).  Rows of Q are first
 // scaled by a power of two so that their amax lies in [128, 256): what the
 // terms cannot hold is below 2^-22 of the row's amax for two terms and 2^-26
-// for three.  P = exp2(s - max) * (page's value scale / largest of the tile) *
+// for three.  P = exp2(s - ref) * (page's value scale / largest of the tile) *
 // 256 is rounded to the same number of terms: with bf16 outputs to 2^-8 of the
 // value at most (2^-9, and f16 on the way; half a step of bf16 itself is
-// 2^-8), with f16 outputs to 2^-14.
+// 2^-8), with f16 outputs to 2^-14.  The terms end at a step, so this holds for
+// P above 2^-6; below, half that step is left, 2^-14 (bf16) or 2^-18 (f16),
+// 2^-22 or 2^-26 of the largest P there can be.  Hence ref is the row's maximum
+// in this tile, not the one so far: what a dominant key costs the small weights
+// beside it ends with its 128 tokens.  (Only tiles more than kReach = 24 powers
+// of two below the maximum so far use that minus kReach, so that sums stay in
+// range: there weights below 2^-46 of the largest are lost.)
 // Accumulation is fp32 in TMEM; O is taken out after every tile and added, in
-// fp32, to accumulators in registers, where the running maximum's factor and
-// the tile's value scale are applied.
+// fp32, to accumulators in registers, which follow ref from tile to tile (times
+// 2^-kReach, so that they are never above the result's own size) and where the
+// tile's value scale is applied.
 //
 // One work unit is a tile: 128 tokens of one (sequence, row tile, kv head);
 // a row tile is R of the S * (H / Hkv) query rows of a kv head.  All tiles of
@@ -59,6 +66,8 @@ constexpr int kChunk = kTok * 128;
 constexpr int kInfo = 16;          // tile info ring: above the tiles between the producer and the accumulators
 constexpr int kSegRing = 5;        // row sums of finished segments: the softmax warps run at most four segments ahead
 constexpr int kMaxSlots = 12;
+constexpr float kReach = 24.0f;    // powers of two that a tile's reference may lie below the row's maximum
+constexpr float kReachScale = 16777216.0f;
 
 struct Args {
   const void* q;
@@ -71,7 +80,7 @@ struct Args {
   const float* sink;               // [H] or null
   void* out;                       // [B, S, H, D]
   int* plan;                       // [1 + B * RT]: places per CTA, first place of each (sequence, row tile)
-  float* part_ml;                  // [2 * grid][R][2]
+  float* part_ml;                  // [2 * grid][R][2]: reference, sum
   float* part_o;                   // [2 * grid][R][NC * 128]
   int B, S, H, Hkv, G, D, RT, page_log2, max_pages, n_pages;
   float scale_log2;                // softmax scale x log2(e)
@@ -772,7 +781,7 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
     const int tok0 = quad * 32 + (lane >> 2);
     const int row0 = wg * RW + 2 * (lane & 3);
     const uint32_t t_lane = tmem + ((uint32_t)(quad * 32) << 16) + wg * RW;
-    float2 l[K], m[K], qf[K];
+    float2 l[K], m[K], ref[K], qf[K];    // sum relative to 2^ref, maximum so far
     int seg = -1, masked = 0;
     bool dead = false;
     for (int i = 0; i < count; ++i) {
@@ -795,7 +804,7 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
 #pragma unroll
             for (int g = 0; g < K; ++g) {
               qf[g] = *reinterpret_cast<const float2*>(&T.qf[seg & 1][row0 + 8 * g]);
-              m[g] = both(-INFINITY);
+              m[g] = ref[g] = both(-INFINITY);
               l[g] = both(0.0f);
             }
           }
@@ -865,11 +874,12 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
         const float4 x = *reinterpret_cast<const float4*>(T.wmax[i & 1][row0 + 8 * g]);
         const float4 y = *reinterpret_cast<const float4*>(T.wmax[i & 1][row0 + 8 * g + 1]);
         const float2 top = mul2(make_float2(fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)), fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w))), qf[g]);
-        const float2 now = make_float2(fmaxf(m[g].x, top.x), fmaxf(m[g].y, top.y));
+        m[g] = make_float2(fmaxf(m[g].x, top.x), fmaxf(m[g].y, top.y));
+        const float2 now = make_float2(fmaxf(top.x, m[g].x - kReach), fmaxf(top.y, m[g].y - kReach));
         // rows that have seen no token yet: -inf - 0
         const float2 use = make_float2(now.x == -INFINITY ? 0.0f : now.x, now.y == -INFINITY ? 0.0f : now.y);
-        const float2 al = make_float2(ex2(m[g].x - use.x), ex2(m[g].y - use.y));
-        m[g] = now;
+        const float2 al = make_float2(ex2(ref[g].x - use.x), ex2(ref[g].y - use.y));
+        ref[g] = now;
         const float2 neg = make_float2(-use.x, -use.y);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -951,7 +961,7 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
             x = add2(x, make_float2(__shfl_xor_sync(0xffffffffu, x.x, o), __shfl_xor_sync(0xffffffffu, x.y, o)));
           if (lane < 4) {
             *reinterpret_cast<float2*>(&T.lsum[seg % kSegRing][quad][row0 + 8 * g]) = x;
-            if (quad == 0) *reinterpret_cast<float2*>(&T.mfin[seg % kSegRing][row0 + 8 * g]) = m[g];
+            if (quad == 0) *reinterpret_cast<float2*>(&T.mfin[seg % kSegRing][row0 + 8 * g]) = ref[g];
           }
         }
         __syncwarp();
@@ -1060,7 +1070,7 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
         ok = __all_sync(0xffffffffu, wait_quick(&T.o_full[ob], (i / C::OB) & 1, abort_flag));
         if (!ok) break;               // out of the tile loop; the group's barrier below ends the role
         tc_fence_after();
-        const float unit = T.info[i % kInfo].unit * (1.0f / 256.0f);
+        const float unit = T.info[i % kInfo].unit * (1.0f / 256.0f / kReachScale);
         const float* al = T.alpha[i & 3];
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
@@ -1087,7 +1097,7 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
       ok = ok && __all_sync(0xffffffffu, wait_quick(&T.l_full[sr], (seg / kSegRing) & 1, abort_flag));
       const bool whole = t0 == 0 && t1 == nt;
       const int64_t slot = 2 * (int64_t)blockIdx.x + (seg == 0 ? 0 : 1);
-      // Row r's factor (1 over its sum), once, by thread r; partial results keep their sum and maximum instead.
+      // Row r's factor (1 over its sum), once, by thread r; partial results keep their sum and reference instead.
       const int row = quad * 32 + lane;
       if (ok && row < R) {
         const float lr = T.lsum[sr][0][row] + T.lsum[sr][1][row] + T.lsum[sr][2][row] + T.lsum[sr][3][row];
@@ -1104,7 +1114,7 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
             f = m == -INFINITY ? 0.0f : exp2f(m - M);
             z = lr * f + (sk == -INFINITY ? 0.0f : exp2f(sk - M));
           }
-          f = z == 0.0f ? 0.0f : f / z;
+          f = z == 0.0f ? 0.0f : f / z * kReachScale;
         }
         T.fin[buf][row] = f;
       }
@@ -1201,7 +1211,7 @@ __global__ void __launch_bounds__(256) merge_kernel(const Args a, int R, int row
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
       if (sk != -INFINITY) z += exp2f(sk - use);
-      const float f = z == 0.0f ? 0.0f : 1.0f / z;
+      const float f = z == 0.0f ? 0.0f : kReachScale / z;
       constexpr int step = SPLIT ? 8 : 1;
       for (int cb = c0 + (SPLIT ? warp : 0); cb <= c1; cb += 32 * step) {
         const int n = min(32, (c1 - cb) / step + 1);

@@ -55,3 +55,80 @@ def test_cache_attn_quick_segments(pkg, B, S, H, Hkv, D, dt, shared):
         out.fill_(float("nan"))
         attn_into(pkg, out, ws, q, cache, table, sl, D ** -0.5)
         assert torch.equal(out, want)
+
+
+# ------------------------------------------------------------------ weights far below a row's largest
+
+def precise_tolerance(q, cache, table, n, scale, lims):
+    """Reference and tolerance of one sequence and one kv head, rows [S x G], that do not grow with the longest context.
+
+    A weight enters as two (bf16) or three (f16) e4m3 terms: 2^-8 or 2^-12 of itself, or, where it is too small for that,
+    half the last term's smallest step, 2^-10 / 16 or / 256, on a scale where the largest weight x page scale that the row
+    sees in the tile of 128 tokens is at least 256 / 4: 2^-20 or 2^-24 of that largest one (in tiles far below the row's
+    maximum, of 2^-24 of that), and never more than the weight itself.  Scores: an ulp (2^-23) of the sum of their magnitudes for each of terms x D products; the rest 2^-18; the
+    result's own rounding.
+    """
+    S, H, D = q.shape[1:]
+    page = cache[0].shape[2]
+    ids = table[0, :(n + page - 1) // page].long()
+    k = (cache[0][ids, 0].double() * cache[2][ids, 0].double()[:, None, None]).flatten(0, 1)[:n]
+    code = cache[1][ids, 0].double().flatten(0, 1)[:n]
+    vs = cache[3][ids, 0].double().repeat_interleave(page)[:n]
+    qq = q[0].double()                                                     # [S, H, D]
+    a = torch.einsum("shd,td->sht", qq, k) * scale
+    see = torch.arange(n, device="cuda")[None, None] < torch.tensor(lims, device="cuda")[:, None, None]
+    a = a.masked_fill(~see, -float("inf"))
+    w = torch.exp(a - a.amax(-1, keepdim=True))
+    w = w / w.sum(-1, keepdim=True)
+    two = q.dtype == torch.bfloat16
+    terms = (torch.einsum("shd,td->sht", qq.abs(), k.abs()) * see).amax(-1, keepdim=True) * scale
+    d = (2 if two else 3) * D * 2.0 ** -23 * terms
+    wv = w * vs.abs()
+    pad = -n % 128
+    tiles = torch.nn.functional.pad(wv, (0, pad)).unflatten(-1, (-1, 128))
+    far = wv.amax(-1, keepdim=True)[..., None] * 2.0 ** -24
+    least = (torch.maximum(tiles.amax(-1, keepdim=True), far) * (2.0 ** -20 if two else 2.0 ** -24)).expand_as(tiles).flatten(-2)[..., :n]
+    out, mass = (w * vs) @ code, wv @ code.abs()
+    small = torch.minimum(wv, least * see) @ code.abs()
+    tol = (mass * ((2.0 ** -8 if two else 2.0 ** -12) + 2 * d + 2.0 ** -18) + small
+           + (out.abs() + mass * d) * torch.finfo(q.dtype).eps / 2 + (0.0 if two else 2.0 ** -25) + 1e-30)
+    return out, tol
+
+
+def assert_precise(pkg, q, cache, table, n, scale, B=1):
+    """B sequences over the same pages, with the same queries."""
+    S = q.shape[1]
+    sl = torch.full((B,), n, dtype=torch.int32, device="cuda")
+    got = pkg.cache_attn(q.expand(B, -1, -1, -1), *cache, table.expand(B, -1), sl, scale).double()
+    want, tol = precise_tolerance(q, cache, table, n, scale, [n - S + i + 1 for i in range(S)])
+    err = (got - want).abs()
+    print(f"worst error / tolerance {float((err / tol).max()):.3f}, rel. Frobenius {float(err.norm() / want.norm()):.2e}")
+    assert (err <= tol).all()
+    return err, want
+
+
+@pytest.mark.parametrize("dt,S", [("bf16", 1), ("f16", 1), ("bf16", 16)])
+@pytest.mark.parametrize("nats", [13.0, 15.0, 18.0, 20.0])
+@pytest.mark.parametrize("at", [0, 7001])
+def test_cache_attn_peak(pkg, dt, S, nats, at):
+    """One key far above 20000 others whose value is zero: the result is the others', a few hundredths of the weight or
+    less, and keeps its digits.  600 such sequences: a CTA has all of a head's tokens, so its maximum stays the peak's."""
+    g = gen(int(nats) + S + at)
+    n, page, H, D = 20000, 64, 4, 128
+    table, n_pages = make_table(g, [n], page)
+    codes = lambda: (torch.randn(n_pages, 1, page, D, generator=g, device="cuda") * 90).clamp(-448, 448)
+    k, v = codes(), codes().abs()
+    ks, vs = torch.full((n_pages, 1), 2.0 ** -7, device="cuda"), torch.full((n_pages, 1), 2.0 ** -8, device="cuda")
+    base = torch.randn(D, generator=g, device="cuda").sign()
+    q = (base + 0.1 * randn(g, 1, S, H, D)).to(DT[dt])
+    p, slot = table[0, at // page].long(), at % page
+    k[p], v[p, 0, slot] = 0, 0                    # a page of the peak's own, so that its scale sets the score
+    k[p, 0, slot] = base
+    scale = D ** -0.5
+    ks[p] = nats / (D * scale)
+    cache = (k.to(torch.float8_e4m3fn), v.to(torch.float8_e4m3fn), ks, vs)
+    err, want = assert_precise(pkg, q, cache, table, n, scale, 600)
+    # Over all outputs: weights off by 2^-8 (2^-12) and a rounding of 2^-9 (2^-12), doubled; and what shares a tile with the
+    # peak may be lost whole.  Those 127 of n tokens weigh 1 (score 0 on the peak's page) or as the others do, 127 / n of
+    # the result at most.
+    assert err.norm() <= want.norm() * 600 ** 0.5 * ((2.0 ** -7 if dt == "bf16" else 2.0 ** -10) + 127 / n)
