@@ -28,7 +28,11 @@
 // in this tile, not the one so far: what a dominant key costs the small weights
 // beside it ends with its 128 tokens.  (Only tiles more than kReach = 24 powers
 // of two below the maximum so far use that minus kReach, so that sums stay in
-// range: there weights below 2^-46 of the largest are lost.)
+// range: there weights below 2^-46 of the largest are lost.)  Where the value
+// scales of a tile's pages differ by more than kSpread = 4, the largest may be
+// that of a page which a row does not see or hardly weighs; in such tiles ref is
+// the row's largest product of weight and scale (scales below 2^-kFar = 2^-64 of
+// the largest count as that, so that weights stay in range).
 // Accumulation is fp32 in TMEM; O is taken out after every tile and added, in
 // fp32, to accumulators in registers, which follow ref from tile to tile (times
 // 2^-kReach, so that they are never above the result's own size) and where the
@@ -68,6 +72,8 @@ constexpr int kSegRing = 5;        // row sums of finished segments: the softmax
 constexpr int kMaxSlots = 12;
 constexpr float kReach = 24.0f;    // powers of two that a tile's reference may lie below the row's maximum
 constexpr float kReachScale = 16777216.0f;
+constexpr float kSpread = 4.0f;    // largest ratio of a tile's value scales that the maximum of the scores takes as one
+constexpr float kFar = 64.0f;
 
 struct Args {
   const void* q;
@@ -155,8 +161,9 @@ struct Info {                       // one tile, from the producer
   int t0;                           // first token
   int limit;                        // tokens that any row sees
   int first, last;                  // of its segment
-  int mask;                         // some row does not see all of the tile
-  int nan;                          // bits of the pages whose value scale is NaN
+  int mask;                         // some row does not see all of the tile, or spread
+  uint16_t nan;                     // bits of the pages whose value scale is NaN
+  uint16_t spread;                  // value scales (other than 0) differ by more than kSpread
 };
 
 __host__ __device__ constexpr int softmax_groups(int R) { return R >= 32 ? R / 16 : 1; }
@@ -664,7 +671,8 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
           Info& in = T.info[tile % kInfo];
           // a NaN scale makes its page's weights NaN where every row sees the tile; else they are 0, and the softmax
           // warps note the page's tokens as NaN values
-          const bool mask = (cur.t + k + 1) * kTok > cur.low || valid != (1u << ppt) - 1u;
+          const bool spread = __any_sync(0xffffffffu, vs != 0.0f && fabsf(vs) * kSpread < unit);
+          const bool mask = (cur.t + k + 1) * kTok > cur.low || valid != (1u << ppt) - 1u || spread;
           const uint32_t nan = __ballot_sync(0xffffffffu, vs != vs) & ((1u << ppt) - 1u);
           if (lane < 8) {
             in.ks[lane] = ks;
@@ -679,7 +687,8 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
             in.first = cur.first && k == 0;
             in.last = cur.last && k + 1 == cur.n;
             in.mask = mask;
-            in.nan = (int)nan;
+            in.nan = (uint16_t)nan;
+            in.spread = spread;
           }
           __syncwarp();
           k_chunks(prow);
@@ -829,6 +838,18 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
               s[g][k] = mul2(x, both(ks[k]));
             }
         }
+        // Maxima of the thread's 2K rows over its tokens, then over the warp's 32, in a butterfly that halves the rows with
+        // the lanes: lane group (lane / 4) % 2K ends up with row 8 (v / 2) + v % 2 of v = that number.
+        float x[2 * K];
+        auto over_tokens = [&](auto of) {
+#pragma unroll
+          for (int g = 0; g < K; ++g) {
+            x[2 * g] = fmaxf(fmaxf(of(s[g][0].x, 0, qf[g].x), of(s[g][1].x, 1, qf[g].x)),
+                             fmaxf(of(s[g][2].x, 2, qf[g].x), of(s[g][3].x, 3, qf[g].x)));
+            x[2 * g + 1] = fmaxf(fmaxf(of(s[g][0].y, 0, qf[g].y), of(s[g][1].y, 1, qf[g].y)),
+                                 fmaxf(of(s[g][2].y, 2, qf[g].y), of(s[g][3].y, 3, qf[g].y)));
+          }
+        };
         if (in.mask) {
 #pragma unroll
           for (int g = 0; g < K; ++g) {
@@ -841,14 +862,18 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
               if (!there || t >= lim.y) s[g][k].y = -INFINITY;
             }
           }
-        }
-        // Maxima of the thread's 2K rows over the warp's 32 tokens, in a butterfly that halves the rows with the lanes:
-        // lane group (lane / 4) % 2K ends up with row 8 (v / 2) + v % 2 of v = that number.
-        float x[2 * K];
+          // (asked here, not for every tile: beside this choice the code of all tiles came out 12 % slower)
+          if (in.spread) {           // of score and the scale's logarithm (x is multiplied by qf afterwards)
+            float lv[4];
 #pragma unroll
-        for (int g = 0; g < K; ++g) {
-          x[2 * g] = fmaxf(fmaxf(s[g][0].x, s[g][1].x), fmaxf(s[g][2].x, s[g][3].x));
-          x[2 * g + 1] = fmaxf(fmaxf(s[g][0].y, s[g][1].y), fmaxf(s[g][2].y, s[g][3].y));
+            for (int k = 0; k < 4; ++k)
+              lv[k] = fmaxf(__log2f(fabsf(in.vr[(tok0 + 8 * k) >> a.page_log2]) * (1.0f / 256.0f)), -kFar);
+            over_tokens([&](float y, int k, float q) { return y + __fdividef(lv[k], q); });
+          } else {
+            over_tokens([](float y, int, float) { return y; });
+          }
+        } else {
+          over_tokens([](float y, int, float) { return y; });
         }
         int n = 2 * K;
 #pragma unroll

@@ -65,7 +65,7 @@ def precise_tolerance(q, cache, table, n, scale, lims):
     A weight enters as two (bf16) or three (f16) e4m3 terms: 2^-8 or 2^-12 of itself, or, where it is too small for that,
     half the last term's smallest step, 2^-10 / 16 or / 256, on a scale where the largest weight x page scale that the row
     sees in the tile of 128 tokens is at least 256 / 4: 2^-20 or 2^-24 of that largest one (in tiles far below the row's
-    maximum, of 2^-24 of that), and never more than the weight itself.  Scores: an ulp (2^-23) of the sum of their magnitudes for each of terms x D products; the rest 2^-18; the
+    maximum, of 2^-24 of that and the tile's largest scale), and never more than the weight itself.  Scores: an ulp (2^-23) of the sum of their magnitudes for each of terms x D products; the rest 2^-18; the
     result's own rounding.
     """
     S, H, D = q.shape[1:]
@@ -86,7 +86,8 @@ def precise_tolerance(q, cache, table, n, scale, lims):
     wv = w * vs.abs()
     pad = -n % 128
     tiles = torch.nn.functional.pad(wv, (0, pad)).unflatten(-1, (-1, 128))
-    far = wv.amax(-1, keepdim=True)[..., None] * 2.0 ** -24
+    scales = torch.nn.functional.pad(vs.abs(), (0, pad)).unflatten(-1, (-1, 128)).amax(-1)[:, None]
+    far = w.amax(-1, keepdim=True)[..., None] * scales * 2.0 ** -24
     least = (torch.maximum(tiles.amax(-1, keepdim=True), far) * (2.0 ** -20 if two else 2.0 ** -24)).expand_as(tiles).flatten(-2)[..., :n]
     out, mass = (w * vs) @ code, wv @ code.abs()
     small = torch.minimum(wv, least * see) @ code.abs()
@@ -132,3 +133,39 @@ def test_cache_attn_peak(pkg, dt, S, nats, at):
     # peak may be lost whole.  Those 127 of n tokens weigh 1 (score 0 on the peak's page) or as the others do, 127 / n of
     # the result at most.
     assert err.norm() <= want.norm() * 600 ** 0.5 * ((2.0 ** -7 if dt == "bf16" else 2.0 ** -10) + 127 / n)
+
+
+@pytest.mark.parametrize("dt,H,S,page", [("bf16", 4, 20, 16), ("f16", 4, 20, 16), ("bf16", 1, 7, 16), ("bf16", 2, 24, 32)])
+def test_cache_attn_hidden_scale(pkg, dt, H, S, page):
+    """A page that a row does not see, or hardly weighs, may have a value scale 2^24 times that of the pages it lives on:
+    the row keeps its digits."""
+    g = gen(H + S + page)
+    n, D = 2 * page + 8, 128
+    table, n_pages = make_table(g, [n], page)
+    k, v, ks, vs = make_cache(g, n_pages, 1, page, D)
+    ids = table[0].long()
+    vs.fill_(2.0 ** -22)
+    vs[ids[2]] = 4.0
+    base = torch.randn(D, generator=g, device="cuda").sign()
+    q = (base + 0.5 * randn(g, 1, S, H, D)).to(DT[dt])
+    assert_precise(pkg, q, (k, v, ks, vs), table, n, D ** -0.5)
+    k[ids[2]] = (-base).to(torch.float8_e4m3fn)                            # the last page 33 nats below
+    ks[ids[2]] = 33.0 / (D * D ** -0.5)
+    assert_precise(pkg, q, (k, v, ks, vs), table, n, D ** -0.5)
+    vs[ids[1]] = 0.0
+    assert_precise(pkg, q, (k, v, ks, vs), table, n, D ** -0.5)
+
+
+@pytest.mark.parametrize("dt,H,S,D,page,n", [("bf16", 8, 1, 128, 16, 9000), ("f16", 16, 1, 64, 32, 5000), ("bf16", 8, 12, 128, 16, 700),
+                                             ("bf16", 32, 1, 512, 64, 3000), ("f16", 4, 7, 256, 16, 650), ("bf16", 32, 1, 256, 128, 5000)])
+@pytest.mark.parametrize("sharp", [1.0, 5.0])
+def test_cache_attn_spread_scales(pkg, dt, H, S, D, page, n, sharp):
+    """Value scales from 2^-22 to 2^3 beside each other, flat and sharp rows."""
+    g = gen(H + S + n)
+    table, n_pages = make_table(g, [n], page)
+    k, v, ks, vs = make_cache(g, n_pages, 1, page, D)
+    vs.copy_(torch.exp2(torch.randint(-22, 4, vs.shape, generator=g, device="cuda").float()))
+    vs[table[0, 1].long()] *= -1.7
+    q = (sharp * randn(g, 1, S, H, D)).to(DT[dt])
+    assert_precise(pkg, q, (k, v, ks, vs), table, n, D ** -0.5)
+    assert_precise(pkg, q, (k, v, ks, vs), table, n, D ** -0.5, 40)
