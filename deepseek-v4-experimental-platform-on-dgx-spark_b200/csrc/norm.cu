@@ -11,13 +11,14 @@
 //   code = e4m3_rn(y / s)      2^ceil(log2 s) for s in the power-of-two form
 //
 // The codes come from the fp32 y: act_quant(rms_norm(x)) would round y to 16
-// bits first.  y is the fp32 number nearest to its exact value: per-thread sums
-// of 8 squares are added up in fp64 (for few rows every square is; for many
-// that costs 18 to 25 % and moves y by a step in about one value of a hundred),
-// the root is kept as a sum of two fp32.  s and y / s are rounded to nearest as well.  It
-// costs a few instructions under the loads, and values next to the border of
-// two codes (with 16-bit inputs y / s often lies on one) fall as the formula
-// in exact fp32 steps says.
+// bits first.  Eight squares at a time are added in fp32 and their sums in fp64,
+// in every form of the kernel, so that a row's result does not depend on how
+// many rows the call has.  (Every square in fp64, or eight with what their sums
+// round away, costs 12 % of 16384 x 7168 bf16 and 21 % of 1999 x 5120 f16; it
+// would move y, by its last fp32 bit, in about one value of a hundred.)  The
+// root is kept as a sum of two fp32; y, s and y / s are rounded to nearest, so
+// values next to the border of two codes (with 16-bit inputs y / s often lies
+// on one) fall as the formula in fp32 steps says, but for that last bit of y.
 //
 // HBM-bound: every value is read and written once.  A block of 128 values is
 // half a warp x 8 values, so its amax is four shuffles.  Two forms:
@@ -74,11 +75,16 @@ BS_DEVINL float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
-// Sum of eight squares.
-BS_DEVINL float squares(const float* f) {
+// Sum of eight squares: in fp32, and where that leaves its range (values above 2^60, tiny ones, infinities, NaN) in fp64.
+BS_DEVINL double squares(const float* f) {
   const float a = fmaf(f[1], f[1], f[0] * f[0]), b = fmaf(f[3], f[3], f[2] * f[2]);
   const float c = fmaf(f[5], f[5], f[4] * f[4]), d = fmaf(f[7], f[7], f[6] * f[6]);
-  return (a + b) + (c + d);
+  const float s = (a + b) + (c + d);
+  if (s > 0x1p-90f && s < 0x1p120f) return (double)s;
+  double t = 0.0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) t = fma((double)f[i], (double)f[i], t);
+  return t;
 }
 BS_DEVINL double row_sum(double sum, double* part) {
 #pragma unroll
@@ -235,12 +241,7 @@ __global__ void __launch_bounds__(kMaxThreads) rms_rows_kernel(const Args a) {
   double sum = 0.0;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    if constexpr (V == 1) {          // few rows: every square exactly
-#pragma unroll
-      for (int i = 0; i < 8; ++i) sum = fma((double)f[v][i], (double)f[v][i], sum);
-    } else {
-      sum += (double)squares(f[v]);
-    }
+    sum += squares(f[v]);
   }
   const float2 r = inv_sqrt(fma(row_sum(sum, part), a.inv_h, (double)a.eps));
   const T* w = reinterpret_cast<const T*>(a.w);
@@ -329,7 +330,7 @@ __global__ void __maxnreg__(RES ? 128 : 96) rms_ring_kernel(const Args a, int st
 #pragma unroll
         for (int i = 0; i < 8; ++i) f[v][i] = 0.0f;
       }
-      sum += (double)squares(f[v]);
+      sum += squares(f[v]);
     }
     // the barrier in row_sum: every thread has read this stage
     const float2 r = inv_sqrt(fma(row_sum(sum, t.part[n & 1]), a.inv_h, (double)a.eps));

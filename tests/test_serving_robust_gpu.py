@@ -169,3 +169,53 @@ def test_cache_attn_spread_scales(pkg, dt, H, S, D, page, n, sharp):
     q = (sharp * randn(g, 1, S, H, D)).to(DT[dt])
     assert_precise(pkg, q, (k, v, ks, vs), table, n, D ** -0.5)
     assert_precise(pkg, q, (k, v, ks, vs), table, n, D ** -0.5, 40)
+
+
+# ------------------------------------------------------------------ norm: values of any size, calls of any number of rows
+
+@pytest.mark.parametrize("dt", ["bf16", "f32", "f16"])
+@pytest.mark.parametrize("rows,H", [(3, 512), (5, 7168), (700, 1024), (1500, 1024), (4000, 4096)])
+@pytest.mark.parametrize("res", [False, True])
+def test_rms_norm_size_of_values(pkg, dt, rows, H, res):
+    """Rows of 1e-30 to 1e37, whose squares leave fp32, beside ordinary ones, zeros, infinities and NaN, in every form."""
+    g = gen(rows + H)
+    big = dt != "f16"
+    size = torch.tensor([1.0, 1e20, 1e30, 1e37, 1e-25, 1e-30, 0.0] if big else [1.0, 1e4, 3e-5, 1e-2, 0.0], device="cuda")
+    x = (torch.randn(rows, H, generator=g, device="cuda") * size[torch.arange(rows, device="cuda") % len(size)][:, None]).to(DT[dt])
+    r = torch.zeros_like(x) if res else None
+    w = (1 + 0.1 * randn(g, H)).to(DT[dt])
+    for eps in (1e-6, 0.0):
+        got = pkg.rms_norm(x, w, eps, residual=r)
+        y = got[0] if res else got
+        want = ref.rms(x, w, eps)
+        tol = want.abs() * (torch.finfo(DT[dt]).eps / 2 + 2.0 ** -18) + (2.0 ** -25 if dt == "f16" else 2.0 ** -126)
+        dead = (x == 0).all(-1)                   # 0 / 0 without an eps
+        ok = ~dead if eps == 0.0 else torch.ones_like(dead)
+        assert ((y.double() - want).abs() <= tol)[ok].all()
+        c, s = pkg.rms_norm_quant(x, w, eps, residual=r)[:2]
+        deq = c.to(torch.float32).double().unflatten(-1, (-1, 128)) * s.double()[..., None]
+        half = torch.maximum(want.abs() * 2.0 ** -4, s.double().repeat_interleave(128, -1) * 2.0 ** -10)
+        assert ((deq.flatten(-2) - want).abs() <= half * (1 + 2.0 ** -12) + want.abs() * 2.0 ** -17)[ok].all()
+    x[1, 7], x[2, 9] = float("inf"), float("nan")
+    y = pkg.rms_norm(x, w, 1e-6)
+    assert y[2].isnan().all() and y[1, 7].isnan() and (y[1, :7] == 0).all() and torch.isfinite(y[0]).all()
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("H,res", [(1024, True), (4096, False), (5120, True)])
+def test_rms_norm_row_alone(pkg, dt, H, res):
+    """A row's result is the same in calls of any number of rows, whatever form of the kernel they take: its sum is the same
+    sum of 8-square sums in fp64 up to their order, 2^-50 or so, which a rounding to 16 bits shows in one value of 2^40."""
+    g = gen(H)
+    rows = 6000
+    x = randn(g, rows, H, dtype=DT[dt])
+    r = randn(g, rows, H, dtype=DT[dt]) if res else None
+    w = (1 + 0.2 * randn(g, H)).to(DT[dt])
+    cut = lambda t, n: None if t is None else t[:n]
+    y = pkg.rms_norm(x, w, residual=r)
+    c = pkg.rms_norm_quant(x, w, residual=r)
+    for n in (1, 200, 295, 296, 1000, 1199, 1200, 2500):
+        for a, b in zip(pkg.rms_norm(cut(x, n), w, residual=cut(r, n)) if res else [pkg.rms_norm(x[:n], w)], y if res else [y]):
+            assert torch.equal(a, b[:n])
+        for a, b in zip(pkg.rms_norm_quant(cut(x, n), w, residual=cut(r, n)), c):
+            assert torch.equal(a.view(torch.uint8), b[:n].view(torch.uint8))
