@@ -11,7 +11,9 @@
 // exponent, and a code changes its value only where it becomes subnormal.
 // A page whose slot 0 is written by this call starts anew (whatever it held
 // before does not count), and slots behind the new tokens are left alone.
-// Infinities and NaN are stored as NaN and take no part in the scale.
+// Infinities and NaN are stored as NaN and take no part in the scale.  A page
+// whose scale is NaN or infinite keeps it, with codes of NaN (new values over an
+// infinite scale are zero), until its slot 0 is written.
 //
 // One CTA per (sequence, page it touches, head), for its keys and values: it owns that
 // page and head, so there are no atomics and the result does not depend on any
@@ -204,8 +206,9 @@ __global__ void __maxnreg__(64) append_kernel(const Args a) {
     __syncthreads();                          // every thread has read the old scales
 #pragma unroll
     for (int w = 0; w < W; ++w) {
-      s[w] = fmaxf(s[w], old[w]);
-      if (s[w] > old[w]) {
+      s[w] = nan_max(s[w], old[w]);
+      // grown, or no number: its codes are none then either (max and quotient as the formula has them)
+      if (s[w] != old[w] || !(s[w] < __uint_as_float(0x7F800000u))) {
         const float f = __fdiv_rn(old[w], s[w]);
         const int n16 = before * a.D / 16;
         uint4* dst = reinterpret_cast<uint4*>(a.cache[w] + sat * ((int64_t)a.D << a.page_log2));

@@ -395,7 +395,8 @@ int bs_rope(const void* x, int dtype, int64_t tokens, int H, int D, int64_t x_to
  * if it has to grow, the page's earlier codes are rounded again to the larger
  * scale.  Writing a page's slot 0 starts it anew; slots behind the new tokens
  * are left as they are.  Non-finite values are stored as NaN and do not count
- * for the scale.  Two sequences of a call must not write to the same page.
+ * for the scale.  A page whose scale is NaN or infinite stays without numbers
+ * until its slot 0 is written.  Two sequences of a call must not write to the same page.
  * A page index or length out of range writes nothing there and is reported
  * by bs_device_error_check().
  */

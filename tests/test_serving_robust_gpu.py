@@ -219,3 +219,28 @@ def test_rms_norm_row_alone(pkg, dt, H, res):
             assert torch.equal(a, b[:n])
         for a, b in zip(pkg.rms_norm_quant(cut(x, n), w, residual=cut(r, n)), c):
             assert torch.equal(a.view(torch.uint8), b[:n].view(torch.uint8))
+
+
+# ------------------------------------------------------------------ cache append: scales that are no numbers
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_cache_append_onto_bad_scale(pkg, dt, bad):
+    """Tokens behind the first of a page whose scale is NaN or infinite do not turn its codes into numbers; a page begun anew
+    forgets it."""
+    g = gen(17)
+    starts, page, Hkv, D, S = [5, 16, 30], 16, 2, 64, 9
+    table, n_pages = make_table(g, [n + S for n in starts], page)
+    k_cache, v_cache, ks, vs = make_cache(g, n_pages, Hkv, page, D)
+    ks[table[0, 0].long(), 1] = bad
+    vs[table[0, 0].long(), 0] = bad
+    vs[table[1, 1].long()] = bad                  # written from slot 0 on
+    ks[table[2, 1].long(), 0] = bad
+    k, v = randn(g, 3, S, Hkv, D, dtype=DT[dt]), randn(g, 3, S, Hkv, D, dtype=DT[dt])
+    k[0, 3, 1, 4] = float("inf")
+    start = torch.tensor(starts, dtype=torch.int32, device="cuda")
+    wk, wv = ref.append(k, k_cache.float(), ks, table, start), ref.append(v, v_cache.float(), vs, table, start)
+    pkg.cache_append(k, v, k_cache, v_cache, ks, vs, table, start)
+    for codes, scale, want in ((k_cache, ks, wk), (v_cache, vs, wv)):
+        assert same_codes(codes, want[0]) and torch.equal(scale.double().nan_to_num(-1.0, -2.0), want[1].nan_to_num(-1.0, -2.0))
+    assert torch.isfinite(vs[table[1, 1].long()]).all()
