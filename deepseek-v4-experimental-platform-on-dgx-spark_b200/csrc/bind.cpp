@@ -8,6 +8,7 @@
 // given again.  Their addresses come from the library that _lib.py loaded, so
 // there is one copy of it.
 #include <ATen/MemoryOverlap.h>
+#include <ATen/core/grad_mode.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -101,6 +102,11 @@ at::Tensor empty(const at::Tensor& like, at::IntArrayRef shape, at::ScalarType d
 
 bool misaligned(const at::Tensor& t, uintptr_t a) { return reinterpret_cast<uintptr_t>(t.const_data_ptr()) % a != 0; }
 
+// What torch's own in-place operators do: autograd's saved tensors then notice that their values are gone.
+void changed(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // t, or a copy where it is not contiguous or does not start on 16 bytes.
 at::Tensor dense(const at::Tensor& t) {
   return t.is_contiguous() && !misaligned(t, 16) ? t : t.clone(at::MemoryFormat::Contiguous);
@@ -160,6 +166,8 @@ py::tuple rope(const at::Tensor& x, const at::Tensor& positions, const at::Tenso
     bad_value("rope: positions ", positions.sizes(), " do not match x ", x.sizes());
   const int64_t H = x.size(-2), D = x.size(-1);
   if (H > INT_MAX || D > INT_MAX) bad_value("rope: x ", x.sizes());
+  if (inplace && at::GradMode::is_enabled() && x.requires_grad())
+    bad_value("rope: an in-place x requires a gradient, which would miss the turn");
   if (inplace && at::has_internal_overlap(x) == at::MemOverlap::Yes) bad_value("rope: an in-place x overlaps itself");
   at::Tensor xt = x;
   int64_t tok = H * D, head = D;
@@ -179,6 +187,7 @@ py::tuple rope(const at::Tensor& x, const at::Tensor& positions, const at::Tenso
   const int st = p_rope(xt.const_data_ptr(), tag(dt), positions.numel(), (int)H, (int)D, tok, head, pc->const_data_ptr(),
                         pt == at::kLong, (const double*)fc->const_data_ptr(), (int)(2 * freqs.numel()), offset, half, inverse,
                         (float)scale, out.mutable_data_ptr(), inplace ? tok : H * D, inplace ? head : D, on.stream);
+  if (inplace && st == BS_OK) changed(x);
   return py::make_tuple(st, out);
 }
 
@@ -228,12 +237,21 @@ int append(const at::Tensor& k, const Opt& v, const at::Tensor& k_cache, const O
   if (B == 0 || S == 0) return BS_OK;
   const int64_t e = 16 / k.element_size();
   const at::Tensor kc = strided(k, e, 16), vc = v ? strided(*v, e, 16) : at::Tensor();
-  return p_cache_append(kc.const_data_ptr(), v ? vc.const_data_ptr() : nullptr, tag(k.scalar_type()), B, S,
-                        fits_int(name, Hkv), fits_int(name, D), kc.strides().data(), v ? vc.strides().data() : nullptr,
-                        k_cache.mutable_data_ptr(), v ? v_cache->mutable_data_ptr() : nullptr,
-                        (float*)k_scale.mutable_data_ptr(), v ? (float*)v_scale->mutable_data_ptr() : nullptr,
-                        k_cache.size(0), fits_int(name, k_cache.size(2)), (const int*)bt.const_data_ptr(), bt.size(1),
-                        (const int*)st.const_data_ptr(), new_lens ? (const int*)nl.const_data_ptr() : nullptr, on.stream);
+  const int status = p_cache_append(kc.const_data_ptr(), v ? vc.const_data_ptr() : nullptr, tag(k.scalar_type()), B, S,
+                                   fits_int(name, Hkv), fits_int(name, D), kc.strides().data(), v ? vc.strides().data() : nullptr,
+                                   k_cache.mutable_data_ptr(), v ? v_cache->mutable_data_ptr() : nullptr,
+                                   (float*)k_scale.mutable_data_ptr(), v ? (float*)v_scale->mutable_data_ptr() : nullptr,
+                                   k_cache.size(0), fits_int(name, k_cache.size(2)), (const int*)bt.const_data_ptr(), bt.size(1),
+                                   (const int*)st.const_data_ptr(), new_lens ? (const int*)nl.const_data_ptr() : nullptr, on.stream);
+  if (status == BS_OK) {
+    changed(k_cache);
+    changed(k_scale);
+    if (v) {
+      changed(*v_cache);
+      changed(*v_scale);
+    }
+  }
+  return status;
 }
 
 py::tuple attn(const at::Tensor& q, const at::Tensor& k_cache, const Opt& v_cache, const at::Tensor& k_scale, const Opt& v_scale,

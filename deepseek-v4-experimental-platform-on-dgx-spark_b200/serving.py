@@ -12,6 +12,11 @@ synchronise, and can be captured into CUDA graphs.  What only the device
 knows (page indices, lengths, positions) is checked there: a page index or
 length out of range reads and writes nothing, and ``device_error_check``
 reports it.
+
+No operator here records a graph for autograd: results are detached from
+inputs that require a gradient.  ``rope(..., inplace=True)`` refuses an x that
+does while gradients are recorded; it and ``cache_append`` count as in-place
+changes of the tensors that they write.
 """
 
 from __future__ import annotations

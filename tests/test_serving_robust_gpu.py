@@ -244,3 +244,37 @@ def test_cache_append_onto_bad_scale(pkg, dt, bad):
     for codes, scale, want in ((k_cache, ks, wk), (v_cache, vs, wv)):
         assert same_codes(codes, want[0]) and torch.equal(scale.double().nan_to_num(-1.0, -2.0), want[1].nan_to_num(-1.0, -2.0))
     assert torch.isfinite(vs[table[1, 1].long()]).all()
+
+
+# ------------------------------------------------------------------ autograd around the in-place operators
+
+def test_in_place_changes_are_seen(pkg):
+    """Tensors saved for a backward pass and then written here are noticed, as after torch's own in-place operators; an
+    in-place turn of something that needs its gradient is refused; inference tensors and recording turned off are fine."""
+    g = gen(5)
+    f, pos = pkg.rope_freqs(64), torch.arange(4, device="cuda")
+    x, w = randn(g, 4, 2, 64), randn(g, 4, 2, 64).requires_grad_()
+    loss = (x * w).sum()
+    pkg.rope(x, pos, f, inplace=True)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    y = w * 2
+    for t in (w, y):
+        was = t.detach().clone()
+        with pytest.raises(ValueError, match="gradient"):
+            pkg.rope(t, pos, f, inplace=True)
+        assert torch.equal(t, was)
+    with torch.no_grad():
+        assert torch.equal(pkg.rope(y, pos, f, inplace=True), pkg.rope(w * 2, pos, f))
+    assert not pkg.rope(w, pos, f).requires_grad
+    table, n = make_table(g, [20], 16)
+    cache = make_cache(g, n, 2, 16, 64)
+    k = randn(g, 1, 3, 2, 64, dtype=torch.bfloat16)
+    before = [t._version for t in cache]
+    pkg.cache_append(k, k, cache[0], cache[1], cache[2], cache[3], table, torch.tensor([7], dtype=torch.int32, device="cuda"))
+    assert all(t._version > b for t, b in zip(cache, before))
+    with torch.inference_mode():
+        c, s = cache[0].clone(), cache[2].clone()
+        z = x.clone()
+    pkg.cache_append(k, None, c, None, s, None, table, torch.tensor([0], dtype=torch.int32, device="cuda"))
+    pkg.rope(z, pos, f, inplace=True)
