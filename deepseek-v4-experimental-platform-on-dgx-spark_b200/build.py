@@ -3,6 +3,9 @@ operators (csrc/bind.cpp, against torch's C++ headers) into ``_native.so``.
 
     python <package dir>/build.py            # writes both into <package dir>
 
+The library comes first and needs nvcc alone; where torch or a C++ compiler is missing the host path is left out,
+with a message.
+
 nvcc cross-compiles without a GPU.  No ``--use_fast_math``: the quantisers
 rely on IEEE division and RNE conversions to match the reference bit for bit.
 """
@@ -62,7 +65,15 @@ def build_native(force: bool = False) -> str:
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
-    build_native(force)
+    build_library(force, verbose)
+    try:
+        build_native(force)
+    except (ImportError, FileNotFoundError) as e:       # no torch, no compiler: callers of the C ABI need neither
+        print(f"{BIND_OUT} not built, the serving operators of the Python package need it: {e}", file=sys.stderr)
+    return OUT
+
+
+def build_library(force: bool = False, verbose: bool = False) -> str:
     if not force and up_to_date():
         return OUT
     cmd = [nvcc(), "-O3", "-std=c++17", "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo",
