@@ -40,9 +40,27 @@ def up_to_date(out: str = OUT, deps=None) -> bool:
     return all(os.path.getmtime(d) <= t for d in (DEPS if deps is None else deps) if os.path.exists(d))
 
 
+def native_versions() -> str:
+    """What the host path's binary interface depends on."""
+    import sysconfig
+
+    import torch
+
+    return f"torch {torch.__version__} cxx11_abi {int(torch._C._GLIBCXX_USE_CXX11_ABI)} python {sysconfig.get_config_var('SOABI')}"
+
+
+def native_up_to_date() -> bool:
+    """Newer than its sources, and built for the torch and Python at hand (kept beside it, in _native.stamp)."""
+    try:
+        with open(BIND_OUT[:-3] + ".stamp") as f:
+            return f.read() == native_versions() and up_to_date(BIND_OUT, [BIND_SRC, DEPS[-1]])
+    except FileNotFoundError:
+        return False
+
+
 def build_native(force: bool = False) -> str:
     """The host path: plain C++ against torch and the C ABI's header, no CUDA code."""
-    if not force and up_to_date(BIND_OUT, [BIND_SRC, DEPS[-1]]):
+    if not force and native_up_to_date():
         return BIND_OUT
     import sysconfig
 
@@ -61,6 +79,8 @@ def build_native(force: bool = False) -> str:
     if r.returncode != 0:
         raise RuntimeError(f"g++ failed ({r.returncode}):\n{r.stdout}\n{r.stderr}")
     os.replace(BIND_OUT + ".tmp", BIND_OUT)
+    with open(BIND_OUT[:-3] + ".stamp", "w") as f:
+        f.write(native_versions())
     return BIND_OUT
 
 

@@ -54,3 +54,14 @@ def test_compile_error_is_raised(b, calls, monkeypatch):
     with pytest.raises(RuntimeError, match="failed"):
         b.build(force=True)
     assert calls == ["nvcc"]
+
+
+def test_host_path_follows_torch(b, calls, monkeypatch):
+    """Another torch or Python than the one it was built for builds the host path again; the same one does not."""
+    b.build_native()
+    b.build_native()
+    assert calls == ["g++"]
+    monkeypatch.setattr(b, "native_versions", lambda: "torch 9.9.9 cxx11_abi 1 python cpython-399")
+    b.build_native()
+    b.build_native()
+    assert calls == ["g++", "g++"]
