@@ -278,3 +278,31 @@ def test_in_place_changes_are_seen(pkg):
         z = x.clone()
     pkg.cache_append(k, None, c, None, s, None, table, torch.tensor([0], dtype=torch.int32, device="cuda"))
     pkg.rope(z, pos, f, inplace=True)
+
+
+@pytest.mark.parametrize("H,D,dt,S", [(4, 128, "bf16", 25), (8, 64, "f16", 9), (2, 512, "bf16", 25), (32, 128, "bf16", 3)])
+def test_cache_attn_spread_scales_with_nan(pkg, H, D, dt, S):
+    """Very different value scales, one of them zero and one NaN, on pages that some rows see: NaN reaches those rows alone."""
+    g = gen(H + D)
+    n, page, i = 150, 16, 144
+    table, n_pages = make_table(g, [n], page)
+    k, v, ks, vs = make_cache(g, n_pages, 1, page, D)
+    vs.copy_(torch.exp2(torch.randint(-22, 4, vs.shape, generator=g, device="cuda").float()))
+    vs[table[0, 8].long()] = 0.0
+    q = randn(g, 1, S, H, D, dtype=DT[dt])
+    want, tol = precise_tolerance(q, (k, v, ks, vs), table, n, D ** -0.5, [n - S + j + 1 for j in range(S)])
+    vs[table[0, i // page].long()] = float("nan")
+    got = pkg.cache_attn(q, k, v, ks, vs, table, torch.tensor([n], dtype=torch.int32, device="cuda"), D ** -0.5)[0].double()
+    sees = n - S + 1 + torch.arange(S, device="cuda") > i
+    assert got[sees].isnan().all() and ((got - want).abs() <= tol)[~sees].all()
+
+
+@pytest.mark.parametrize("scale", [1.7 * 2.0 ** -100, 1.3 * 2.0 ** 90])
+@pytest.mark.parametrize("n,B", [(300, 1), (9000, 40)])
+def test_cache_attn_value_scales_far_from_one(pkg, scale, n, B):
+    """Results of any size that bf16 holds."""
+    g = gen(n)
+    table, n_pages = make_table(g, [n], 64)
+    k, v, ks, vs = make_cache(g, n_pages, 1, 64, 128)
+    vs.mul_(scale * 2.0 ** 8)
+    assert_precise(pkg, 2 * randn(g, 1, 2, 4, 128, dtype=torch.bfloat16), (k, v, ks, vs), table, n, 128 ** -0.5, B)
