@@ -161,9 +161,8 @@ struct Info {                       // one tile, from the producer
   int t0;                           // first token
   int limit;                        // tokens that any row sees
   int first, last;                  // of its segment
-  int mask;                         // some row does not see all of the tile, or spread
-  uint16_t nan;                     // bits of the pages whose value scale is NaN
-  uint16_t spread;                  // value scales (other than 0) differ by more than kSpread
+  int mask;                         // 1: some row does not see all of the tile; 2: value scales (not 0) kSpread apart
+  int nan;                          // bits of the pages whose value scale is NaN
 };
 
 __host__ __device__ constexpr int softmax_groups(int R) { return R >= 32 ? R / 16 : 1; }
@@ -672,7 +671,7 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
           // a NaN scale makes its page's weights NaN where every row sees the tile; else they are 0, and the softmax
           // warps note the page's tokens as NaN values
           const bool spread = __any_sync(0xffffffffu, vs != 0.0f && fabsf(vs) * kSpread < unit);
-          const bool mask = (cur.t + k + 1) * kTok > cur.low || valid != (1u << ppt) - 1u || spread;
+          const bool mask = (cur.t + k + 1) * kTok > cur.low || valid != (1u << ppt) - 1u;
           const uint32_t nan = __ballot_sync(0xffffffffu, vs != vs) & ((1u << ppt) - 1u);
           if (lane < 8) {
             in.ks[lane] = ks;
@@ -686,9 +685,8 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
             in.limit = cur.limit;
             in.first = cur.first && k == 0;
             in.last = cur.last && k + 1 == cur.n;
-            in.mask = mask;
-            in.nan = (uint16_t)nan;
-            in.spread = spread;
+            in.mask = (mask ? 1 : 0) | (spread ? 2 : 0);
+            in.nan = (int)nan;
           }
           __syncwarp();
           k_chunks(prow);
@@ -759,7 +757,7 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
         const uint32_t at = i * NC + min(lane, NC - 1);
         if (!warp_wait(&T.full[v_slot(at)], v_par(at), lane < NC, abort_flag)) break;
         // the softmax warps look the values of a partly hidden tile over before they hand in its weights
-        if (lane == 0 && T.info[i % kInfo].mask) mbar_arrive(&T.v_ready);
+        if (lane == 0 && (T.info[i % kInfo].mask & 1)) mbar_arrive(&T.v_ready);
         __syncwarp();
         if (!warp_wait(lane ? &T.o_empty[ob] : &T.p_full[pb], lane ? ((i / C::OB) & 1) ^ 1 : (i >> 1) & 1, lane < 2, abort_flag))
           break;
@@ -863,7 +861,7 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
             }
           }
           // (asked here, not for every tile: beside this choice the code of all tiles came out 12 % slower)
-          if (in.spread) {           // of score and the scale's logarithm (x is multiplied by qf afterwards)
+          if (in.mask & 2) {         // of score and the scale's logarithm (x is multiplied by qf afterwards)
             float lv[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k)
@@ -937,7 +935,7 @@ __global__ void __launch_bounds__(Cfg<R, PP, NC>::kThreads, Cfg<R, PP, NC>::kCta
           }
         }
       }
-      if (in.mask && wg == 0) {
+      if ((in.mask & 1) && wg == 0) {
         // Values that some row must not see: 0 x NaN would reach its sum.  Rows that no query sees become zero; a NaN
         // in a row that only some see becomes zero too, and is put back for those when the segment ends.
         const int tok = quad * 32 + lane, t = in.t0 + tok;
