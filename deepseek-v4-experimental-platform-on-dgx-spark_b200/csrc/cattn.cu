@@ -47,12 +47,14 @@
 // joins them.  Lengths are read on the device only.
 //
 // What bounds it: few rows, HBM (64 sequences of up to 16384 tokens, 8 kv heads
-// of 128, 8 query heads each: 1.09 GB of codes in 180 us, 0.92 of the copy
-// bandwidth; 200000 tokens f16, 3 terms: 76 us, 0.83); 64 rows a tile, the
-// instructions of the softmax (a chunk of 512 tokens on 8192: 290 us, issue
-// slots 65 % busy, 22 instructions a score); a latent of 512 dims with 64
-// heads, the chain copy - S - softmax - O of a ring of two and a half tiles
-// (48 sequences of up to 8192: 82 us, 314 TFLOP/s).
+// of 128, 8 query heads each: 1.09 GB of codes in 186 to 192 us, 0.87 to 0.90 of
+// the copy bandwidth; 200000 tokens f16, 3 terms: 77 to 79 us, 0.80 to 0.82); 64
+// rows a tile, the instructions of the softmax (a chunk of 512 tokens on 8192:
+// 291 us, issue slots 65 % busy, 32 instructions a score); a latent of 512 dims
+// with 64 heads, the chain copy - S - softmax - O of a ring of two and a half
+// tiles, each fetched twice, as its 64 rows take two row tiles (48 sequences of
+// up to 8192: 85 us, 304 TFLOP/s).  Tiles of spread scales on every page: 187,
+// 77, 338 and 87 us.
 //
 // Roles: one warpgroup with the TMA producer and an issuer for each of the two
 // products; one softmax warpgroup, or from 32 rows on one for every 16 of them;
@@ -177,7 +179,7 @@ struct Cfg {
   static constexpr int kPBytes = N * kTok;
   static constexpr int QB = kQBytes >= 32768 ? 1 : 2;              // Q buffers
   // Places before a head's tiles on the line of work, for staging its rows, draining the pipeline and writing its
-  // results.  Measured with 0 to 8: 1 is best for 64 ragged sequences of 8 rows a head (182 us; 0: 184, 2: 183), 4 to 6
+  // results.  Measured with 0 to 8: 1 is best for 64 ragged sequences of 8 rows a head (182 us then; 0: 184, 2: 183), 4 to 6
   // for a chunk of 512 tokens (301 us then; 2: 333, 8: 305), 6 to 8 with one Q buffer (latent: 89 us then; 2: 97).
   static constexpr int kSegCost = QB == 1 ? 7 : WG > 1 ? 5 : 1;
   static constexpr int OB = 2 * N + 2 * NC * N <= 512 ? 2 : 1;     // O buffers

@@ -27,7 +27,8 @@
 //             bulk copies in a ring of shared-memory buffers, so that loads go
 //             on through the reduction and the stores of the row at hand; the
 //             weight stays in registers.  16384 x 7168 bf16 with residual and
-//             codes: 144 us against 192 (0.88 of the copy bandwidth).
+//             codes: 146 to 155 us (0.82 to 0.87 of the copy bandwidth; 142 in a
+//             graph) against 192.
 #include "common.cuh"
 
 namespace rmsn {

@@ -158,7 +158,7 @@ cudaError_t bs_launch_rope(rope::Args a, int dtype, int half, cudaStream_t st) {
   // Tasks of a CTA: two per thread in the half layout (two vectors each), one in the interleaved one, of as many whole
   // tokens as that is (their cos/sin pairs have to fit) or of part of a token's heads; fewer when the CTAs would not
   // fill the GPU a few times.  More per thread costs registers, and with them loads in flight: 8192 tokens x 40 heads x
-  // 128 bf16 take 30 us half (1: 41, 3: 42) and 43 us interleaved (2: 52, 4: 63); 64 tokens x 64 heads x 512 with 64
+  // 128 bf16 take 30 us half (1: 41, 3: 42) and 43 to 46 us interleaved (2: 52, 4: 63); 64 tokens x 64 heads x 512 with 64
   // dims turned 2.9 us (2: 3.4, 4: 4.7).
   const int want = half ? 2 * rope::kThreads : rope::kThreads;
   const int64_t per_token = (int64_t)per_head * a.H;

@@ -189,6 +189,11 @@ def cache_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: Optional[torch.T
     [B, S, H, D] in q's type; rows that see nothing, and padded query tokens,
     are zero.  Infinities and NaN in slots that a row does not see do not reach
     it.
+
+    Softmax weights enter the product with the values rounded to about the
+    result's type (2^-8 of a weight at most with bf16, 2^-12 with f16).  Among
+    the 128 tokens of a tile, those that count less than 2^-20 (f16: 2^-24) of
+    the largest one may be lost; what they weigh in the denominator stays.
     """
     t0 = _time.perf_counter()
     status, out = (_mod or _native()).attn(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, softmax_scale,

@@ -416,7 +416,9 @@ int bs_cache_append(const void* k, const void* v, int dtype, int64_t B, int64_t 
  * attn_sink fp32 [H] or NULL: a logit per head that takes softmax weight and
  * adds no value.  A row that sees nothing is zero, padded query tokens too.
  * Softmax statistics and sums in fp32; weights and queries enter the tensor
- * cores as sums of two (bf16) or three (f16) e4m3 terms.  Results do not
+ * cores as sums of two (bf16) or three (f16) e4m3 terms: a weight is off by
+ * 2^-8 or 2^-12 of itself, or by 2^-20 or 2^-24 of its row's largest product of
+ * weight and value scale among the 128 tokens of its tile.  Results do not
  * depend on any order of execution.  A page index or length out of range
  * reads as absent and is reported by bs_device_error_check().
  * The workspace may be reused once the call's work is done; calls that may
