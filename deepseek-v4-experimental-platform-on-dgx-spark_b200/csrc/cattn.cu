@@ -43,7 +43,7 @@
 // the call lie in one line, every head's preceded by what its start and end
 // cost (in tiles), and each resident CTA takes an equal stretch of the line,
 // whatever the lengths; where a stretch ends inside a head's tokens, both
-// sides leave partial results (unnormalised O, max, sum) and a second kernel
+// sides leave partial results (unnormalised O, reference, sum) and a second kernel
 // joins them.  Lengths are read on the device only.
 //
 // What bounds it: few rows, HBM (64 sequences of up to 16384 tokens, 8 kv heads
